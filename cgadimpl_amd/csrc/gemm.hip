@@ -13,7 +13,7 @@
 // stored h would be; rowscale multiplies the fp32 accumulator.)
 //
 // Three kernels.  A product without a k-scale runs on the direct-to-LDS kernel
-// further below (256 x 256 tiles, whole 128-byte lines of either operand layout
+// of gemm_direct.hpp (256 x 256 tiles, whole 128-byte lines of either operand layout
 // staged through two 64-deep LDS stages without registers) or, where those tiles
 // would leave CUs idle, on the ring kernel of gemm_ring.hpp (smaller tiles, more
 // bytes in flight); pick_shape chooses.  A k-scale, or a leading dimension too
@@ -49,17 +49,14 @@
 
 #include "agk_rmsnorm.h"
 #include "gemm_common.hpp"
+#include "gemm_direct.hpp"
 #include "gemm_ring.hpp"
 #include "rowcommon.hpp"
 
 namespace agk_gemm {
 
-constexpr int BM = 256, BN = 256;
 constexpr int kThreads = 512;
 constexpr int kWavesN = 4;
-constexpr int WM = 128, WN = 64;            // per-wave tile
-constexpr int TM = WM / 32, TN = WN / 32;   // MFMA tiles per wave
-constexpr int kStageElems = (BM + BN) * kStride;
 
 // ---- operand staging --------------------------------------------------------
 // An operand tile is R = 256 rows (of A: m, of B: n) by BK = 64 k.
@@ -267,304 +264,7 @@ __global__ __launch_bounds__(kThreads) void gemm_bf16_kernel(
 }
 
 // ---- direct-to-LDS kernel -----------------------------------------------------
-// Staging without registers: buffer_load_dwordx4 ... lds writes lane l's 16
-// bytes to LDS at (wave-uniform base) + 16 * l, so one wave instruction fills
-// a contiguous kilobyte of LDS; each lane fetches the global chunk that belongs
-// at its position of the swizzled layout.  Rows past M or N are fetched from
-// the last valid row (never stored).  The epilogue store_block writes the wave's
-// block of C.  K % 64 k at the end of K are staged through registers with
-// zeros past K (stage_k_tail) and multiplied before the whole k-tiles.
-//
-// The same 256 x 256 tile, over 4 waves of 128 x 128 (2 x 2; 4 x 4 MFMA tiles
-// per wave, whose 256 accumulator registers live in AGPRs).  K is walked in
-// 64-deep tiles through two LDS stages of 64 KiB (32 KiB per operand), filled by
-// `buffer_load_dwordx4 ... lds`, so staging takes no registers.  Each operand is
-// staged in the layout it has in memory:
-// - k-contiguous ([rows][K]): 256 LDS rows of 64 k (128 bytes, 8 XOR-swizzled
-//   16-byte chunks: lds_off above); a fragment is one 16-byte read.
-// - k-strided (TR; [K][cols], the columns contiguous): 64 LDS rows of one k
-//   each, 256 columns (512 bytes, 32 chunks whose 64-byte groups are XOR-
-//   swizzled by k % 4: tr_off); a fragment is two ds_read_b64_tr_b16.  Within
-//   each 16 lanes that instruction hands lane 4a + b, for e = 0..3, the element
-//   at offset b from the address of lane 4e + a (checked on MI355X), so lane s
-//   pointing at k0 + s / 4, column c0 + 4 (s % 4) gives lane j the four k
-//   k0 .. k0 + 3 of column c0 + j: the MFMA operand layout.  No transposed copy
-//   of the operand is made.
-// Either way one load instruction moves 1 KiB of whole 128-byte lines, and the
-// LDS destination of load j of wave w is the same kilobyte.
-//
-// Why this shape (measured on MI355X, c5 products):
-// - Whole 128-byte rows per load: 32-deep tiles (64 bytes per row) asked L2 for
-//   each line twice, half at a time, and the L1's queue of pending misses, not
-//   HBM, set the pace (twice hipBLASLt's L2 request count for the same bytes,
-//   TCP_TCC_READ_REQ).
-// - One wave per SIMD with a 128 x 128 block reads a third fewer LDS bytes per
-//   MFMA than two waves of 128 x 64, and its stream of 64 MFMAs per tile has
-//   the loads and fragment reads interleaved between them; it was 4-6 % faster
-//   than eight waves of 128 x 64 with the same stages.
-//
-// Schedule of tile t (after the barrier that makes tile t visible and frees the
-// other stage): the 16 loads of tile t + 1 go into the other stage, one per
-// two MFMAs of the first two substeps; the fragments run one 16-deep substep
-// ahead of the MFMAs, so the substep that straddles the barrier (the last of
-// tile t - 1) multiplies while tile t's first fragments are read.  At the end
-// of the tile each wave waits for its own loads and reads, then the barrier.
-constexpr int kDirectThreads = 256;
-constexpr int kTrRow = 256;               // bf16 per LDS row of a k-strided operand
-
-// Element offset of column col (a multiple of 4) of k-row k in a k-strided stage.
-__device__ __forceinline__ int tr_off(int k, int col) {
-    return k * kTrRow + ((((col >> 3) ^ ((k & 3) << 2))) << 3) + (col & 7);
-}
-
-struct DirectStage {
-    __amdgpu_buffer_rsrc_t ra, rb;  // the tile's A and B (base and size in SGPRs)
-    uint32_t oa[8], ob[8];          // byte offset of each lane's chunk, per load
-    int step_a, step_b;             // bytes from one 64-deep k-tile to the next
-};
-
-// Load j of a wave (j = 0..7) fills kilobyte wave * 8 + j of one operand's half
-// of `stage`; tile t's data starts t * step bytes into the operand.
-__device__ __forceinline__ void direct_issue_a(const DirectStage& d, uint16_t* stage, int t,
-                                               int wave) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(d.ra, (lds_ptr_t)(stage + (wave * 8 + j) * 512),
-                                                 16, d.oa[j], t * d.step_a, 0, 0);
-}
-__device__ __forceinline__ void direct_issue_b(const DirectStage& d, uint16_t* stage, int t,
-                                               int wave) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            d.rb, (lds_ptr_t)(stage + BM * BK + (wave * 8 + j) * 512), 16, d.ob[j], t * d.step_b,
-            0, 0);
-}
-
-// Per-lane byte offsets of one operand's loads.  rows: valid rows (k-contiguous)
-// or columns (k-strided) of the tile; ld: leading dimension in elements.
-template <bool TR>
-__device__ __forceinline__ void direct_offsets(uint32_t (&o)[8], int wave, int lane, int rows,
-                                               int64_t ld) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if constexpr (!TR) {
-            const int row = wave * 64 + j * 8 + (lane >> 3);
-            const int c = (lane & 7) ^ (row & 7) ^ ((row >> 3) & 7);  // chunk of slot lane % 8
-            const int r = row < rows ? row : rows - 1;  // rows past M or N: the last valid row
-            o[j] = (static_cast<uint32_t>(r) * static_cast<uint32_t>(ld) + c * 8) * 2;
-        } else {
-            const int k = wave * 16 + j * 2 + (lane >> 5);
-            const int c = (lane & 31) ^ ((k & 3) << 2);  // chunk of slot lane % 32
-            const int col = c * 8 < rows ? c * 8 : rows - 8;  // columns past M or N: the last 8
-            o[j] = (static_cast<uint32_t>(k) * static_cast<uint32_t>(ld) + col) * 2;
-        }
-    }
-}
-
-// The fragments of one 16-deep substep s (0..3) of a wave: 4 of A (128 rows),
-// NB of B (32 NB columns: 4 for the 256 x 256 tile, 2 for the 256 x 128 half
-// tiles of a last round).
-template <int NB>
-struct Frags {
-    bf16x8 a[TM], b[NB];
-};
-
-// MFMA operand lane l (row or column l % 32, k 8 (l / 32) .. + 7) of block
-// column base c0, substep s, from a k-strided stage: two transposing reads of
-// four k each.
-__device__ __forceinline__ bf16x8 tr_frag(const uint16_t* lds, int c0, int s, int lane) {
-    const int g = lane >> 4, sl = lane & 15;
-    const int k = s * 16 + (g >> 1) * 8 + (sl >> 2);
-    const int col = c0 + (g & 1) * 16 + 4 * (sl & 3);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(lds + tr_off(k, col)));
-    const s16x4 hi =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(lds + tr_off(k + 4, col)));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// bc: the wave's first B column within the stage.
-template <bool A_TR, bool B_TR, int NB>
-__device__ __forceinline__ void read_frags(Frags<NB>& f, const uint16_t* stage, int s, int wm,
-                                           int bc, int frow, int fk, int lane) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        if constexpr (A_TR) f.a[i] = tr_frag(stage, wm * WM + i * 32, s, lane);
-        else f.a[i] = lds_frag(stage, wm * WM + i * 32 + frow, s * 16 + fk);
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        if constexpr (B_TR) f.b[j] = tr_frag(stage + BM * BK, bc + j * 32, s, lane);
-        else f.b[j] = lds_frag(stage + BM * kStride, bc + j * 32 + frow, s * 16 + fk);
-    }
-}
-
-template <int NB>
-__device__ __forceinline__ void mfma_sub(const Frags<NB>& f, f32x16 (&acc)[TM][NB]) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
-}
-
-// Scheduling groups: one load, one fragment read, two MFMAs (AGK_LRM); one
-// fragment read, two MFMAs (AGK_RM).  Eight of them cover a substep's 16 MFMAs.
-#define AGK_LRM                                         \
-    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); \
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); \
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-#define AGK_RM                                          \
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); \
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-#define AGK_X8(g) g g g g g g g g
-
-// Tile t of nk.  FIRST (tile 0) has no straddling substep; every step loads
-// tile t + 1 (the last tile again at the end, into the stage nothing reads
-// again).  Entering, f1 holds substep 3 of tile t - 1.  NB = 4: the 256 x 256
-// tile, whose substeps interleave one load, one fragment read and two MFMAs;
-// NB = 2 (half tiles): the same loads and reads around half the MFMAs, left to
-// the compiler's schedule.
-#define AGK_SUBSTEP_LRM    \
-    if constexpr (NB == 4) { \
-        AGK_X8(AGK_LRM)    \
-    }
-#define AGK_SUBSTEP_RM     \
-    if constexpr (NB == 4) { \
-        AGK_X8(AGK_RM)     \
-    }
-template <bool FIRST, bool A_TR, bool B_TR, int NB>
-__device__ __forceinline__ void direct_step(const DirectStage& d, const uint16_t* cur,
-                                            uint16_t* other, int t, int nk,
-                                            f32x16 (&acc)[TM][NB], Frags<NB>& f0, Frags<NB>& f1,
-                                            int wm, int bc, int frow, int fk, int lane,
-                                            int wave) {
-    const int tn = t + 1 < nk ? t + 1 : nk - 1;
-    direct_issue_a(d, other, tn, wave);
-    read_frags<A_TR, B_TR>(f0, cur, 0, wm, bc, frow, fk, lane);
-    if constexpr (!FIRST) {
-        mfma_sub(f1, acc);
-        AGK_SUBSTEP_LRM
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    direct_issue_b(d, other, tn, wave);
-    read_frags<A_TR, B_TR>(f1, cur, 1, wm, bc, frow, fk, lane);
-    mfma_sub(f0, acc);
-    AGK_SUBSTEP_LRM
-    __builtin_amdgcn_sched_barrier(0);
-    read_frags<A_TR, B_TR>(f0, cur, 2, wm, bc, frow, fk, lane);
-    mfma_sub(f1, acc);
-    AGK_SUBSTEP_RM
-    __builtin_amdgcn_sched_barrier(0);
-    read_frags<A_TR, B_TR>(f1, cur, 3, wm, bc, frow, fk, lane);
-    mfma_sub(f0, acc);
-    AGK_SUBSTEP_RM
-    __builtin_amdgcn_sched_barrier(0);
-    // This wave's loads of tile t + 1 have landed and its reads of tile t are
-    // done; after the barrier every wave's are.  A bare barrier:
-    // __syncthreads()'s fence adds nothing here (vmcnt and lgkmcnt are zero).
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-// Stores columns [64 H, 64 H + 64) of a wave's 128 x 128 block, whose first column
-// is col0 of C.  H is a template argument, not a loop's: a loop over the halves is
-// too large for the compiler to unroll, and acc, indexed by a variable, moves to
-// scratch memory.
-template <bool OUT_F32, Stores S, int H>
-__device__ __forceinline__ void store_half(const f32x16 (&acc)[TM][2 * TN], void* __restrict__ C,
-                                           int64_t ldc, int M, int N, int row0, int col0,
-                                           int lane, const float* __restrict__ rowscale,
-                                           const uint16_t* __restrict__ colbias, int accumulate) {
-    f32x16 part[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) part[i][j] = acc[i][H * TN + j];
-    store_block<OUT_F32, S>(part, C, ldc, M, N, row0, col0, lane, rowscale, colbias, accumulate);
-}
-
-// One tile's k loop and store.  NB = 4: the 256 x 256 tile at (m0, n0), wave
-// (wm, wn) owning its 128 x 128 block; NB = 2: the 256 x 128 half of that tile
-// starting at column n0 + half_off, wave (wm, wn) owning a 128 x 64 block.
-// Both stage the tile's full 256 B columns (the same loads).  TAIL: K is not a
-// multiple of 64; the last K % 64 k are multiplied first, staged through
-// registers into st1 (which tile 1's loads fill only after it).
-template <bool OUT_F32, bool A_TR, bool B_TR, int NB, bool TAIL, Stores S>
-__device__ __forceinline__ void direct_tile(const DirectStage& d, uint16_t* st0, uint16_t* st1,
-                                            const uint16_t* __restrict__ a0, int64_t lda,
-                                            int rows_a, const uint16_t* __restrict__ b0,
-                                            int64_t ldb, int rows_b, void* __restrict__ C, int64_t ldc, int M, int N,
-                                            int K, int m0, int n0, int half_off, int wm, int wn,
-                                            int lane, int wave,
-                                            const float* __restrict__ rowscale,
-                                            const uint16_t* __restrict__ colbias,
-                                            int accumulate) {
-    f32x16 acc[TM][NB];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-
-    const int nk = K / BK;  // >= 1
-    const int frow = lane & 31;
-    const int fk = (lane >> 5) * 8;  // MFMA operand lanes 32..63 hold k 8..15
-    const int bc = half_off + wn * (NB * 32);  // the wave's first B column in the stage
-    if constexpr (TAIL) {
-        stage_k_tail<A_TR, BM>(st1, a0, lda, rows_a, nk * BK, K);
-        stage_k_tail<B_TR, BN>(st1 + BM * BK, b0, ldb, rows_b, nk * BK, K);
-    }
-    direct_issue_a(d, st0, 0, wave);
-    direct_issue_b(d, st0, 0, wave);
-    if constexpr (TAIL) {
-        stage_barrier<16>();  // the tail's LDS writes, every wave (tile 0 still in flight)
-        for (int s = 0; s * 16 < K - nk * BK; ++s) {
-            Frags<NB> f;
-            read_frags<A_TR, B_TR>(f, st1, s, wm, bc, frow, fk, lane);
-            mfma_sub(f, acc);
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    Frags<NB> f0, f1;
-    direct_step<true, A_TR, B_TR>(d, st0, st1, 0, nk, acc, f0, f1, wm, bc, frow, fk, lane, wave);
-    int t = 1;
-    for (; t + 1 < nk; t += 2) {
-        direct_step<false, A_TR, B_TR>(d, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
-                                       wave);
-        direct_step<false, A_TR, B_TR>(d, st0, st1, t + 1, nk, acc, f0, f1, wm, bc, frow, fk,
-                                       lane, wave);
-    }
-    if (t < nk)
-        direct_step<false, A_TR, B_TR>(d, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
-                                       wave);
-    mfma_sub(f1, acc);  // substep 3 of the last tile
-
-    if constexpr (NB == 4) {
-        // the wave's 128 x 128 block leaves as two 128 x 64 halves
-        store_half<OUT_F32, S, 0>(acc, C, ldc, M, N, m0 + wm * WM, n0 + 2 * wn * WN, lane, rowscale,
-                               colbias, accumulate);
-        store_half<OUT_F32, S, 1>(acc, C, ldc, M, N, m0 + wm * WM, n0 + (2 * wn + 1) * WN, lane,
-                               rowscale, colbias, accumulate);
-    } else {
-        store_block<OUT_F32, S>(acc, C, ldc, M, N, m0 + wm * WM, n0 + half_off + wn * WN, lane,
-                                rowscale, colbias, accumulate);
-    }
-}
-
-// A_TR: A stored [K][lda] (its m contiguous); B_TR: B stored [K][ldb] (its n
-// contiguous).  Otherwise the operand is [rows][ld] with k contiguous.
-// Workgroups below full_tiles compute whole 256 x 256 tiles (tile_of's order);
-// the ones after them split each remaining tile into two 256 x 128 halves
-// (workgroup full_tiles + 2 h + q: half q of tile full_tiles + h), so that a
-// last round of few tiles runs on twice as many CUs for half as long.  Every
-// output element is summed in the same k order either way (bit-identical).
+// gemm_direct.hpp's, storing C.
 template <bool OUT_F32, bool A_TR, bool B_TR, bool TAIL, Stores S>
 __global__ __launch_bounds__(kDirectThreads) void gemm_nt_direct_kernel(
     const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb,
@@ -574,49 +274,9 @@ __global__ __launch_bounds__(kDirectThreads) void gemm_nt_direct_kernel(
     __shared__ __attribute__((aligned(16))) uint16_t st0[kStageElems];
     __shared__ __attribute__((aligned(16))) uint16_t st1[kStageElems];
 
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
-    // wave-uniform, so kept in scalar registers (LDS destinations of the loads)
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1;
-    const int wn = wave & 1;
-    const int L = static_cast<int>(blockIdx.x);
-    const bool halves = L >= full_tiles;
-    const int tile = halves ? full_tiles + ((L - full_tiles) >> 1) : L;
-    int tm, tn;
-    tile_of(tile, tiles_m, tiles_n, group_m, tm, tn);
-    const int m0 = tm * BM;
-    const int n0 = tn * BN;
-
-    const int rows_a = M - m0 < BM ? M - m0 : BM;
-    const int rows_b = N - n0 < BN ? N - n0 : BN;
-    const uint16_t* a0 = A_TR ? A + m0 : A + static_cast<int64_t>(m0) * lda;
-    const uint16_t* b0 = B_TR ? B + n0 : B + static_cast<int64_t>(n0) * ldb;
-    DirectStage d;
-    // the resources span the bytes the tile's loads can address (their k
-    // position is the scalar offset, always inside the operand)
-    d.ra = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t*>(a0), static_cast<short>(0),
-        static_cast<int>(A_TR ? ((K - 1) * lda + rows_a) * 2 : ((rows_a - 1) * lda + K) * 2),
-        0x00020000);
-    d.rb = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t*>(b0), static_cast<short>(0),
-        static_cast<int>(B_TR ? ((K - 1) * ldb + rows_b) * 2 : ((rows_b - 1) * ldb + K) * 2),
-        0x00020000);
-    d.step_a = A_TR ? static_cast<int>(BK * lda * 2) : BK * 2;
-    d.step_b = B_TR ? static_cast<int>(BK * ldb * 2) : BK * 2;
-    direct_offsets<A_TR>(d.oa, wave, lane, rows_a, lda);
-    direct_offsets<B_TR>(d.ob, wave, lane, rows_b, ldb);
-
-    if (!halves)
-        direct_tile<OUT_F32, A_TR, B_TR, 4, TAIL, S>(d, st0, st1, a0, lda, rows_a, b0, ldb, rows_b,
-                                                  C, ldc, M, N, K, m0, n0, 0, wm, wn, lane, wave,
-                                                  rowscale, colbias, accumulate);
-    else
-        direct_tile<OUT_F32, A_TR, B_TR, 2, TAIL, S>(d, st0, st1, a0, lda, rows_a, b0, ldb, rows_b,
-                                                  C, ldc, M, N, K, m0, n0,
-                                                  ((L - full_tiles) & 1) * (BN / 2), wm, wn,
-                                                  lane, wave, rowscale, colbias, accumulate);
+    const StoreC<OUT_F32, S> epi{C, ldc, M, N, rowscale, colbias, accumulate};
+    direct_body<A_TR, B_TR, TAIL>(A, lda, B, ldb, M, N, K, tiles_m, tiles_n, group_m, full_tiles,
+                                  st0, st1, epi);
 }
 
 // C for an empty reduction (K == 0): zeros, or the bf16 column bias in every
@@ -696,14 +356,6 @@ inline int launch_transpose(const void* src, int64_t ld_src, void* dst, int64_t 
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// How many tiles the direct kernel computes whole: all of them, unless the
-// last round (tiles beyond a multiple of the CU count) would fill at most half
-// of the CUs; those tiles then run as two 256 x 128 halves each.
-inline int direct_full_tiles(int tiles, int cus) {
-    const int rem = tiles % cus;
-    return (rem != 0 && 2 * rem <= cus) ? tiles - rem : tiles;
-}
-
 template <bool AK, bool BK_, bool KS, bool F32>
 int launch(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int M,
            int N, int K, const float* kscale, const float* rowscale, const uint16_t* colbias,
@@ -768,57 +420,6 @@ int launch_direct(bool f32, const GemmCall& c) {
     }
 #undef AGK_DIRECT
     return hipGetLastError() == hipSuccess ? AGK_OK : AGK_EHIP;
-}
-
-// The kernel and tile a product runs on: 0 the direct kernel's 256 x 256
-// tiles, otherwise a ring shape.  The cost of a shape is its rounds of tiles
-// over the CUs times a k-step's time, which depends on how full the round is
-// (the loads of a full chip queue behind each other; the MFMAs of a full chip
-// lower the clock): light for a round of few workgroups, full for a full one,
-// light + (full - light) * fill^2 between.  The two times per shape were
-// measured on MI355X (random bf16, k-contiguous operands, K = 4096: 512 and
-// 8192 rows by 4096 columns).  What a round costs besides its k-steps is left out,
-// so K decides only below one k-tile.  Against every shape's time at 1179 products of
-// 64 to 8192 rows, 128 to 11008 columns and K of 64 to 4096, in the three layouts of a
-// layer's products (both k-contiguous, B strided, A and B strided with fp32 output), the
-// rule's shape takes 3.5 % more than the best one on average, and 21 % in one of twenty;
-// costs with a fixed part per round, fitted to them, came to 1.4 % and 9 % but were up to
-// 45 % slower at single sizes.
-//   rows x columns x K (us)   256x256  ring shape taken   other shapes
-//   512 x 4096 x 4096              58      22 (128x64)    22-42
-//   1032 x 4096 x 4096             65      39 (192x128)   39-73
-//   1032 x 4096 x 64               6.5     8.0 (192x128)  6.3-8.1
-//   2048 x 4096 x 4096             84      57 (128x256)   59-137
-//   4096 x 4096 x 1032             36      -              38-77
-//   8192 x 4096 x 4096            204      -              225-489
-// A shape whose workgroups are more than a grid holds is passed over (columns of
-// 8 by rows in the billions; the direct kernel has the largest tiles).
-inline int pick_shape(int64_t M, int64_t N, int64_t K, int cus) {
-    auto tiles_of = [&](const RingCost& s) {
-        return ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
-    };
-    if (K < BK) {  // the direct kernel needs a whole k-tile
-        int best = kRingSmallK;
-        for (const RingCost& s : kRingCosts)
-            if (s.id == best && !agk::grid_fits(tiles_of(s), 256)) best = kRingLargest;
-        return best;
-    }
-    int best = 0;
-    double best_cost = 0.0;
-    for (const RingCost& s : kRingCosts) {
-        if (s.id != 0 && !agk::grid_fits(tiles_of(s), 256)) continue;
-        const double tiles = static_cast<double>(tiles_of(s));
-        const double slots = static_cast<double>(cus) * s.per_cu;
-        const double rounds = static_cast<double>(static_cast<int64_t>(tiles / slots));
-        const double fill = tiles / slots - rounds;
-        const double cost =
-            rounds * s.full + (fill > 0 ? s.light + (s.full - s.light) * fill * fill : 0.0);
-        if (s.id == 0 || cost < best_cost) {
-            best = s.id;
-            best_cost = cost;
-        }
-    }
-    return best;
 }
 
 template <bool A_TR, bool B_TR>

@@ -272,6 +272,25 @@ __device__ __forceinline__ void store_block(const f32x16 (&acc)[TMW][TNW], void*
     }
 }
 
+// The epilogue that stores C.  An epilogue is called once for each block of a wave
+// (twice by the 256 x 256 kernel) with the block's accumulators and its first row
+// and column.
+template <bool OUT_F32, Stores S>
+struct StoreC {
+    void* C;
+    int64_t ldc;
+    int M, N;
+    const float* rowscale;
+    const uint16_t* colbias;
+    int accumulate;
+    template <int TMW, int TNW>
+    __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
+                                               int lane) const {
+        store_block<OUT_F32, S>(acc, C, ldc, M, N, row0, col0, lane, rowscale, colbias,
+                                accumulate);
+    }
+};
+
 // Compute units of the current device (looked up once per device; 256 on
 // MI355X), for the choice of a tile shape and the direct kernel's last-round split.
 inline int device_cus() {

@@ -28,6 +28,7 @@
 #pragma once
 
 #include "gemm_common.hpp"
+#include "rowcommon.hpp"
 
 namespace agk_gemm {
 
@@ -59,6 +60,57 @@ constexpr RingCost kRingCosts[] = {
     {3, 128, 192, 1, 0.51, 0.67}, {4, 128, 256, 1, 0.59, 0.88}, {5, 128, 128, 1, 0.39, 0.53},
     {6, 128, 64, 2, 0.30, 0.65},  {7, 64, 128, 2, 0.32, 0.65},  {8, 64, 64, 2, 0.29, 0.46},
 };
+
+// The kernel and tile a product runs on: 0 the direct kernel's 256 x 256
+// tiles, otherwise a ring shape.  The cost of a shape is its rounds of tiles
+// over the CUs times a k-step's time, which depends on how full the round is
+// (the loads of a full chip queue behind each other; the MFMAs of a full chip
+// lower the clock): light for a round of few workgroups, full for a full one,
+// light + (full - light) * fill^2 between.  The two times per shape were
+// measured on MI355X (random bf16, k-contiguous operands, K = 4096: 512 and
+// 8192 rows by 4096 columns).  What a round costs besides its k-steps is left out,
+// so K decides only below one k-tile.  Against every shape's time at 1179 products of
+// 64 to 8192 rows, 128 to 11008 columns and K of 64 to 4096, in the three layouts of a
+// layer's products (both k-contiguous, B strided, A and B strided with fp32 output), the
+// rule's shape takes 3.5 % more than the best one on average, and 21 % in one of twenty;
+// costs with a fixed part per round, fitted to them, came to 1.4 % and 9 % but were up to
+// 45 % slower at single sizes.
+//   rows x columns x K (us)   256x256  ring shape taken   other shapes
+//   512 x 4096 x 4096              58      22 (128x64)    22-42
+//   1032 x 4096 x 4096             65      39 (192x128)   39-73
+//   1032 x 4096 x 64               6.5     8.0 (192x128)  6.3-8.1
+//   2048 x 4096 x 4096             84      57 (128x256)   59-137
+//   4096 x 4096 x 1032             36      -              38-77
+//   8192 x 4096 x 4096            204      -              225-489
+// A shape whose workgroups are more than a grid holds is passed over (columns of
+// 8 by rows in the billions; the direct kernel has the largest tiles).
+inline int pick_shape(int64_t M, int64_t N, int64_t K, int cus) {
+    auto tiles_of = [&](const RingCost& s) {
+        return ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
+    };
+    if (K < BK) {  // the direct kernel needs a whole k-tile
+        int best = kRingSmallK;
+        for (const RingCost& s : kRingCosts)
+            if (s.id == best && !agk::grid_fits(tiles_of(s), 256)) best = kRingLargest;
+        return best;
+    }
+    int best = 0;
+    double best_cost = 0.0;
+    for (const RingCost& s : kRingCosts) {
+        if (s.id != 0 && !agk::grid_fits(tiles_of(s), 256)) continue;
+        const double tiles = static_cast<double>(tiles_of(s));
+        const double slots = static_cast<double>(cus) * s.per_cu;
+        const double rounds = static_cast<double>(static_cast<int64_t>(tiles / slots));
+        const double fill = tiles / slots - rounds;
+        const double cost =
+            rounds * s.full + (fill > 0 ? s.light + (s.full - s.light) * fill * fill : 0.0);
+        if (s.id == 0 || cost < best_cost) {
+            best = s.id;
+            best_cost = cost;
+        }
+    }
+    return best;
+}
 
 template <bool A_TR, bool B_TR>
 int launch_ring(int shape, bool f32, const GemmCall& c);
@@ -254,11 +306,11 @@ __device__ __forceinline__ void ring_tail(const uint16_t* stage, int k_left,
     }
 }
 
-template <bool OUT_F32, bool A_TR, bool B_TR, class SH>
-__global__ __launch_bounds__(256, SH::kPerCu) void gemm_ring_kernel(
-    const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb,
-    void* __restrict__ C, int64_t ldc, int M, int N, int K, const float* __restrict__ rowscale,
-    const uint16_t* __restrict__ colbias, int accumulate, int tiles_m, int tiles_n, int group_m) {
+template <bool A_TR, bool B_TR, class SH, class Epi>
+__device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_t lda,
+                                          const uint16_t* __restrict__ B, int64_t ldb, int M,
+                                          int N, int K, int tiles_m, int tiles_n, int group_m,
+                                          const Epi& epi) {
     constexpr int NST = SH::kStages;
     __shared__ __attribute__((aligned(16))) uint16_t st0[SH::kElems];
     __shared__ __attribute__((aligned(16))) uint16_t st1[SH::kElems];
@@ -354,9 +406,16 @@ __global__ __launch_bounds__(256, SH::kPerCu) void gemm_ring_kernel(
     }
     // the empty loads of the last steps still name this workgroup's LDS
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    store_block<OUT_F32, Stores::kAll>(acc, C, ldc, M, N, m0 + wm * SH::kTm * 32,
-                                       n0 + wn * SH::kTn * 32, lane, rowscale, colbias,
-                                       accumulate);
+    epi(acc, m0 + wm * SH::kTm * 32, n0 + wn * SH::kTn * 32, lane);
+}
+
+template <bool OUT_F32, bool A_TR, bool B_TR, class SH>
+__global__ __launch_bounds__(256, SH::kPerCu) void gemm_ring_kernel(
+    const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb,
+    void* __restrict__ C, int64_t ldc, int M, int N, int K, const float* __restrict__ rowscale,
+    const uint16_t* __restrict__ colbias, int accumulate, int tiles_m, int tiles_n, int group_m) {
+    const StoreC<OUT_F32, Stores::kAll> epi{C, ldc, M, N, rowscale, colbias, accumulate};
+    ring_body<A_TR, B_TR, SH>(A, lda, B, ldb, M, N, K, tiles_m, tiles_n, group_m, epi);
 }
 
 template <bool A_TR, bool B_TR>
