@@ -1,8 +1,8 @@
 """cgadimpl_amd -- MI355X (gfx950) RMSNorm layer path for cgadimpl's autodiff API.
 
-The product is native: HIP kernels behind the C ABI in ``include/agk_rmsnorm.h``
-and ``include/agk_rowops.h`` (``lib/libagk_rmsnorm.so``) and the C++ ``ag::`` layer above it.  This Python
-module is plumbing for tests and benchmarks: it binds that C ABI with ctypes
+The product is native: HIP kernels behind the C ABI in ``include/agk_rmsnorm.h``,
+``include/agk_rowops.h`` and ``include/agk_losses.h`` (``lib/libagk_rmsnorm.so``) and the C++
+``ag::`` layer above it.  This Python module is plumbing for tests and benchmarks: it binds that C ABI with ctypes
 and hands it torch device tensors (memory) and the current HIP stream.  There
 is no Python or CPU fallback: if the library is missing, every call raises.
 """
@@ -19,6 +19,8 @@ __all__ = [
     "layernorm_bwd", "softmax_fwd", "softmax_bwd", "logsumexp_fwd", "logsumexp_bwd",
     "logsumexp_jvp", "logsumexp_fwd_keep", "logsumexp_bwd_from_value", "rms_mul_bwd", "sum_rows", "linear_bf16",
     "mul_bcast_shape", "mul_bcast_fwd", "mul_bcast_bwd",
+    "layernorm_affine_fwd", "layernorm_affine_bwd", "linear_cross_entropy_fwd",
+    "linear_cross_entropy_bwd", "distill_topk_fwd", "distill_topk_bwd",
     "mul_bcast_grad_dtype", "gemm_f32", "set_exchange_wait_limit", "set_team_backward",
     "AGK_F32", "AGK_BF16", "STATUS",
 ]
@@ -33,11 +35,12 @@ AGK_BF16 = 1
 AGK_ACCUM_DX = 1
 AGK_ACCUM_DGAMMA = 2
 AGK_ACCUM_ALL = 3
+AGK_ACCUM_DBETA = 4
+AGK_DISTILL_MAX_K = 1024
 AGK_WIDE_MIN_COLS = 16385  # rows this wide and wider can take the split paths
 STATUS = {0: "AGK_OK", 1: "AGK_EINVAL", 2: "AGK_EDTYPE", 3: "AGK_EWORKSPACE", 4: "AGK_EHIP"}
 
-# Every symbol include/agk_rmsnorm.h and include/agk_rowops.h declare, with its
-# ctypes signature.
+# Every symbol the headers in include/ declare, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 SIGNATURES = {
@@ -85,6 +88,26 @@ SIGNATURES = {
                                          _P]),
     "agk_layernorm_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I64, ctypes.c_int, ctypes.c_int,
                                          _P]),
+    "agk_layernorm_affine_fwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, ctypes.c_float,
+                                                ctypes.c_int, _P]),
+    "agk_layernorm_affine_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "agk_layernorm_affine_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                                ctypes.c_size_t, _I64, _I64, ctypes.c_int,
+                                                ctypes.c_int, _P]),
+    "agk_linear_xent_fwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, ctypes.c_int]),
+    "agk_linear_xent_fwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _P, ctypes.c_size_t,
+                                           _I64, _I64, _I64, ctypes.c_int, _P]),
+    "agk_linear_xent_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, ctypes.c_int,
+                                                              _I64]),
+    "agk_linear_xent_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, ctypes.c_int,
+                                           _P, ctypes.c_size_t, _I64, _I64, _I64, _I64,
+                                           ctypes.c_int, ctypes.c_int, _P]),
+    "agk_distill_topk_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "agk_distill_topk_fwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, ctypes.c_size_t, _I64, _I64,
+                                            _I64, ctypes.c_float, ctypes.c_int, ctypes.c_int, _P]),
+    "agk_distill_topk_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64,
+                                            ctypes.c_float, ctypes.c_int, ctypes.c_int,
+                                            ctypes.c_int, _P]),
     "agk_softmax_fwd": (ctypes.c_int, [_P, _P, _I64, _I64, ctypes.c_int, _P]),
     "agk_softmax_bwd": (ctypes.c_int, [_P, _P, _P, _I64, _I64, ctypes.c_int, ctypes.c_int, _P]),
     "agk_logsumexp_fwd": (ctypes.c_int, [_P, _P, _I64, _I64, ctypes.c_int, _P]),
@@ -802,3 +825,208 @@ def logsumexp_jvp(z, tz, ty=None, stream=None):
                                  _stream(stream))
     _check(rc, "agk_logsumexp_jvp")
     return ty
+
+
+# ---- LayerNorm with weight and bias (include/agk_rowops.h) ------------------------
+
+def _want(t, name, like, shape, dtype):
+    """Checks one operand: a contiguous GPU tensor of `dtype` and `shape` (numel where shape is
+    an int) on the device of `like`, which must be the current one."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+    if (t.numel() != shape) if isinstance(shape, int) else (tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {like.device}")
+
+
+def _want_current(t):
+    """The kernels run on the current device's current stream: the tensors have to be there."""
+    if not t.is_cuda:
+        raise ValueError("tensor must live on the GPU")
+    if t.device.index != _torch().cuda.current_device():
+        raise ValueError(f"tensors on {t.device} while another device is current")
+
+
+def _scratch(workspace, need, like):
+    """(workspace, bytes): the caller's tensor, or what the call needs."""
+    if workspace is None:
+        workspace = _empty((need,), _torch().uint8, like) if need else None
+    elif workspace.device != like.device:
+        raise ValueError("the workspace is on another device")
+    return workspace, workspace.numel() * workspace.element_size() if workspace is not None else 0
+
+
+def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None,
+                         stream=None):
+    """y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis (gamma, beta: [cols] of
+    x's dtype, or None); returns (y, mean, rstd), the statistics float32 [..., 1]."""
+    torch = _torch()
+    _want_current(x)
+    rows, cols = _rows_cols(x)
+    for t, name in ((gamma, "gamma"), (beta, "beta")):
+        if t is not None:
+            _want(t, name, x, cols, x.dtype)
+    y = torch.empty_like(x) if y is None else y
+    mean = _row_stat_like(x, torch.float32) if mean is None else mean
+    rstd = _row_stat_like(x, torch.float32) if rstd is None else rstd
+    _want(y, "y", x, x.numel(), x.dtype)
+    _want(mean, "mean", x, rows, torch.float32)
+    _want(rstd, "rstd", x, rows, torch.float32)
+    rc = lib().agk_layernorm_affine_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean),
+                                        _ptr(rstd), rows, cols, float(eps), _dtype_code(x),
+                                        _stream(stream))
+    _check(rc, "agk_layernorm_affine_fwd")
+    return y, mean, rstd
+
+
+def layernorm_affine_bwd(x, gamma, mean, rstd, dy, dx=None, dgamma=None, dbeta=None,
+                         accumulate=False, want_dx: bool = True, want_dgamma: bool = True,
+                         want_dbeta: bool = True, workspace=None, stream=None):
+    """VJP of layernorm_affine_fwd: (dx, dgamma, dbeta), None where not wanted; dgamma and dbeta
+    float32 [cols].  accumulate: a bool (every output) or AGK_ACCUM_DX / _DGAMMA / _DBETA bits."""
+    torch = _torch()
+    _want_current(x)
+    rows, cols = _rows_cols(x)
+    acc = (7 if accumulate else 0) if isinstance(accumulate, bool) else int(accumulate)
+    if want_dx and dx is None:
+        dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
+    new = torch.zeros if acc else torch.empty
+    if want_dgamma and dgamma is None:
+        dgamma = new(cols, dtype=torch.float32, device=x.device)
+    if want_dbeta and dbeta is None:
+        dbeta = new(cols, dtype=torch.float32, device=x.device)
+    _want(dy, "dy", x, x.numel(), x.dtype)
+    _want(mean, "mean", x, rows, torch.float32)
+    _want(rstd, "rstd", x, rows, torch.float32)
+    if gamma is not None:
+        _want(gamma, "gamma", x, cols, x.dtype)
+    if dx is not None:
+        _want(dx, "dx", x, x.numel(), x.dtype)
+    need = 0
+    for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
+        if t is not None:
+            _want(t, name, x, cols, torch.float32)
+            need = int(lib().agk_layernorm_affine_bwd_workspace_bytes(rows, cols))
+    ws, ws_bytes = _scratch(workspace, need, x)
+    rc = lib().agk_layernorm_affine_bwd(_ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dy),
+                                        _ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(ws), ws_bytes,
+                                        rows, cols, _dtype_code(x), acc, _stream(stream))
+    _check(rc, "agk_layernorm_affine_bwd")
+    return dx, dgamma, dbeta
+
+
+# ---- losses (include/agk_losses.h) --------------------------------------------------
+
+def _xent_sizes(x, w, labels):
+    torch = _torch()
+    _want_current(x)
+    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1]:
+        raise ValueError("expected x [..., cols] and w [vocab, cols]")
+    rows, cols = _rows_cols(x)
+    _want(w, "w", x, w.shape, x.dtype)
+    _want(labels, "labels", x, x.shape[:-1], torch.int64)
+    return rows, w.shape[0], cols
+
+
+def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None, stream=None):
+    """The softmax cross entropy of z = x @ w.T against labels, without z in memory
+    (agk_linear_xent_fwd): x [..., cols], w [vocab, cols], labels int64 [...]; a negative label is
+    a row without a loss.  Returns (loss, stats): float32 [...] and [..., 2] (each row's maximum
+    logit and log of its sum of exponentials above it, for the backward)."""
+    torch = _torch()
+    rows, vocab, cols = _xent_sizes(x, w, labels)
+    loss = _empty(x.shape[:-1], torch.float32, x) if loss is None else loss
+    stats = _empty(x.shape[:-1] + (2,), torch.float32, x) if stats is None else stats
+    _want(loss, "loss", x, rows, torch.float32)
+    _want(stats, "stats", x, 2 * rows, torch.float32)
+    dt = _dtype_code(x)
+    ws, ws_bytes = _scratch(workspace, int(lib().agk_linear_xent_fwd_workspace_bytes(
+        rows, vocab, cols, dt)), x)
+    rc = lib().agk_linear_xent_fwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(loss),
+                                   _ptr(stats), _ptr(ws), ws_bytes, rows, vocab, cols, dt,
+                                   _stream(stream))
+    _check(rc, "agk_linear_xent_fwd")
+    return loss, stats
+
+
+def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dtype=None,
+                             accumulate=False, want_dx: bool = True, want_dw: bool = True,
+                             piece: int = 0, workspace=None, stream=None):
+    """Gradients of linear_cross_entropy_fwd for dloss, the float32 gradient of each row's loss
+    (agk_linear_xent_bwd): (dx, dw), None where not wanted.  dw is float32 unless dw_dtype (or
+    dw) says otherwise.  accumulate: a bool (both) or AGK_ACCUM_DX / AGK_ACCUM_DGAMMA (dw) bits.
+    piece: vocabulary rows whose logits exist at a time (0: the library's choice)."""
+    torch = _torch()
+    rows, vocab, cols = _xent_sizes(x, w, labels)
+    acc = _accum_flags(accumulate)
+    if want_dx and dx is None:
+        dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
+    if want_dw and dw is None:
+        new = torch.zeros if acc & AGK_ACCUM_DGAMMA else torch.empty
+        dw = new(vocab, cols, dtype=dw_dtype or torch.float32, device=x.device)
+    _want(stats, "stats", x, 2 * rows, torch.float32)
+    _want(dloss, "dloss", x, rows, torch.float32)
+    if dx is not None:
+        _want(dx, "dx", x, x.numel(), x.dtype)
+    if dw is not None:
+        _want(dw, "dw", x, (vocab, cols), dw_dtype or dw.dtype)
+    dt = _dtype_code(x)
+    ws, ws_bytes = _scratch(workspace, int(lib().agk_linear_xent_bwd_workspace_bytes(
+        rows, vocab, cols, dt, piece)), x)
+    rc = lib().agk_linear_xent_bwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(stats),
+                                   _ptr(dloss), _ptr(dx), _ptr(dw),
+                                   _dtype_code(dw) if dw is not None else AGK_F32, _ptr(ws),
+                                   ws_bytes, rows, vocab, cols, piece, dt, acc, _stream(stream))
+    _check(rc, "agk_linear_xent_bwd")
+    return dx, dw
+
+
+def _distill_sizes(z, index, teacher):
+    torch = _torch()
+    _want_current(z)
+    if z.dim() < 1 or index.dim() != z.dim() or index.shape[:-1] != z.shape[:-1]:
+        raise ValueError("expected z [..., cols] and index [..., k]")
+    _want(index, "index", z, index.shape, torch.int64)
+    _want(teacher, "teacher", z, index.shape, teacher.dtype)
+    rows = 1
+    for n in z.shape[:-1]:
+        rows *= n
+    return rows, z.shape[-1], index.shape[-1]
+
+
+def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, stats=None,
+                     workspace=None, stream=None):
+    """T^2 KL(p || q) per row of q = softmax(z / T) over all columns from p = softmax(teacher / T)
+    over the row's k named columns (agk_distill_topk_fwd): z [..., cols], index int64 [..., k] (a
+    negative one is an empty entry), teacher [..., k] float32 or bfloat16.  Returns (loss, stats):
+    float32 [...] and [..., 2]."""
+    torch = _torch()
+    rows, cols, k = _distill_sizes(z, index, teacher)
+    loss = _empty(z.shape[:-1], torch.float32, z) if loss is None else loss
+    stats = _empty(z.shape[:-1] + (2,), torch.float32, z) if stats is None else stats
+    _want(loss, "loss", z, rows, torch.float32)
+    _want(stats, "stats", z, 2 * rows, torch.float32)
+    ws, ws_bytes = _scratch(workspace, int(lib().agk_distill_topk_workspace_bytes(rows, cols)), z)
+    rc = lib().agk_distill_topk_fwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(loss), _ptr(stats),
+                                    _ptr(ws), ws_bytes, rows, cols, k, float(temperature),
+                                    _dtype_code(z), _dtype_code(teacher), _stream(stream))
+    _check(rc, "agk_distill_topk_fwd")
+    return loss, stats
+
+
+def distill_topk_bwd(z, index, teacher, stats, dloss, temperature: float = 1.0, dz=None,
+                     accumulate: bool = False, stream=None):
+    """Gradient of z for dloss, the float32 gradient of each row's loss: dz (+)= dloss * T *
+    (q - p at the named columns) (agk_distill_topk_bwd).  dz may be z (in place)."""
+    torch = _torch()
+    rows, cols, k = _distill_sizes(z, index, teacher)
+    dz = (torch.zeros_like(z) if accumulate else torch.empty_like(z)) if dz is None else dz
+    _want(stats, "stats", z, 2 * rows, torch.float32)
+    _want(dloss, "dloss", z, rows, torch.float32)
+    _want(dz, "dz", z, z.numel(), z.dtype)
+    rc = lib().agk_distill_topk_bwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(stats), _ptr(dloss),
+                                    _ptr(dz), rows, cols, k, float(temperature), _dtype_code(z),
+                                    _dtype_code(teacher), _acc_dx(accumulate), _stream(stream))
+    _check(rc, "agk_distill_topk_bwd")
+    return dz

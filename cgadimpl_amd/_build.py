@@ -2,7 +2,7 @@
 
 Outputs (in-tree, git-ignored, shipped with the source tree):
   cgadimpl_amd/lib/libagk_rmsnorm.so   HIP kernels + C ABI (include/agk_rmsnorm.h,
-                                       include/agk_rowops.h)
+                                       include/agk_rowops.h, include/agk_losses.h)
   cgadimpl_amd/lib/libagk_bench.so     bench.py's measurement probes (csrc/agk_bench.h;
                                        not product ABI)
   cgadimpl_amd/lib/libagk_synth.so     seeded synthetic input generator (host)
@@ -91,7 +91,8 @@ def host_library(name: str, sources: list[str], compiler: str = "g++") -> str:
 # The kernel library's sources (every kernel hand-written: it links nothing
 # beyond the HIP runtime).
 KERNEL_SOURCES = ["rmsnorm.hip", "gemm.hip", "gemm_ring_n.hip", "gemm_ring_t.hip", "gemm_f32.hip",
-                  "rowops.hip", "bcast.hip"]
+                  "rowops.hip", "bcast.hip", "layernorm.hip", "xent.hip", "xent_lse.hip",
+                  "xent_grad.hip", "xent_dx.hip", "xent_dw.hip", "distill.hip"]
 KERNEL_LIBS: list[str] = []
 # The benchmark's own measurement probes (csrc/agk_bench.h): loaded by bench.py
 # only, not part of the product ABI.

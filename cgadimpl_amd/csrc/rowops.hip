@@ -879,6 +879,25 @@ struct LnFwd {
     }
 };
 
+// LayerNorm with weight and bias (col0 = gamma, col1 = beta besides):
+//   y = (x - mean) * rstd * gamma + beta
+struct LnAffineFwd {
+    static constexpr int kIn = 1;
+    template <class C>
+    __device__ static void run(C& c, const RowArgs& p) {
+        const float mean = c.sum([](float x, float) { return x; }) / c.ncols;
+        const float var = c.sum([=](float x, float) {
+            const float d = x - mean;
+            return d * d;
+        }) / c.ncols;
+        const float rstd = 1.0f / sqrtf(var + p.eps);
+        c.put_f32(p.ws0, mean);
+        c.put_f32(p.ws1, rstd);
+        c.store(p.out, 0, p.col0, 1.0f, p.col1, 0.0f,
+                [=](float x, float, float g, float b) { return (x - mean) * rstd * g + b; });
+    }
+};
+
 // LayerNorm backward (in0 = x, in1 = dy, rs0 = mean, rs1 = rstd, out = dx):
 //   xhat = (x - mean) * rstd,  dx (+)= rstd * (dy - sum(dy)/cols - xhat * sum(dy*xhat)/cols)
 struct LnBwd {
@@ -1413,6 +1432,25 @@ int agk_layernorm_fwd(const void* x, void* y, float* mean, float* rstd, int64_t 
     p.ws1 = rstd;
     p.eps = eps;
     return run<LnFwd>(p, rows, cols, dtype, stream);
+}
+
+int agk_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta, void* y,
+                             float* mean, float* rstd, int64_t rows, int64_t cols, float eps,
+                             int dtype, agk_stream_t stream) {
+    using namespace agk::rowops;
+    bool done;
+    if (int rc = precheck(rows, cols, dtype, &done)) return rc;
+    if (done) return AGK_OK;
+    if (!x || !y || !mean || !rstd) return AGK_EINVAL;
+    RowArgs p;
+    p.in0 = x;
+    p.col0 = gamma;
+    p.col1 = beta;
+    p.out = y;
+    p.ws0 = mean;
+    p.ws1 = rstd;
+    p.eps = eps;
+    return run<LnAffineFwd>(p, rows, cols, dtype, stream);
 }
 
 int agk_layernorm_bwd(const void* x, const float* mean, const float* rstd, const void* dy,

@@ -1,0 +1,289 @@
+// xent_gemm.hpp -- the bf16 products of the vocabulary head's loss (xent.hip): the
+// direct and ring kernels of gemm_direct.hpp / gemm_ring.hpp with epilogues that
+// take the logits while they are in registers.  One translation unit per product
+// instantiates its kernels (AGK_XENT_KERNELS and AGK_RING_KERNELS), to compile side by side.
+//
+// Every product has the vocabulary along M and the tokens along N where it makes or
+// takes logits (z^T = w x^T): an accumulator tile then holds, in each lane, 16
+// vocabulary rows of one token per 32 x 32 block (32 blocks' worth in the 256 x 256
+// kernel), so a token's maximum and sum of exponentials are sums within a lane and
+// one exchange between the wave's halves, where tokens along M would take a
+// 5-step exchange over 32 lanes for every row of the tile.
+#pragma once
+
+#include "gemm_common.hpp"
+#include "gemm_direct.hpp"
+#include "gemm_ring.hpp"
+
+namespace agk_xent {
+
+using agk_gemm::f32x16;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp(x) on v_exp_f32; see fast_exp in rowops.hip for its error.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// One v_max_f32 (fmaxf first quiets both operands).  It drops a NaN, which reaches
+// the result through exp(z - max).
+__device__ __forceinline__ float max_of(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// Row of element e of a wave block's 32-row group i, from its first row.
+__device__ __forceinline__ int acc_row(int i, int e, int half) {
+    return i * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+}
+
+// Where a token's label lies in the block of `rows` vocabulary rows from row0 (-1:
+// elsewhere).
+__device__ __forceinline__ int label_row(int64_t label, int64_t row0, int rows) {
+    const int64_t r = label - row0;
+    return r >= 0 && r < rows ? static_cast<int>(r) : -1;
+}
+
+// Forward: the block's maximum and sum of exponentials of each token, and the logit
+// of its label.  part[(row0 / block rows) * tokens + token] = {max, sum of exp(z - max)}.
+struct LseEpi {
+    float2* part;
+    float* picked;
+    const int64_t* labels;
+    int vocab, tokens;
+
+    template <int TMW, int TNW>
+    __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
+                                               int lane) const {
+        if (row0 >= vocab) return;
+        const int half = lane >> 5;
+        const bool inner = row0 + TMW * 32 <= vocab;
+        float2* const out = part + static_cast<int64_t>(row0 / (TMW * 32)) * tokens;
+#pragma unroll
+        for (int j = 0; j < TNW; ++j) {
+            const int col = col0 + j * 32 + (lane & 31);
+            float m = -__builtin_inff();
+            if (inner) {
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) m = max_of(m, acc[i][j][e]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (row0 + acc_row(i, e, half) < vocab) m = max_of(m, acc[i][j][e]);
+            }
+            m = max_of(m, other_half(m));
+            const float shift = m == -__builtin_inff() ? 0.0f : m;  // no -inf - -inf
+            float s = 0.0f;
+            if (inner) {
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s += exp_of(acc[i][j][e] - shift);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (row0 + acc_row(i, e, half) < vocab) s += exp_of(acc[i][j][e] - shift);
+            }
+            s += other_half(s);
+            const bool in = col < tokens;
+            if (in && half == 0) out[col] = make_float2(m, s);
+            const int at = in ? label_row(labels[col], row0, TMW * 32) : -1;
+            if (__any(at >= 0)) {
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (at == acc_row(i, e, half) && row0 + at < vocab)
+                            picked[col] = acc[i][j][e];
+            }
+        }
+    }
+};
+
+// Backward: G^T, weight * (softmax - [label]), rounded to bf16: rows v0 .. of the
+// vocabulary as rows of ldg tokens, zeros in the columns from `tokens` to ldg (the
+// padding that makes ldg a multiple of 8: the product over tokens reads it).
+struct GradEpi {
+    uint16_t* G;
+    const float2* stats;
+    const float* weight;  // 0: a token that is left out
+    const int64_t* labels;
+    int64_t v0;
+    int ldg, rows, tokens;
+
+    template <int TMW, int TNW>
+    __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
+                                               int lane) const {
+        if (row0 >= rows) return;
+        const int half = lane >> 5;
+        const bool inner = row0 + TMW * 32 <= rows;
+#pragma unroll
+        for (int j = 0; j < TNW; ++j) {
+            const int col = col0 + j * 32 + (lane & 31);
+            const bool in = col < tokens;
+            const float2 st = in ? stats[col] : make_float2(0.0f, 0.0f);
+            const float w = in ? weight[col] : 0.0f;
+            const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
+            const bool hit = __any(at >= 0);
+            if (col < ldg) {
+                uint16_t* const out = G + col;
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int r = acc_row(i, e, half);
+                        float p = exp_of((acc[i][j][e] - st.x) - st.y);
+                        if (hit) p -= at == r ? 1.0f : 0.0f;
+                        const float g = w != 0.0f ? w * p : 0.0f;
+                        if (inner || row0 + r < rows)
+                            out[static_cast<int64_t>(row0 + r) * ldg] =
+                                static_cast<uint16_t>(agk_gemm::f32_to_bf16_bits(g));
+                    }
+            }
+        }
+    }
+};
+
+// C (+)= alpha * product (alpha NULL: 1), the product rounded before it is added.  The
+// old values of a 32-row group are loaded together: one wait for 16 TNW loads.
+template <bool OUT_F32>
+struct AddEpi {
+    void* C;
+    int64_t ldc;
+    int64_t slice;  // elements between the K slices' outputs
+    const float* alpha;
+    int M, N, accumulate;
+
+    template <int TMW, int TNW>
+    __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
+                                               int lane) const {
+        using T = typename std::conditional<OUT_F32, float, uint16_t>::type;
+        if (row0 >= M || col0 >= N) return;
+        const int half = lane >> 5;
+        const float a = alpha ? *alpha : 1.0f;
+        T* const c0 = static_cast<T*>(C) + static_cast<int64_t>(blockIdx.y) * slice;
+        const bool inner = row0 + TMW * 32 <= M && col0 + TNW * 32 <= N;
+#pragma unroll
+        for (int i = 0; i < TMW; ++i) {
+            T* const p0 = c0 + static_cast<int64_t>(row0 + i * 32 + 4 * half) * ldc + col0 +
+                          (lane & 31);
+            const int rows_left = M - (row0 + i * 32 + 4 * half);
+            const int cols_left = N - (col0 + (lane & 31));
+            T old[TNW][16] = {};
+            if (accumulate) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+#pragma unroll
+                    for (int j = 0; j < TNW; ++j)
+                        if (inner || (8 * (e >> 2) + (e & 3) < rows_left && j * 32 < cols_left))
+                            old[j][e] = p0[static_cast<int64_t>(8 * (e >> 2) + (e & 3)) * ldc + j * 32];
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int j = 0; j < TNW; ++j) {
+                    float v = acc[i][j][e] * a;
+                    if (accumulate) {
+                        float o;
+                        if constexpr (OUT_F32) o = old[j][e];
+                        else o = __uint_as_float(static_cast<uint32_t>(old[j][e]) << 16);
+                        v = agk::acc_add(o, v);
+                    }
+                    if (inner || (8 * (e >> 2) + (e & 3) < rows_left && j * 32 < cols_left)) {
+                        T* const p = p0 + static_cast<int64_t>(8 * (e >> 2) + (e & 3)) * ldc + j * 32;
+                        if constexpr (OUT_F32) *p = v;
+                        else *p = static_cast<uint16_t>(agk_gemm::f32_to_bf16_bits(v));
+                    }
+                }
+        }
+    }
+};
+
+// One product: M, N as staged (an operand with rows contiguous needs them to be
+// multiples of 8), the epilogue's own bounds what is stored.  slices > 1: K cut into
+// that many parts of k_slice (a multiple of 64; the last takes the rest), one per
+// grid row, each with its own output.
+struct Product {
+    const uint16_t* A;
+    int64_t lda;
+    const uint16_t* B;
+    int64_t ldb;
+    int M, N, K, slices, k_slice;
+    hipStream_t st;
+};
+
+int launch_lse(int shape, const Product& p, const LseEpi& e);
+int launch_grad(int shape, const Product& p, const GradEpi& e);
+int launch_dx(int shape, const Product& p, const AddEpi<true>& e);
+int launch_dw(int shape, const Product& p, const AddEpi<true>& e);
+int launch_dw(int shape, const Product& p, const AddEpi<false>& e);
+
+}  // namespace agk_xent
+
+#ifdef AGK_XENT_KERNELS
+
+namespace agk_xent {
+
+template <bool A_TR, bool B_TR, bool TAIL, class Epi>
+__global__ __launch_bounds__(agk_gemm::kDirectThreads) void xent_direct_kernel(
+    const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
+    int N, int K, const Epi epi, int tiles_m, int tiles_n, int full_tiles) {
+    __shared__ __attribute__((aligned(16))) uint16_t st0[agk_gemm::kStageElems];
+    __shared__ __attribute__((aligned(16))) uint16_t st1[agk_gemm::kStageElems];
+    agk_gemm::direct_body<A_TR, B_TR, TAIL>(A, lda, B, ldb, M, N, K, tiles_m, tiles_n,
+                                            agk_gemm::kGroupM, full_tiles, st0, st1, epi);
+}
+
+template <bool A_TR, bool B_TR, class SH, class Epi>
+__global__ __launch_bounds__(256, SH::kPerCu) void xent_ring_kernel(
+    const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
+    int N, int K, int k_slice, const Epi epi, int tiles_m, int tiles_n) {
+    const int k0 = static_cast<int>(blockIdx.y) * k_slice;
+    A += A_TR ? static_cast<int64_t>(k0) * lda : k0;
+    B += B_TR ? static_cast<int64_t>(k0) * ldb : k0;
+    const int k = blockIdx.y + 1 < gridDim.y ? k_slice : K - k0;
+    agk_gemm::ring_body<A_TR, B_TR, SH>(A, lda, B, ldb, M, N, k, tiles_m, tiles_n,
+                                        agk_gemm::kGroupM, epi);
+}
+
+template <bool A_TR, bool B_TR, class Epi>
+int launch_product(int shape, const Product& p, const Epi& e) {
+    using namespace agk_gemm;
+    if (shape == 0) {
+        const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+        const int tiles = tiles_m * tiles_n;
+        const int full = direct_full_tiles(tiles, device_cus());
+        const dim3 grid(full + 2 * (tiles - full)), block(kDirectThreads);
+        if (p.K % BK != 0)
+            hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, true, Epi>), grid, block, 0, p.st,
+                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, e, tiles_m, tiles_n, full);
+        else
+            hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, false, Epi>), grid, block, 0, p.st,
+                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, e, tiles_m, tiles_n, full);
+        return agk::check_launch();
+    }
+#define AGK_XENT_CASE(ID, BM_, BN_, WVM, NST)                                                    \
+    case ID: {                                                                                   \
+        using SH = RingShape<BM_, BN_, WVM, NST>;                                                \
+        const int tiles_m = (p.M + BM_ - 1) / BM_, tiles_n = (p.N + BN_ - 1) / BN_;              \
+        hipLaunchKernelGGL((xent_ring_kernel<A_TR, B_TR, SH, Epi>),                              \
+                           dim3(tiles_m * tiles_n, p.slices), dim3(256), 0, p.st, p.A, p.lda,    \
+                           p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, tiles_m, tiles_n);           \
+        break;                                                                                   \
+    }
+    switch (shape) { AGK_RING_SHAPES(AGK_XENT_CASE) }
+#undef AGK_XENT_CASE
+    return agk::check_launch();
+}
+
+}  // namespace agk_xent
+
+#endif  // AGK_XENT_KERNELS

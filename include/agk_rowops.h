@@ -1,7 +1,8 @@
 /*
  * agk_rowops.h -- C ABI of the row kernels that share the RMSNorm layer's
- * row-reduce skeleton: the forward-mode product (JVP) of RMSNorm, LayerNorm,
- * row softmax and row log-sum-exp, with their vector-Jacobian products.
+ * row-reduce skeleton: the forward-mode product (JVP) of RMSNorm, LayerNorm
+ * (without and with weight and bias), row softmax and row log-sum-exp, with
+ * their vector-Jacobian products.
  *
  * Implemented by the same library as agk_rmsnorm.h (libagk_rmsnorm.so), with
  * the same conventions: device pointers; row-major contiguous [rows, cols]
@@ -69,6 +70,34 @@ int agk_layernorm_fwd(const void* x, void* y, float* mean, float* rstd,
 int agk_layernorm_bwd(const void* x, const float* mean, const float* rstd,
                       const void* dy, void* dx, int64_t rows, int64_t cols,
                       int dtype, int accumulate, agk_stream_t stream);
+
+/* LayerNorm with weight and bias, y = (x - mean) * rstd * gamma + beta; gamma
+ * and beta [cols] of the storage type, NULL for none (ones, zeros; both NULL is
+ * agk_layernorm_fwd).  Saves mean[rows] and rstd[rows] = 1/sqrt(var + eps) in
+ * fp32, the variance as in agk_layernorm_fwd.  y may be x itself.  The
+ * reference's layer has no weight and bias (laynor_nodeops,
+ * cgadimpl/src/ops/normalization.cpp:10-22).                                 */
+int agk_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta, void* y,
+                             float* mean, float* rstd, int64_t rows, int64_t cols, float eps,
+                             int dtype, agk_stream_t stream);
+
+/* Its VJP, with xhat = (x - mean) * rstd and h = dy * gamma:
+ *     dx (+)= rstd * (h - sum(h)/cols - xhat * sum(h * xhat)/cols)
+ *     dgamma (+)= sum_rows dy * xhat,  dbeta (+)= sum_rows dy      (fp32)
+ * in one pass over x and dy.  dx, dgamma and dbeta may each be NULL; dx may be
+ * dy itself.  accumulate: AGK_ACCUM_DX, AGK_ACCUM_DGAMMA and AGK_ACCUM_DBETA.
+ * workspace: agk_layernorm_affine_bwd_workspace_bytes(rows, cols) bytes of
+ * scratch, 4-byte aligned (two fp32 partial rows per workgroup, of which there
+ * are min(rows, 256)); NULL without dgamma and dbeta.  Calls that share one
+ * must not overlap in time.  rows == 0 zero-fills dgamma and dbeta unless they
+ * accumulate.  Deterministic: partial rows are added in a fixed order.       */
+#define AGK_ACCUM_DBETA 4 /* dbeta += ... */
+size_t agk_layernorm_affine_bwd_workspace_bytes(int64_t rows, int64_t cols);
+
+int agk_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean,
+                             const float* rstd, const void* dy, void* dx, float* dgamma,
+                             float* dbeta, void* workspace, size_t workspace_bytes, int64_t rows,
+                             int64_t cols, int dtype, int accumulate, agk_stream_t stream);
 
 /* Row softmax, y = exp(z - max(z)) / sum(exp(z - max(z))) over the last
  * axis.  Replaces softmax_row_nodeops, cgadimpl/src/ops/reduction.cpp:42-53. */
