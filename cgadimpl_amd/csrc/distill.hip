@@ -25,7 +25,6 @@ namespace distill {
 constexpr int kLanes = 256;
 constexpr int kWaves = kLanes / 64;
 constexpr int kMaxK = AGK_DISTILL_MAX_K;
-constexpr int kPerLane = kMaxK / kLanes;  // entries of the teacher a lane holds
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float max_of(float a, float b) {  // one v_max_f32; drops a NaN
@@ -72,22 +71,25 @@ struct Args {
     float temperature, scale;  // scale = log2(e) / T
 };
 
-// A row's teacher as the lanes hold it: entry j = lane + i * kLanes.
+// A row's teacher as the lanes hold it: PER entries, j = lane + i * kLanes.  Kernels are built
+// for PER = 1 (k <= 256) and for the most entries: the rest of a kernel then keeps the registers.
+template <int PER>
 struct Teacher {
-    int64_t index[kPerLane];  // < 0: no entry
-    float p[kPerLane], logp[kPerLane];
+    int64_t index[PER];  // < 0: no entry
+    float p[PER], logp[PER];
     bool any, bad;  // an entry with a probability; a column past the last
 };
 
 // red: three arrays of kWaves floats.
-__device__ __forceinline__ void load_teacher(const Args& a, int64_t row, Teacher& o,
+template <int PER>
+__device__ __forceinline__ void load_teacher(const Args& a, int64_t row, Teacher<PER>& o,
                                              float (*red)[kWaves]) {
-    float t[kPerLane];
+    float t[PER];
     float top = -__builtin_inff();
     int flags = 0;
     const int64_t base = row * a.k;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const int j = static_cast<int>(threadIdx.x) + i * kLanes;
         o.index[i] = -1;
         t[i] = -__builtin_inff();
@@ -107,22 +109,21 @@ __device__ __forceinline__ void load_teacher(const Args& a, int64_t row, Teacher
     o.any = any;
     o.bad = bad;
     top = block_max(top, red[0]);
-    float e[kPerLane], sum = 0.0f;
+    float e[PER], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
+    for (int i = 0; i < PER; ++i) {
         e[i] = t[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((t[i] - top) * a.scale);
         sum += e[i];
     }
     sum = block_sum(sum, red[1]);
     const float logs = logf(sum);
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
+    for (int i = 0; i < PER; ++i) {
         o.p[i] = e[i] / sum;
         o.logp[i] = (t[i] - top) / a.temperature - logs;
     }
 }
 
-template <class S>
 __device__ __forceinline__ void seg_range(const Args& a, int seg, int64_t& c0, int& n) {
     c0 = static_cast<int64_t>(seg) * a.seg_cols;
     const int64_t left = a.cols - c0;
@@ -138,7 +139,65 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, flo
     s = x + y;
 }
 
-// {max, sum} of a segment, in lane 0.
+// A segment as its elements before the first 16-byte boundary (at most W - 1), a body of
+// whole 16-byte slots and the elements after it (at most W - 1): rows of odd widths start
+// at any element, and 16-byte accesses off their boundary run at 5.8 of 6.4 TB/s.
+struct Parts {
+    int head, slots, tail0;  // tail0: the first element after the body
+};
+template <class S>
+__device__ __forceinline__ Parts parts_of(const void* p, int n) {
+    using T = typename S::T;
+    constexpr int W = S::kVec;
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+    Parts q;
+    q.head = off ? W - off : 0;
+    if (q.head > n) q.head = n;
+    q.slots = (n - q.head) / W;
+    q.tail0 = q.head + q.slots * W;
+    return q;
+}
+// The element of head or tail that lane t has (-1: none).
+__device__ __forceinline__ int edge(const Parts& q, int n) {
+    const int t = static_cast<int>(threadIdx.x);
+    const int c = t < 8 ? (t < q.head ? t : -1) : t < 16 ? q.tail0 + t - 8 : -1;
+    return c < n ? c : -1;
+}
+
+// A lane's running maximum m and sum s of 2^((z - m) scale).  The exponent is one fma,
+// z scale - t with t = m scale rounded once; what the rounding left, d = m scale - t, is
+// exact as an fma and goes into the sum as 2^-d, so that sums of different m add up as if
+// t were exact.  Where m scale overflows (logits of 1e38, or masks of the type's lowest
+// value and nothing else) the difference is formed first.
+struct Lse {
+    float m, s;
+    template <int N>
+    __device__ __forceinline__ void add(const float (&f)[N], float scale) {
+        float top = m;
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = max_of(top, f[e]);
+        if (top == -__builtin_inff()) {  // s stays 0, or takes a NaN
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += f[e] == f[e] ? 0.0f : f[e];
+            return;
+        }
+        if (top != m) s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f((m - top) * scale);
+        m = top;
+        const float t = top * scale;
+        float sum = 0.0f;
+        if (__builtin_fabsf(t) < 1e37f) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                sum += __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], scale, -t));
+            s += sum * __builtin_amdgcn_exp2f(-__builtin_fmaf(top, scale, -t));
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += __builtin_amdgcn_exp2f((f[e] - top) * scale);
+        }
+    }
+};
+
+// {max, sum} of a segment, in every lane.
 constexpr int kBatch = 4;  // 16-byte loads in flight per lane
 template <class S>
 __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, float& m, float& s,
@@ -147,48 +206,37 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
     constexpr int W = S::kVec;
     int64_t c0;
     int n;
-    seg_range<S>(a, seg, c0, n);
+    seg_range(a, seg, c0, n);
     const T* const z = static_cast<const T*>(a.z) + row * a.cols + c0;
-    m = -__builtin_inff();
-    s = 0.0f;
-    const int nvec = n / W;
-    for (int v0 = threadIdx.x; v0 < nvec; v0 += kLanes * kBatch) {
+    const Parts q = parts_of<S>(z, n);
+    const u32x4* const body = reinterpret_cast<const u32x4*>(z + q.head);
+    Lse r{-__builtin_inff(), 0.0f};
+    int v = static_cast<int>(threadIdx.x);
+    for (; v + (kBatch - 1) * kLanes < q.slots; v += kLanes * kBatch) {
         u32x4 raw[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int v = v0 + u * kLanes;
-            raw[u] = load16_any_stream<S>(z + static_cast<int64_t>(v < nvec ? v : v0) * W);
-        }
-        float f[kBatch][W];
-        float top = m;
+        for (int u = 0; u < kBatch; ++u) raw[u] = __builtin_nontemporal_load(body + v + u * kLanes);
+        float f[kBatch * W];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            S::unpack(raw[u], f[u]);
+            float g[W];
+            S::unpack(raw[u], g);
 #pragma unroll
-            for (int e = 0; e < W; ++e) {
-                if (v0 + u * kLanes >= nvec) f[u][e] = -__builtin_inff();
-                top = max_of(top, f[u][e]);
-            }
+            for (int e = 0; e < W; ++e) f[u * W + e] = g[e];
         }
-        const float shift = top == -__builtin_inff() ? 0.0f : top;
-        // before the first finite value s is 0, or a NaN already met
-        float sum = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f((m - shift) * a.scale);
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-#pragma unroll
-            for (int e = 0; e < W; ++e) sum += __builtin_amdgcn_exp2f((f[u][e] - shift) * a.scale);
-        m = top;
-        s = sum;
+        r.add(f, a.scale);
     }
-    const int c = nvec * W + static_cast<int>(threadIdx.x);
-    if (c < n) {
-        const float v = S::get(z + c);
-        const float top = max_of(m, v);
-        const float shift = top == -__builtin_inff() ? 0.0f : top;
-        s = (m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f((m - shift) * a.scale)) +
-            __builtin_amdgcn_exp2f((v - shift) * a.scale);
-        m = top;
+    for (; v < q.slots; v += kLanes) {
+        float f[W];
+        S::unpack(__builtin_nontemporal_load(body + v), f);
+        r.add(f, a.scale);
     }
+    if (const int c = edge(q, n); c >= 0) {
+        const float f[1] = {S::get(z + c)};
+        r.add(f, a.scale);
+    }
+    m = r.m;
+    s = r.s;
 #pragma unroll
     for (int h = 32; h > 0; h /= 2) {
         const float m2 = __shfl_xor(m, h), s2 = __shfl_xor(s, h);
@@ -203,17 +251,17 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
 }
 
 // The row's loss from its {max, sum}; called by the whole workgroup.
-template <class S>
+template <class S, int PER>
 __device__ __forceinline__ void row_loss(const Args& a, int64_t row, float m, float s, float* loss,
                                          float2* stats, float (*red)[kWaves]) {
     using T = typename S::T;
     const T* const z = static_cast<const T*>(a.z) + row * a.cols;
     const float l = logf(s);
-    Teacher t;
+    Teacher<PER> t;
     load_teacher(a, row, t, red);
     float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
+    for (int i = 0; i < PER; ++i)
         if (t.index[i] >= 0 && t.index[i] < a.cols && !(t.p[i] == 0.0f)) {
             const float logq = (S::get(z + t.index[i]) - m) / a.temperature - l;
             v += t.p[i] * (t.logp[i] - logq);
@@ -226,7 +274,7 @@ __device__ __forceinline__ void row_loss(const Args& a, int64_t row, float m, fl
 }
 
 // One workgroup per row (segs == 1), looping over what the grid leaves.
-template <class S>
+template <class S, int PER>
 __global__ __launch_bounds__(kLanes) void distill_fwd(const Args a, float* __restrict__ loss,
                                                       float2* __restrict__ stats) {
     __shared__ float2 red2[kWaves];
@@ -234,7 +282,7 @@ __global__ __launch_bounds__(kLanes) void distill_fwd(const Args a, float* __res
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float m, s;
         seg_lse<S>(a, row, 0, m, s, red2);
-        row_loss<S>(a, row, m, s, loss, stats, red);
+        row_loss<S, PER>(a, row, m, s, loss, stats, red);
         __syncthreads();
     }
 }
@@ -250,7 +298,7 @@ __global__ __launch_bounds__(kLanes) void distill_part(const Args a, float2* __r
     if (threadIdx.x == 0) part[blockIdx.x] = make_float2(m, s);
 }
 
-template <class S>
+template <class S, int PER>
 __global__ __launch_bounds__(kLanes) void distill_join(const Args a, const float2* __restrict__ part,
                                                        float* __restrict__ loss,
                                                        float2* __restrict__ stats) {
@@ -266,106 +314,127 @@ __global__ __launch_bounds__(kLanes) void distill_join(const Args a, const float
         const float m2 = __shfl_xor(m, h), s2 = __shfl_xor(s, h);
         join(m, s, m2, s2, a.scale);
     }
-    row_loss<S>(a, row, m, s, loss, stats, red);
+    row_loss<S, PER>(a, row, m, s, loss, stats, red);
 }
 
-// dz of one segment of one row.
-template <class S>
-__global__ __launch_bounds__(kLanes) void distill_bwd(const Args a, const float2* __restrict__ stats,
-                                                      const float* __restrict__ dloss, void* dz_,
-                                                      int accumulate) {
+// dz of one segment of one row.  The columns that the teacher named are stored twice, as
+// q first and then, after every store of the segment, with their p subtracted.  A bit map of the
+// segment's columns finds whether any is named twice; only then are the entries
+// compared with each other.  (bf16 96 x 131072, k = 256: 56 us comparing always.)
+constexpr int kMapBits = 1 << 16;  // columns that far apart share a bit
+template <class S, int PER, bool ACC>
+__global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : 4) void distill_bwd(const Args a, const float2* __restrict__ stats,
+                                                      const float* __restrict__ dloss, void* dz_) {
     using T = typename S::T;
     constexpr int W = S::kVec;
     __shared__ float red[3][kWaves];
     __shared__ int at[kMaxK];   // column within the segment; -1: elsewhere
     __shared__ float prob[kMaxK];
+    __shared__ unsigned map[kMapBits / 32];
     for (int64_t item = blockIdx.x; item < a.rows * a.segs; item += gridDim.x) {
         const int64_t row = item / a.segs;
         int64_t c0;
         int n;
-        seg_range<S>(a, static_cast<int>(item - row * a.segs), c0, n);
+        seg_range(a, static_cast<int>(item - row * a.segs), c0, n);
         const int64_t base = row * a.cols + c0;
         const T* const z = static_cast<const T*>(a.z) + base;
         T* const dz = static_cast<T*>(dz_) + base;
-        Teacher t;
-        load_teacher(a, row, t, red);
+        const int words = ((n < kMapBits ? n : kMapBits) + 31) / 32;
+        for (int i = threadIdx.x; i < words; i += kLanes) map[i] = 0u;
+        Teacher<PER> t;
+        load_teacher(a, row, t, red);  // has the barrier that the map needs
         const float2 st = stats[row];
         const float c = t.bad ? __builtin_nanf("") : t.any ? dloss[row] * a.temperature : 0.0f;
+        const float l2 = st.y * kLog2e;
         auto grad = [&](float v) {
-            return c * __builtin_amdgcn_exp2f((v - st.x) * a.scale - st.y * kLog2e);
+            return c * __builtin_amdgcn_exp2f(__builtin_fmaf(v - st.x, a.scale, -l2));
         };
-        // The columns the teacher named: what they need of z and the old dz is read
-        // before any of dz is written.
-        float own_z[kPerLane], own_old[kPerLane];
-        int own_at[kPerLane];
+        // What the named columns need of z and the old dz is read before any of dz is
+        // written.
+        float own_z[PER], own_old[PER];
+        int own_at[PER], twice = 0;
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
+        for (int i = 0; i < PER; ++i) {
             const int j = static_cast<int>(threadIdx.x) + i * kLanes;
             const int64_t r = t.index[i] - c0;
             own_at[i] = t.index[i] >= 0 && r >= 0 && r < n ? static_cast<int>(r) : -1;
             own_z[i] = own_old[i] = 0.0f;
             if (own_at[i] >= 0) {
                 own_z[i] = S::get(z + own_at[i]);
-                if (accumulate) own_old[i] = S::get(dz + own_at[i]);
+                if constexpr (ACC) own_old[i] = S::get(dz + own_at[i]);
+                const unsigned bit = static_cast<unsigned>(own_at[i]) % kMapBits;
+                if (atomicOr(&map[bit / 32], 1u << (bit % 32)) >> (bit % 32) & 1u) twice = 1;
             }
             if (j < a.k) {
                 at[j] = own_at[i];
                 prob[j] = t.p[i];
             }
         }
-        __syncthreads();
-        const int nvec = n / W;
+        twice = __syncthreads_or(twice);
+        const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
         if (c == 0.0f) {
-            if (!accumulate) {
-                const u32x4 zero = {0u, 0u, 0u, 0u};
-                for (int v = threadIdx.x; v < nvec; v += kLanes)
-                    store16_any_stream<S>(dz + static_cast<int64_t>(v) * W, zero);
-                const int e = nvec * W + static_cast<int>(threadIdx.x);
-                if (e < n) S::put(dz + e, 0.0f);
+            if constexpr (!ACC) {
+                const Parts q = parts_of<S>(dz, n);
+                u32x4* const db = reinterpret_cast<u32x4*>(dz + q.head);
+                for (int v = threadIdx.x; v < q.slots; v += kLanes)
+                    __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, db + v);
+                if (const int e = edge(q, n); e >= 0) S::put(dz + e, 0.0f);
+            }
+        } else if (!same) {  // z and dz at different offsets from a 16-byte boundary
+            for (int e = threadIdx.x; e < n; e += kLanes) {
+                const float g = grad(S::get(z + e));
+                S::put(dz + e, ACC ? acc_add(S::get(dz + e), g) : g);
             }
         } else {
-            for (int v0 = threadIdx.x; v0 < nvec; v0 += kLanes * kBatch) {
-                u32x4 raw[kBatch], old[kBatch];
+            const Parts q = parts_of<S>(z, n);
+            const u32x4* const zb = reinterpret_cast<const u32x4*>(z + q.head);
+            u32x4* const db = reinterpret_cast<u32x4*>(dz + q.head);
+            auto slot = [&](int v, u32x4 raw, u32x4 old) {
+                float f[W];
+                S::unpack(raw, f);
+#pragma unroll
+                for (int e = 0; e < W; ++e) f[e] = grad(f[e]);
+                if constexpr (ACC) {
+                    float o[W];
+                    S::unpack(old, o);
+#pragma unroll
+                    for (int e = 0; e < W; ++e) f[e] = acc_add(o[e], f[e]);
+                }
+                __builtin_nontemporal_store(S::pack(f), db + v);
+            };
+            int v = static_cast<int>(threadIdx.x);
+            for (; v + (kBatch - 1) * kLanes < q.slots; v += kLanes * kBatch) {
+                u32x4 raw[kBatch], old[kBatch] = {};
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
-                    const int v = v0 + u * kLanes;
-                    const int64_t e = static_cast<int64_t>(v < nvec ? v : v0) * W;
-                    raw[u] = load16_any_stream<S>(z + e);
-                    if (accumulate) old[u] = load16_any_stream<S>(dz + e);
+                    raw[u] = __builtin_nontemporal_load(zb + v + u * kLanes);
+                    if constexpr (ACC) old[u] = __builtin_nontemporal_load(db + v + u * kLanes);
                 }
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int v = v0 + u * kLanes;
-                    if (v >= nvec) continue;
-                    float f[W];
-                    S::unpack(raw[u], f);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) f[e] = grad(f[e]);
-                    if (accumulate) {
-                        float o[W];
-                        S::unpack(old[u], o);
-#pragma unroll
-                        for (int e = 0; e < W; ++e) f[e] = acc_add(o[e], f[e]);
-                    }
-                    store16_any_stream<S>(dz + static_cast<int64_t>(v) * W, S::pack(f));
-                }
+                for (int u = 0; u < kBatch; ++u) slot(v + u * kLanes, raw[u], old[u]);
             }
-            const int e = nvec * W + static_cast<int>(threadIdx.x);
-            if (e < n) {
+            for (; v < q.slots; v += kLanes)
+                slot(v, __builtin_nontemporal_load(zb + v),
+                     ACC ? __builtin_nontemporal_load(db + v) : u32x4{0u, 0u, 0u, 0u});
+            if (const int e = edge(q, n); e >= 0) {
                 const float g = grad(S::get(z + e));
-                S::put(dz + e, accumulate ? acc_add(S::get(dz + e), g) : g);
+                S::put(dz + e, ACC ? acc_add(S::get(dz + e), g) : g);
             }
-            // The named columns again, after every store of the segment: q - sum of
-            // their p.  Entries of one column all write the same value.
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+        }
+        // Entries of one column all write the same value.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (c != 0.0f) {
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
+            for (int i = 0; i < PER; ++i) {
                 if (own_at[i] < 0) continue;
-                float p = 0.0f;
-                for (int j = 0; j < a.k; ++j) p += at[j] == own_at[i] ? prob[j] : 0.0f;
+                float p = t.p[i];
+                if (twice) {
+                    p = 0.0f;
+                    for (int j = 0; j < a.k; ++j) p += at[j] == own_at[i] ? prob[j] : 0.0f;
+                }
                 const float g = grad(own_z[i]) - c * p;
-                S::put(dz + own_at[i], accumulate ? acc_add(own_old[i], g) : g);
+                S::put(dz + own_at[i], ACC ? acc_add(own_old[i], g) : g);
             }
         }
         __syncthreads();
@@ -410,21 +479,32 @@ inline Args args(const void* z, const int64_t* index, const void* t, int64_t row
     return a;
 }
 
-template <class S>
+template <class S, int PER>
 int forward(const Args& a, float* loss, float2* stats, float2* part, hipStream_t st) {
     if (a.segs == 1) {
-        hipLaunchKernelGGL(distill_fwd<S>, dim3(capped_blocks(a.rows, kLanes)), dim3(kLanes), 0, st,
-                           a, loss, stats);
+        hipLaunchKernelGGL((distill_fwd<S, PER>), dim3(capped_blocks(a.rows, kLanes)), dim3(kLanes),
+                           0, st, a, loss, stats);
         return check_launch();
     }
     hipLaunchKernelGGL(distill_part<S>, dim3(static_cast<unsigned>(a.rows * a.segs)), dim3(kLanes),
                        0, st, a, part);
     const int rc = check_launch();
     if (rc != AGK_OK) return rc;
-    hipLaunchKernelGGL(distill_join<S>, dim3(static_cast<unsigned>(a.rows)), dim3(kLanes), 0, st, a,
-                       part, loss, stats);
+    hipLaunchKernelGGL((distill_join<S, PER>), dim3(static_cast<unsigned>(a.rows)), dim3(kLanes), 0,
+                       st, a, part, loss, stats);
     return check_launch();
 }
+
+template <class S, int PER>
+int backward(const Args& a, const float2* stats, const float* dloss, void* dz, bool acc,
+             hipStream_t st) {
+    const dim3 grid(capped_blocks(a.rows * a.segs, kLanes)), block(kLanes);
+    if (acc) hipLaunchKernelGGL((distill_bwd<S, PER, true>), grid, block, 0, st, a, stats, dloss, dz);
+    else hipLaunchKernelGGL((distill_bwd<S, PER, false>), grid, block, 0, st, a, stats, dloss, dz);
+    return check_launch();
+}
+
+constexpr int kMostPer = kMaxK / kLanes;
 
 }  // namespace distill
 }  // namespace agk
@@ -456,8 +536,11 @@ int agk_distill_topk_fwd(const void* z, const int64_t* index, const void* t, flo
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     float2* const out = reinterpret_cast<float2*>(stats);
     float2* const part = static_cast<float2*>(workspace);
-    return dtype == AGK_F32 ? forward<agk::F32>(a, loss, out, part, st)
-                            : forward<agk::BF16>(a, loss, out, part, st);
+    if (dtype == AGK_F32)
+        return k <= kLanes ? forward<agk::F32, 1>(a, loss, out, part, st)
+                           : forward<agk::F32, kMostPer>(a, loss, out, part, st);
+    return k <= kLanes ? forward<agk::BF16, 1>(a, loss, out, part, st)
+                       : forward<agk::BF16, kMostPer>(a, loss, out, part, st);
 }
 
 int agk_distill_topk_bwd(const void* z, const int64_t* index, const void* t, const float* stats,
@@ -478,14 +561,12 @@ int agk_distill_topk_bwd(const void* z, const int64_t* index, const void* t, con
     const Args a = args(z, index, t, rows, cols, k, temperature, t_dtype);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const float2* const in = reinterpret_cast<const float2*>(stats);
-    const dim3 grid(agk::capped_blocks(rows * a.segs, kLanes));
-    const int acc = accumulate != 0;
+    const bool acc = accumulate != 0;
     if (dtype == AGK_F32)
-        hipLaunchKernelGGL(distill_bwd<agk::F32>, grid, dim3(kLanes), 0, st, a, in, dloss, dz, acc);
-    else
-        hipLaunchKernelGGL(distill_bwd<agk::BF16>, grid, dim3(kLanes), 0, st, a, in, dloss, dz,
-                           acc);
-    return agk::check_launch();
+        return k <= kLanes ? backward<agk::F32, 1>(a, in, dloss, dz, acc, st)
+                           : backward<agk::F32, kMostPer>(a, in, dloss, dz, acc, st);
+    return k <= kLanes ? backward<agk::BF16, 1>(a, in, dloss, dz, acc, st)
+                       : backward<agk::BF16, kMostPer>(a, in, dloss, dz, acc, st);
 }
 
 }  // extern "C"

@@ -7,8 +7,7 @@
 // each wave's block of z^T leaves as {max, sum of exponentials} per token, 8 bytes for 32 to
 // 128 logits, and a second kernel joins a token's blocks.  The backward makes z
 // again, a piece of the vocabulary at a time, leaving G's piece in bf16 (the matrix
-// cores' operand), and takes the two products from it while it is in the Infinity
-// Cache.  dw's rows belong to one piece; dx adds up in fp32 over the pieces.
+// cores' operand), and takes the two products from it.  dw's rows belong to one piece; dx adds up in fp32 over the pieces.
 // 8 tokens vocab cols flop a step, 2 of the forward and 6 of the backward (2 of them
 // the logits again: the price of not keeping them).
 //
@@ -239,10 +238,19 @@ __global__ __launch_bounds__(256) void xent_zero(uint32_t* __restrict__ out, int
 
 // ---- sizes -------------------------------------------------------------------------------
 
-constexpr int64_t kPieceBytes = 256LL << 20;  // of G: what the Infinity Cache holds
+// G's piece.  Larger pieces cost dx fewer additions and leave fewer part-filled rounds of
+// tiles; that G then no longer fits the Infinity Cache does not show, the products being
+// bound by the matrix cores.  Backward on MI355X, us for pieces of 64 / 128 / 256 / 512 MiB / 1 GiB: 8192
+// tokens x 4096 x 131072 22842 / 21095 / 20474 / 20068 / 20073; 4099 x 2048 x 50257 (pieces of
+// 8192 / 16384 / 32768 rows, one piece) 2843 / 2805 / 2698 / 2444.
+constexpr int64_t kPieceBytes = 512LL << 20;
 constexpr int64_t kMaxOperand = 1LL << 30;    // values a product's 31-bit offsets reach
 constexpr int64_t kMaxPiece = 1LL << 20;      // vocabulary rows, 32 per grid row of the fp32 kernels
 constexpr int64_t kMaxTokens = 1LL << 24;     // a workgroup per token within a grid
+
+// G's rows are padded to whole 128-byte lines of bf16: the products fetch 128 bytes of
+// a row at a time, which at any other pitch straddle two lines.
+constexpr int64_t kLine = 64;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 inline size_t region(int64_t bytes) { return static_cast<size_t>(up(bytes, 256)); }
@@ -250,10 +258,10 @@ inline size_t region(int64_t bytes) { return static_cast<size_t>(up(bytes, 256))
 // The vocabulary rows of a piece: `asked`, or what fills kPieceBytes, cut to equal
 // pieces of whole 256-row tiles that the products' offsets reach.
 inline int64_t piece_rows(int64_t rows, int64_t vocab, int64_t ldw, int size, int64_t asked) {
-    const int64_t row_bytes = up(rows, 8) * size;
+    const int64_t row_bytes = up(rows, kLine) * size;
     int64_t p = asked > 0 ? up(std::min(asked, vocab), 256) : kPieceBytes / row_bytes;
     p = std::min(p, kMaxPiece);
-    if (size == 2) p = std::min(p, std::min(kMaxOperand / ldw, kMaxOperand / up(rows, 8)));
+    if (size == 2) p = std::min(p, std::min(kMaxOperand / ldw, kMaxOperand / up(rows, kLine)));
     p = std::max<int64_t>(p / 256 * 256, 256);
     if (p >= vocab) return vocab;
     const int64_t n = (vocab + p - 1) / p;
@@ -269,6 +277,9 @@ inline int lse_shape(int64_t rows, int64_t vocab, int64_t cols) {
     if ((s != 7 && s != 8) || rows <= kFewTokens) return s;
     return agk::grid_fits(((vocab + 127) / 128) * ((rows + 63) / 64), 256) ? 6 : kRingLargest;
 }
+constexpr int64_t kMaxSlices = 32, kMinSlice = 512;
+constexpr double kRoundUs = 5.0;
+
 // Vocabulary rows of one wave's block.
 inline int lse_block(int shape) {
     switch (shape) {
@@ -286,33 +297,61 @@ inline int64_t max_blocks(int64_t rows, int64_t vocab, int dtype) {
     return (vocab + least - 1) / least;
 }
 
-// K slices of dx = G w, K = the piece's vocabulary rows: few tokens make few tiles, so K
-// is cut until the tiles fill the CUs, in slices of at least 512.
+// The tile and K slices of dx = G w.  K is the piece's vocabulary rows, far longer than
+// the tokens by cols output is large: tiles that fill the last round of CUs badly are cut along K
+// until they fill it, each slice with an fp32 output of its own (xent_dx_out adds
+// them in order).  The cost: the tile rule's (pick_shape) per 64-deep step, plus what a
+// round costs besides (its first loads and its stores) and the slices' traffic.
 struct DxPlan {
     int shape, slices, k_slice;
 };
 inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k) {
     using namespace agk_gemm;
-    DxPlan d;
-    d.shape = pick_shape(rows8, cols, k, device_cus());
-    d.slices = 1;
-    d.k_slice = static_cast<int>(up(k, 64));
+    const int64_t cus = device_cus();
+    DxPlan best{pick_shape(rows8, cols, k, device_cus()), 1, static_cast<int>(up(k, 64))};
+    double best_cost = 1e30;
     for (const RingCost& s : kRingCosts) {
-        if (s.id != d.shape || s.id == 0) continue;
         const int64_t tiles = ((rows8 + s.bm - 1) / s.bm) * ((cols + s.bn - 1) / s.bn);
-        const int64_t most = k / 512, want = static_cast<int64_t>(device_cus()) * s.per_cu / tiles;
-        const int64_t n = std::min(most, want);
-        if (n > 1) {
-            d.k_slice = static_cast<int>(up((k + n - 1) / n, 64));
-            d.slices = static_cast<int>((k + d.k_slice - 1) / d.k_slice);
+        const double slots = static_cast<double>(cus * s.per_cu);
+        for (int64_t n = 1; n <= kMaxSlices && (n == 1 || n * kMinSlice <= k); ++n) {
+            if (k < BK || !agk::grid_fits(tiles, 256)) break;
+            const int64_t ks = up((k + n - 1) / n, 64), m = (k + ks - 1) / ks;
+            if (m != n || k - (n - 1) * ks < BK) continue;  // every slice has a whole k-tile
+            const double load = static_cast<double>(tiles * n) / slots;
+            const double rounds = static_cast<double>(static_cast<int64_t>(load));
+            const double fill = load - rounds;
+            const double steps = static_cast<double>(ks) / 64;
+            // the 256 x 256 kernel on two k-strided operands and a long K: 1.36 us a step at 53 %
+            // fill, 1.64-1.70 full
+            const double light = s.id == 0 ? 1.25 : s.light, full = s.id == 0 ? 1.65 : s.full;
+            const double step =
+                rounds * full + (fill > 0 ? light + (full - light) * fill * fill : 0.0);
+            const double cost = step * steps + (rounds + (fill > 0)) * kRoundUs +
+                                static_cast<double>(n * rows8 * cols) * 8 / 5e6;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = DxPlan{s.id, static_cast<int>(n), static_cast<int>(ks)};
+            }
         }
     }
+    return best;
+}
+
+// The plan for the last piece, of n rows: as many of the slices as leave each a whole k-tile.
+inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
+    DxPlan d = plan;
+    for (;; --d.slices) {
+        d.k_slice = static_cast<int>(up((n + d.slices - 1) / d.slices, 64));
+        d.slices = static_cast<int>((n + d.k_slice - 1) / d.k_slice);
+        if (d.slices == 1 || n - (d.slices - 1) * static_cast<int64_t>(d.k_slice) >= 64) break;
+    }
+    if (n < 64) d.shape = agk_gemm::kRingSmallK;
     return d;
 }
 
 // The backward's workspace.
 struct Layout {
-    int64_t piece, rows8;
+    int64_t piece, rows8, ldg;
     size_t weight, alpha, keep, g, acc, total;
 };
 inline Layout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t ldw, int dtype,
@@ -320,12 +359,13 @@ inline Layout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t ldw,
     Layout o;
     const int size = dtype == AGK_F32 ? 4 : 2;
     o.rows8 = up(rows, 8);
+    o.ldg = dtype == AGK_F32 ? rows : up(rows, kLine);
     o.piece = piece_rows(rows, vocab, ldw, size, piece);
     o.weight = 0;
     o.alpha = o.weight + region(o.rows8 * 4);
     o.keep = o.alpha + region(4);
     o.g = o.keep + region(rows * cols * size);
-    o.acc = o.g + region(o.piece * o.rows8 * size);
+    o.acc = o.g + region(o.piece * o.ldg * size);
     o.total = o.acc;
     if (dtype == AGK_BF16) {
         const DxPlan d = dx_plan(o.rows8, cols, o.piece);
@@ -505,9 +545,9 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         if ((rc = check_launch()) != AGK_OK) return rc;
     }
     const int cus = agk_gemm::device_cus();
-    int slices = 1;
     const int64_t slice = o.rows8 * cols;
-    if (bf16) slices = dx_plan(o.rows8, cols, o.piece).slices;
+    DxPlan plan{0, 1, 0};
+    if (bf16) plan = dx_plan(o.rows8, cols, o.piece);
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
         if (!bf16) {
@@ -537,21 +577,19 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         }
         const uint16_t* const wp = static_cast<const uint16_t*>(w) + v0 * ldw;
         uint16_t* const g = reinterpret_cast<uint16_t*>(ws + o.g);
-        const int ldg = static_cast<int>(o.rows8), m = static_cast<int>(n);
+        const int ldg = static_cast<int>(o.ldg), m = static_cast<int>(n);
         const Product zp{wp, ldw, static_cast<const uint16_t*>(x), ldx, m, static_cast<int>(rows),
                          static_cast<int>(cols), 1, 0, st};
         const GradEpi ge{g, in, weight, labels, v0, ldg, m, static_cast<int>(rows)};
         rc = launch_grad(agk_gemm::pick_shape(n, rows, cols, cus), zp, ge);
         if (rc != AGK_OK) return rc;
         if (dx) {
-            DxPlan d = dx_plan(o.rows8, cols, o.piece);
-            // the last piece may be short of a whole slice for each
-            d.k_slice = static_cast<int>(up((n + slices - 1) / slices, 64));
-            d.slices = static_cast<int>((n + d.k_slice - 1) / d.k_slice);
-            if (n < 64) d.shape = agk_gemm::pick_shape(o.rows8, cols, n, cus);  // no whole k-tile
-            const Product dp{g, ldg, wp, ldw, ldg, static_cast<int>(cols), m, d.slices, d.k_slice,
+            DxPlan d = plan;
+            if (n != o.piece) d = last_piece(plan, n);
+            const int m8 = static_cast<int>(o.rows8);
+            const Product dp{g, ldg, wp, ldw, m8, static_cast<int>(cols), m, d.slices, d.k_slice,
                              st};
-            const AddEpi<true> de{acc, cols, slice, nullptr, ldg, static_cast<int>(cols), v0 > 0};
+            const AddEpi<true> de{acc, cols, slice, nullptr, m8, static_cast<int>(cols), v0 > 0};
             if ((rc = launch_dx(d.shape, dp, de)) != AGK_OK) return rc;
         }
         if (dw) {
@@ -571,7 +609,7 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     if (bf16 && dx) {
         const int64_t n8 = rows * cols / 8;
         hipLaunchKernelGGL(xent_dx_out, dim3(static_cast<unsigned>((n8 + 255) / 256)), dim3(256), 0,
-                           st, acc, slices, slice, alpha, weight, static_cast<uint16_t*>(dx), n8,
+                           st, acc, plan.slices, slice, alpha, weight, static_cast<uint16_t*>(dx), n8,
                            static_cast<int>(cols / 8), acc_dx);
         return check_launch();
     }

@@ -46,13 +46,55 @@ __device__ __forceinline__ int label_row(int64_t label, int64_t row0, int rows) 
     return r >= 0 && r < rows ? static_cast<int>(r) : -1;
 }
 
+// max(a, b, c) in one instruction.
+__device__ __forceinline__ float max3_of(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // Forward: the block's maximum and sum of exponentials of each token, and the logit
 // of its label.  part[(row0 / block rows) * tokens + token] = {max, sum of exp(z - max)}.
+//
+// One wave per SIMD runs this while the matrix cores wait, so it is kept short: two
+// maxima per instruction, one fma, one exponential and one addition per logit, in four
+// chains.  The fma takes z log2(e) - t, t = m log2(e) rounded; the rounding, exact as
+// another fma, goes into the sum as a factor.
 struct LseEpi {
     float2* part;
     float* picked;
     const int64_t* labels;
     int vocab, tokens;
+
+    template <bool INNER, int TMW, int TNW>
+    __device__ __forceinline__ float2 reduce(const f32x16 (&acc)[TMW][TNW], int j, int left,
+                                             int half) const {
+        constexpr float kNone = -__builtin_inff();
+        // rows past the vocabulary: the smallest value, so that the sums below leave them out
+        auto at = [&](int i, int e) -> float {
+            if constexpr (INNER) return acc[i][j][e];
+            else return acc_row(i, e, half) < left ? acc[i][j][e] : kNone;
+        };
+        float m4[4] = {kNone, kNone, kNone, kNone};
+#pragma unroll
+        for (int i = 0; i < TMW; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2)
+                m4[(e / 2) & 3] = max3_of(m4[(e / 2) & 3], at(i, e), at(i, e + 1));
+        float m = max_of(max_of(m4[0], m4[1]), max_of(m4[2], m4[3]));
+        m = max_of(m, other_half(m));
+        const float t = m == kNone ? 0.0f : m * kLog2e;  // no -inf - -inf
+        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < TMW; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                s4[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(at(i, e), kLog2e, -t));
+        float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        s += other_half(s);
+        if (m != kNone) s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -t));
+        return make_float2(m, s);
+    }
 
     template <int TMW, int TNW>
     __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
@@ -64,38 +106,11 @@ struct LseEpi {
 #pragma unroll
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
-            float m = -__builtin_inff();
-            if (inner) {
-#pragma unroll
-                for (int i = 0; i < TMW; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) m = max_of(m, acc[i][j][e]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < TMW; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (row0 + acc_row(i, e, half) < vocab) m = max_of(m, acc[i][j][e]);
-            }
-            m = max_of(m, other_half(m));
-            const float shift = m == -__builtin_inff() ? 0.0f : m;  // no -inf - -inf
-            float s = 0.0f;
-            if (inner) {
-#pragma unroll
-                for (int i = 0; i < TMW; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s += exp_of(acc[i][j][e] - shift);
-            } else {
-#pragma unroll
-                for (int i = 0; i < TMW; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (row0 + acc_row(i, e, half) < vocab) s += exp_of(acc[i][j][e] - shift);
-            }
-            s += other_half(s);
             const bool in = col < tokens;
-            if (in && half == 0) out[col] = make_float2(m, s);
             const int at = in ? label_row(labels[col], row0, TMW * 32) : -1;
+            const float2 v = inner ? reduce<true>(acc, j, 0, half)
+                                   : reduce<false>(acc, j, vocab - row0, half);
+            if (in && half == 0) out[col] = v;
             if (__any(at >= 0)) {
 #pragma unroll
                 for (int i = 0; i < TMW; ++i)
@@ -110,7 +125,11 @@ struct LseEpi {
 
 // Backward: G^T, weight * (softmax - [label]), rounded to bf16: rows v0 .. of the
 // vocabulary as rows of ldg tokens, zeros in the columns from `tokens` to ldg (the
-// padding that makes ldg a multiple of 8: the product over tokens reads it).
+// padding of G's rows: the product over tokens reads up to 7 of them).
+//
+// One fma, one exponential and one product per logit; exp(z - m - l) takes m + l rounded once
+// (2^-24 of its size: far below G's rounding to bf16).  Lanes c and c + 1 exchange rows e
+// and e + 1, so that a store is 4 bytes of two neighbouring tokens.
 struct GradEpi {
     uint16_t* G;
     const float2* stats;
@@ -123,8 +142,10 @@ struct GradEpi {
     __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
                                                int lane) const {
         if (row0 >= rows) return;
-        const int half = lane >> 5;
+        const int half = lane >> 5, odd = lane & 1;
         const bool inner = row0 + TMW * 32 <= rows;
+        // even lanes: {own low, neighbour's low}; odd lanes: {neighbour's high, own high}
+        const uint32_t pick = odd ? 0x07060302u : 0x01000504u;
 #pragma unroll
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
@@ -133,21 +154,31 @@ struct GradEpi {
             const float w = in ? weight[col] : 0.0f;
             const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
             const bool hit = __any(at >= 0);
-            if (col < ldg) {
-                uint16_t* const out = G + col;
+            const bool some_out = __any(w == 0.0f);
+            const float shift = (st.x + st.y) * kLog2e;
+            const bool store = col < ldg;  // ldg is even: a pair is in or out
+            uint16_t* const out = G + (col & ~1) + static_cast<int64_t>(row0 + odd) * ldg;
 #pragma unroll
-                for (int i = 0; i < TMW; ++i)
+            for (int i = 0; i < TMW; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int r = acc_row(i, e, half);
-                        float p = exp_of((acc[i][j][e] - st.x) - st.y);
-                        if (hit) p -= at == r ? 1.0f : 0.0f;
-                        const float g = w != 0.0f ? w * p : 0.0f;
-                        if (inner || row0 + r < rows)
-                            out[static_cast<int64_t>(row0 + r) * ldg] =
-                                static_cast<uint16_t>(agk_gemm::f32_to_bf16_bits(g));
+                for (int e = 0; e < 16; e += 2) {
+                    const int r = acc_row(i, e, half);
+                    float g[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float p = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(acc[i][j][e + u], kLog2e, -shift));
+                        if (hit) p -= at == r + u ? 1.0f : 0.0f;
+                        g[u] = w * p;
+                        if (some_out) g[u] = w != 0.0f ? g[u] : 0.0f;  // z may be NaN there
                     }
-            }
+                    const uint32_t own = agk_gemm::pack_bf16(g[0], g[1]);
+                    const uint32_t other = static_cast<uint32_t>(
+                        __builtin_amdgcn_mov_dpp(static_cast<int>(own), 0xb1, 0xf, 0xf, true));
+                    const uint32_t v = __builtin_amdgcn_perm(own, other, pick);
+                    if (store && (inner || row0 + r + odd < rows))
+                        *reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(r) * ldg) = v;
+                }
         }
     }
 };
@@ -232,13 +263,27 @@ int launch_dw(int shape, const Product& p, const AddEpi<false>& e);
 
 namespace agk_xent {
 
+// Moves the operands to this grid row's K slice; its length.  (A kernel built for a K tail
+// that the last slice alone has stages it for the others too, from the k that follow
+// them, as zeros.)
+template <bool A_TR, bool B_TR>
+__device__ __forceinline__ int slice_of(const uint16_t* __restrict__& A, int64_t lda,
+                                        const uint16_t* __restrict__& B, int64_t ldb, int K,
+                                        int k_slice) {
+    const int k0 = static_cast<int>(blockIdx.y) * k_slice;
+    A += A_TR ? static_cast<int64_t>(k0) * lda : k0;
+    B += B_TR ? static_cast<int64_t>(k0) * ldb : k0;
+    return blockIdx.y + 1 < gridDim.y ? k_slice : K - k0;
+}
+
 template <bool A_TR, bool B_TR, bool TAIL, class Epi>
 __global__ __launch_bounds__(agk_gemm::kDirectThreads) void xent_direct_kernel(
     const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
-    int N, int K, const Epi epi, int tiles_m, int tiles_n, int full_tiles) {
+    int N, int K, int k_slice, const Epi epi, int tiles_m, int tiles_n, int full_tiles) {
     __shared__ __attribute__((aligned(16))) uint16_t st0[agk_gemm::kStageElems];
     __shared__ __attribute__((aligned(16))) uint16_t st1[agk_gemm::kStageElems];
-    agk_gemm::direct_body<A_TR, B_TR, TAIL>(A, lda, B, ldb, M, N, K, tiles_m, tiles_n,
+    const int k = slice_of<A_TR, B_TR>(A, lda, B, ldb, K, k_slice);
+    agk_gemm::direct_body<A_TR, B_TR, TAIL>(A, lda, B, ldb, M, N, k, tiles_m, tiles_n,
                                             agk_gemm::kGroupM, full_tiles, st0, st1, epi);
 }
 
@@ -246,10 +291,7 @@ template <bool A_TR, bool B_TR, class SH, class Epi>
 __global__ __launch_bounds__(256, SH::kPerCu) void xent_ring_kernel(
     const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
     int N, int K, int k_slice, const Epi epi, int tiles_m, int tiles_n) {
-    const int k0 = static_cast<int>(blockIdx.y) * k_slice;
-    A += A_TR ? static_cast<int64_t>(k0) * lda : k0;
-    B += B_TR ? static_cast<int64_t>(k0) * ldb : k0;
-    const int k = blockIdx.y + 1 < gridDim.y ? k_slice : K - k0;
+    const int k = slice_of<A_TR, B_TR>(A, lda, B, ldb, K, k_slice);
     agk_gemm::ring_body<A_TR, B_TR, SH>(A, lda, B, ldb, M, N, k, tiles_m, tiles_n,
                                         agk_gemm::kGroupM, epi);
 }
@@ -260,14 +302,14 @@ int launch_product(int shape, const Product& p, const Epi& e) {
     if (shape == 0) {
         const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
         const int tiles = tiles_m * tiles_n;
-        const int full = direct_full_tiles(tiles, device_cus());
-        const dim3 grid(full + 2 * (tiles - full)), block(kDirectThreads);
+        const int full = p.slices > 1 ? tiles : direct_full_tiles(tiles, device_cus());
+        const dim3 grid(full + 2 * (tiles - full), p.slices), block(kDirectThreads);
         if (p.K % BK != 0)
             hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, true, Epi>), grid, block, 0, p.st,
-                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, e, tiles_m, tiles_n, full);
+                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, tiles_m, tiles_n, full);
         else
             hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, false, Epi>), grid, block, 0, p.st,
-                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, e, tiles_m, tiles_n, full);
+                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, tiles_m, tiles_n, full);
         return agk::check_launch();
     }
 #define AGK_XENT_CASE(ID, BM_, BN_, WVM, NST)                                                    \

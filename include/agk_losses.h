@@ -53,7 +53,7 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
  *     G = dloss * (exp((z - m) - l) - [column == label])
  *     dx (+)= G w,   dw (+)= G^T x
  * with z computed again, `piece` vocabulary rows at a time (0: as many as make
- * G's piece about 256 MiB; others are rounded up to a multiple of 256).  Rows
+ * G's piece about 512 MiB; others are rounded up to a multiple of 256).  Rows
  * whose label is negative or whose dloss is 0 are left out: dx (+)= 0 and
  * nothing in dw.
  * dx [rows][cols] of `dtype`; dw [vocab][cols] of dw_dtype (AGK_F32, or

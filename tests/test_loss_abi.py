@@ -113,7 +113,7 @@ def test_linear_xent_more_validation():
     assert f(9, 9, 8, 3) == 0 and b(9, 9, 8, 3, 0) == 0
     # the logits of all tokens would be 4096 x 131072 x 4 bytes
     assert 0 < f(4096, 131072, 4096, BF16) < 4096 * 131072 * 4 // 16
-    assert 0 < b(4096, 131072, 4096, BF16, 0) < 512 << 20
+    assert 0 < b(4096, 131072, 4096, BF16, 0) < 768 << 20
     assert b(4096, 131072, 4096, BF16, 256) < b(4096, 131072, 4096, BF16, 0)
     assert b(4096, 131072, 4096, BF16, 1) == b(4096, 131072, 4096, BF16, 256)
 
