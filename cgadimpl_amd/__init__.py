@@ -829,32 +829,42 @@ def logsumexp_jvp(z, tz, ty=None, stream=None):
 
 # ---- LayerNorm with weight and bias (include/agk_rowops.h) ------------------------
 
-def _want(t, name, like, shape, dtype):
-    """Checks one operand: a contiguous GPU tensor of `dtype` and `shape` (numel where shape is
-    an int) on the device of `like`, which must be the current one."""
-    if t.dtype != dtype:
+def _want(t, name, dev, n, dtype):
+    """Checks one operand: n values of `dtype` on device `dev` (_ptr checks that it is contiguous)."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
-    if (t.numel() != shape) if isinstance(shape, int) else (tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {like.device}")
+    if t.numel() != n:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {n} values")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{dev}")
 
 
-def _want_current(t):
-    """The kernels run on the current device's current stream: the tensors have to be there."""
-    if not t.is_cuda:
+_current_device = None
+
+
+def _want_current(t) -> int:
+    """The device of t, which has to be the current one: the kernels run on its current stream."""
+    global _current_device
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("tensor must live on the GPU")
-    if t.device.index != _torch().cuda.current_device():
-        raise ValueError(f"tensors on {t.device} while another device is current")
+    if _current_device is None:
+        torch = _torch()
+        torch.cuda.init()
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    if dev != _current_device():
+        raise ValueError(f"tensors on {t.device} while cuda:{_current_device()} is current")
+    return dev
 
 
 def _scratch(workspace, need, like):
     """(workspace, bytes): the caller's tensor, or what the call needs."""
     if workspace is None:
         workspace = _empty((need,), _torch().uint8, like) if need else None
-    elif workspace.device != like.device:
+        return workspace, need
+    if workspace.device != like.device:
         raise ValueError("the workspace is on another device")
-    return workspace, workspace.numel() * workspace.element_size() if workspace is not None else 0
+    return workspace, workspace.numel() * workspace.element_size()
 
 
 def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None,
@@ -862,17 +872,24 @@ def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, r
     """y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis (gamma, beta: [cols] of
     x's dtype, or None); returns (y, mean, rstd), the statistics float32 [..., 1]."""
     torch = _torch()
-    _want_current(x)
+    dev = _want_current(x)
     rows, cols = _rows_cols(x)
-    for t, name in ((gamma, "gamma"), (beta, "beta")):
-        if t is not None:
-            _want(t, name, x, cols, x.dtype)
-    y = torch.empty_like(x) if y is None else y
-    mean = _row_stat_like(x, torch.float32) if mean is None else mean
-    rstd = _row_stat_like(x, torch.float32) if rstd is None else rstd
-    _want(y, "y", x, x.numel(), x.dtype)
-    _want(mean, "mean", x, rows, torch.float32)
-    _want(rstd, "rstd", x, rows, torch.float32)
+    if gamma is not None:
+        _want(gamma, "gamma", dev, cols, x.dtype)
+    if beta is not None:
+        _want(beta, "beta", dev, cols, x.dtype)
+    if y is None:
+        y = torch.empty_like(x)
+    else:
+        _want(y, "y", dev, x.numel(), x.dtype)
+    if mean is None:
+        mean = _row_stat_like(x, torch.float32)
+    else:
+        _want(mean, "mean", dev, rows, torch.float32)
+    if rstd is None:
+        rstd = _row_stat_like(x, torch.float32)
+    else:
+        _want(rstd, "rstd", dev, rows, torch.float32)
     rc = lib().agk_layernorm_affine_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean),
                                         _ptr(rstd), rows, cols, float(eps), _dtype_code(x),
                                         _stream(stream))
@@ -886,28 +903,33 @@ def layernorm_affine_bwd(x, gamma, mean, rstd, dy, dx=None, dgamma=None, dbeta=N
     """VJP of layernorm_affine_fwd: (dx, dgamma, dbeta), None where not wanted; dgamma and dbeta
     float32 [cols].  accumulate: a bool (every output) or AGK_ACCUM_DX / _DGAMMA / _DBETA bits."""
     torch = _torch()
-    _want_current(x)
+    dev = _want_current(x)
     rows, cols = _rows_cols(x)
     acc = (7 if accumulate else 0) if isinstance(accumulate, bool) else int(accumulate)
-    if want_dx and dx is None:
-        dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
-    new = torch.zeros if acc else torch.empty
-    if want_dgamma and dgamma is None:
-        dgamma = new(cols, dtype=torch.float32, device=x.device)
-    if want_dbeta and dbeta is None:
-        dbeta = new(cols, dtype=torch.float32, device=x.device)
-    _want(dy, "dy", x, x.numel(), x.dtype)
-    _want(mean, "mean", x, rows, torch.float32)
-    _want(rstd, "rstd", x, rows, torch.float32)
+    _want(dy, "dy", dev, x.numel(), x.dtype)
+    _want(mean, "mean", dev, rows, torch.float32)
+    _want(rstd, "rstd", dev, rows, torch.float32)
     if gamma is not None:
-        _want(gamma, "gamma", x, cols, x.dtype)
+        _want(gamma, "gamma", dev, cols, x.dtype)
     if dx is not None:
-        _want(dx, "dx", x, x.numel(), x.dtype)
+        _want(dx, "dx", dev, x.numel(), x.dtype)
+    elif want_dx:
+        dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
+    if dgamma is not None:
+        _want(dgamma, "dgamma", dev, cols, torch.float32)
+    elif want_dgamma:
+        dgamma = _empty((cols,), torch.float32, x)
+        if acc & AGK_ACCUM_DGAMMA:
+            dgamma.zero_()
+    if dbeta is not None:
+        _want(dbeta, "dbeta", dev, cols, torch.float32)
+    elif want_dbeta:
+        dbeta = _empty((cols,), torch.float32, x)
+        if acc & AGK_ACCUM_DBETA:
+            dbeta.zero_()
     need = 0
-    for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
-        if t is not None:
-            _want(t, name, x, cols, torch.float32)
-            need = int(lib().agk_layernorm_affine_bwd_workspace_bytes(rows, cols))
+    if dgamma is not None or dbeta is not None:
+        need = lib().agk_layernorm_affine_bwd_workspace_bytes(rows, cols)
     ws, ws_bytes = _scratch(workspace, need, x)
     rc = lib().agk_layernorm_affine_bwd(_ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dy),
                                         _ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(ws), ws_bytes,
@@ -919,14 +941,28 @@ def layernorm_affine_bwd(x, gamma, mean, rstd, dy, dx=None, dgamma=None, dbeta=N
 # ---- losses (include/agk_losses.h) --------------------------------------------------
 
 def _xent_sizes(x, w, labels):
-    torch = _torch()
-    _want_current(x)
+    dev = _want_current(x)
     if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1]:
         raise ValueError("expected x [..., cols] and w [vocab, cols]")
-    rows, cols = _rows_cols(x)
-    _want(w, "w", x, w.shape, x.dtype)
-    _want(labels, "labels", x, x.shape[:-1], torch.int64)
-    return rows, w.shape[0], cols
+    if labels.shape != x.shape[:-1]:
+        raise ValueError("expected one label for each row of x")
+    rows, cols = labels.numel(), x.shape[-1]
+    _want(w, "w", dev, w.numel(), x.dtype)
+    _want(labels, "labels", dev, rows, _torch().int64)
+    return dev, rows, w.shape[0], cols
+
+
+def _loss_and_stats(shape, rows, dev, like, loss, stats):
+    f32 = _torch().float32
+    if loss is None:
+        loss = _empty(shape, f32, like)
+    else:
+        _want(loss, "loss", dev, rows, f32)
+    if stats is None:
+        stats = _empty(shape + (2,), f32, like)
+    else:
+        _want(stats, "stats", dev, 2 * rows, f32)
+    return loss, stats
 
 
 def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None, stream=None):
@@ -935,14 +971,11 @@ def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None
     a row without a loss.  Returns (loss, stats): float32 [...] and [..., 2] (each row's maximum
     logit and log of its sum of exponentials above it, for the backward)."""
     torch = _torch()
-    rows, vocab, cols = _xent_sizes(x, w, labels)
-    loss = _empty(x.shape[:-1], torch.float32, x) if loss is None else loss
-    stats = _empty(x.shape[:-1] + (2,), torch.float32, x) if stats is None else stats
-    _want(loss, "loss", x, rows, torch.float32)
-    _want(stats, "stats", x, 2 * rows, torch.float32)
+    dev, rows, vocab, cols = _xent_sizes(x, w, labels)
+    loss, stats = _loss_and_stats(labels.shape, rows, dev, x, loss, stats)
     dt = _dtype_code(x)
-    ws, ws_bytes = _scratch(workspace, int(lib().agk_linear_xent_fwd_workspace_bytes(
-        rows, vocab, cols, dt)), x)
+    ws, ws_bytes = _scratch(workspace, lib().agk_linear_xent_fwd_workspace_bytes(
+        rows, vocab, cols, dt), x)
     rc = lib().agk_linear_xent_fwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(loss),
                                    _ptr(stats), _ptr(ws), ws_bytes, rows, vocab, cols, dt,
                                    _stream(stream))
@@ -958,22 +991,22 @@ def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dt
     dw) says otherwise.  accumulate: a bool (both) or AGK_ACCUM_DX / AGK_ACCUM_DGAMMA (dw) bits.
     piece: vocabulary rows whose logits exist at a time (0: the library's choice)."""
     torch = _torch()
-    rows, vocab, cols = _xent_sizes(x, w, labels)
+    dev, rows, vocab, cols = _xent_sizes(x, w, labels)
     acc = _accum_flags(accumulate)
-    if want_dx and dx is None:
+    _want(stats, "stats", dev, 2 * rows, torch.float32)
+    _want(dloss, "dloss", dev, rows, torch.float32)
+    if dx is not None:
+        _want(dx, "dx", dev, x.numel(), x.dtype)
+    elif want_dx:
         dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
-    if want_dw and dw is None:
+    if dw is not None:
+        _want(dw, "dw", dev, w.numel(), dw_dtype or dw.dtype)
+    elif want_dw:
         new = torch.zeros if acc & AGK_ACCUM_DGAMMA else torch.empty
         dw = new(vocab, cols, dtype=dw_dtype or torch.float32, device=x.device)
-    _want(stats, "stats", x, 2 * rows, torch.float32)
-    _want(dloss, "dloss", x, rows, torch.float32)
-    if dx is not None:
-        _want(dx, "dx", x, x.numel(), x.dtype)
-    if dw is not None:
-        _want(dw, "dw", x, (vocab, cols), dw_dtype or dw.dtype)
     dt = _dtype_code(x)
-    ws, ws_bytes = _scratch(workspace, int(lib().agk_linear_xent_bwd_workspace_bytes(
-        rows, vocab, cols, dt, piece)), x)
+    ws, ws_bytes = _scratch(workspace, lib().agk_linear_xent_bwd_workspace_bytes(
+        rows, vocab, cols, dt, piece), x)
     rc = lib().agk_linear_xent_bwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(stats),
                                    _ptr(dloss), _ptr(dx), _ptr(dw),
                                    _dtype_code(dw) if dw is not None else AGK_F32, _ptr(ws),
@@ -983,16 +1016,16 @@ def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dt
 
 
 def _distill_sizes(z, index, teacher):
-    torch = _torch()
-    _want_current(z)
+    dev = _want_current(z)
     if z.dim() < 1 or index.dim() != z.dim() or index.shape[:-1] != z.shape[:-1]:
         raise ValueError("expected z [..., cols] and index [..., k]")
-    _want(index, "index", z, index.shape, torch.int64)
-    _want(teacher, "teacher", z, index.shape, teacher.dtype)
-    rows = 1
-    for n in z.shape[:-1]:
-        rows *= n
-    return rows, z.shape[-1], index.shape[-1]
+    cols, k = z.shape[-1], index.shape[-1]
+    rows = z.numel() // cols if cols else index.shape[:-1].numel()
+    _want(index, "index", dev, rows * k, _torch().int64)
+    _want(teacher, "teacher", dev, rows * k, teacher.dtype)
+    if teacher.shape != index.shape:
+        raise ValueError("expected teacher [..., k]")
+    return dev, rows, cols, k
 
 
 def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, stats=None,
@@ -1001,13 +1034,9 @@ def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, sta
     over the row's k named columns (agk_distill_topk_fwd): z [..., cols], index int64 [..., k] (a
     negative one is an empty entry), teacher [..., k] float32 or bfloat16.  Returns (loss, stats):
     float32 [...] and [..., 2]."""
-    torch = _torch()
-    rows, cols, k = _distill_sizes(z, index, teacher)
-    loss = _empty(z.shape[:-1], torch.float32, z) if loss is None else loss
-    stats = _empty(z.shape[:-1] + (2,), torch.float32, z) if stats is None else stats
-    _want(loss, "loss", z, rows, torch.float32)
-    _want(stats, "stats", z, 2 * rows, torch.float32)
-    ws, ws_bytes = _scratch(workspace, int(lib().agk_distill_topk_workspace_bytes(rows, cols)), z)
+    dev, rows, cols, k = _distill_sizes(z, index, teacher)
+    loss, stats = _loss_and_stats(z.shape[:-1], rows, dev, z, loss, stats)
+    ws, ws_bytes = _scratch(workspace, lib().agk_distill_topk_workspace_bytes(rows, cols), z)
     rc = lib().agk_distill_topk_fwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(loss), _ptr(stats),
                                     _ptr(ws), ws_bytes, rows, cols, k, float(temperature),
                                     _dtype_code(z), _dtype_code(teacher), _stream(stream))
@@ -1020,11 +1049,13 @@ def distill_topk_bwd(z, index, teacher, stats, dloss, temperature: float = 1.0, 
     """Gradient of z for dloss, the float32 gradient of each row's loss: dz (+)= dloss * T *
     (q - p at the named columns) (agk_distill_topk_bwd).  dz may be z (in place)."""
     torch = _torch()
-    rows, cols, k = _distill_sizes(z, index, teacher)
-    dz = (torch.zeros_like(z) if accumulate else torch.empty_like(z)) if dz is None else dz
-    _want(stats, "stats", z, 2 * rows, torch.float32)
-    _want(dloss, "dloss", z, rows, torch.float32)
-    _want(dz, "dz", z, z.numel(), z.dtype)
+    dev, rows, cols, k = _distill_sizes(z, index, teacher)
+    _want(stats, "stats", dev, 2 * rows, torch.float32)
+    _want(dloss, "dloss", dev, rows, torch.float32)
+    if dz is None:
+        dz = torch.zeros_like(z) if accumulate else torch.empty_like(z)
+    else:
+        _want(dz, "dz", dev, z.numel(), z.dtype)
     rc = lib().agk_distill_topk_bwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(stats), _ptr(dloss),
                                     _ptr(dz), rows, cols, k, float(temperature), _dtype_code(z),
                                     _dtype_code(teacher), _acc_dx(accumulate), _stream(stream))

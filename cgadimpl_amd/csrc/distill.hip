@@ -7,8 +7,8 @@
 // Both passes stream z: the forward reads it once, keeping a running maximum and sum
 // per lane, the backward reads it once and writes dz.  The teacher's part is a few
 // hundred values a row.  HBM bounds them.  A row is one workgroup's; rows too few to fill the chip are
-// cut into segments, whose {max, sum} meet in a second kernel (forward), or which
-// are independent, each computing the row's p again (backward).
+// cut into segments, whose {max, sum} meet in a second kernel (forward); the backward takes
+// a row in chunks always, each computing the row's p again.
 
 #include <hip/hip_runtime.h>
 
@@ -317,127 +317,160 @@ __global__ __launch_bounds__(kLanes) void distill_join(const Args a, const float
     row_loss<S, PER>(a, row, m, s, loss, stats, red);
 }
 
-// dz of one segment of one row.  The columns that the teacher named are stored twice, as
-// q first and then, after every store of the segment, with their p subtracted.  A bit map of the
-// segment's columns finds whether any is named twice; only then are the entries
-// compared with each other.  (bf16 96 x 131072, k = 256: 56 us comparing always.)
-constexpr int kMapBits = 1 << 16;  // columns that far apart share a bit
+// ---- backward ------------------------------------------------------------------------
+// One wave per chunk of kChunk 16-byte slots of a row, four chunks in a row per workgroup
+// and no barrier: a stream of reads and writes runs fastest where the chip works through
+// memory in one compact window (copies: 6.05 TB/s with 16 KiB per workgroup, 4.2-5.2 with
+// workgroups that loop over long rows).  The wave issues its loads of z behind those of the
+// row's teacher and computes p for itself while they are in flight (PER entries per lane, a
+// maximum and a sum over the wave).  The entries whose column lies in the chunk are then taken one by one, in order:
+// the column's slot and element are the same for the whole wave, so that one lane's
+// register takes - c p.  Columns named twice need nothing more.
+constexpr int kSlots = 4;              // 16-byte slots per lane
+constexpr int kChunk = 64 * kSlots;    // and per wave
+
 template <class S, int PER, bool ACC>
-__global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : 4) void distill_bwd(const Args a, const float2* __restrict__ stats,
-                                                      const float* __restrict__ dloss, void* dz_) {
+__global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) void distill_bwd(
+    const Args a, const float2* __restrict__ stats, const float* __restrict__ dloss, void* dz_,
+    int chunks) {
     using T = typename S::T;
     constexpr int W = S::kVec;
-    __shared__ float red[3][kWaves];
-    __shared__ int at[kMaxK];   // column within the segment; -1: elsewhere
-    __shared__ float prob[kMaxK];
-    __shared__ unsigned map[kMapBits / 32];
-    for (int64_t item = blockIdx.x; item < a.rows * a.segs; item += gridDim.x) {
-        const int64_t row = item / a.segs;
-        int64_t c0;
-        int n;
-        seg_range(a, static_cast<int>(item - row * a.segs), c0, n);
-        const int64_t base = row * a.cols + c0;
-        const T* const z = static_cast<const T*>(a.z) + base;
-        T* const dz = static_cast<T*>(dz_) + base;
-        const int words = ((n < kMapBits ? n : kMapBits) + 31) / 32;
-        for (int i = threadIdx.x; i < words; i += kLanes) map[i] = 0u;
-        Teacher<PER> t;
-        load_teacher(a, row, t, red);  // has the barrier that the map needs
+    const int lane = static_cast<int>(threadIdx.x & 63);
+    const int64_t items = a.rows * chunks;
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves +
+                        __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+         item < items; item += static_cast<int64_t>(gridDim.x) * kWaves) {
+        const int64_t row = item / chunks;
+        const int chunk = static_cast<int>(item - row * chunks);
+        const int cols = static_cast<int>(a.cols);
+        const T* const z = static_cast<const T*>(a.z) + row * a.cols;
+        T* const dz = static_cast<T*>(dz_) + row * a.cols;
+        const Parts q = parts_of<S>(z, cols);
+        const u32x4* const zb = reinterpret_cast<const u32x4*>(z + q.head);
+        T* const db = dz + q.head;  // 16-byte aligned where z and dz start alike
+        // the row's teacher (loads return in order: those that are needed first, first)
+        int64_t index[PER];
+        float p[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int j = i * 64 + lane;
+            index[i] = -1;
+            p[i] = 0.0f;
+            if (a.k) {  // uniform; lanes past the entries load the first one
+                const int64_t e = row * a.k + (j < a.k ? j : 0);
+                index[i] = a.index[e];
+                p[i] = a.t_bf16 ? BF16::get(static_cast<const uint16_t*>(a.t) + e)
+                                : static_cast<const float*>(a.t)[e];
+            }
+        }
         const float2 st = stats[row];
-        const float c = t.bad ? __builtin_nanf("") : t.any ? dloss[row] * a.temperature : 0.0f;
+        const float weight = dloss[row];
+        __builtin_amdgcn_sched_barrier(0);
+
+        // the chunk's slots, and the edges with the first and the last chunk
+        u32x4 raw[kSlots], old[ACC ? kSlots : 1];
+#pragma unroll
+        for (int u = 0; u < kSlots; ++u) {
+            const int v = chunk * kChunk + u * 64 + lane;
+            const int vc = v < q.slots ? v : 0;
+            raw[u] = q.slots ? __builtin_nontemporal_load(zb + vc) : u32x4{0u, 0u, 0u, 0u};
+            if constexpr (ACC)
+                old[u] = q.slots ? load16_any_stream<S>(db + static_cast<int64_t>(vc) * W) : u32x4{0u, 0u, 0u, 0u};
+        }
+        int ec = -1;
+        if (chunk == 0 && lane < q.head) ec = lane;
+        if (chunk == chunks - 1 && lane >= 8 && q.tail0 + lane - 8 < cols) ec = q.tail0 + lane - 8;
+        float ez = 0.0f, eold = 0.0f;
+        if (ec >= 0) {
+            ez = S::get(z + ec);
+            if constexpr (ACC) eold = S::get(dz + ec);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        int at[PER];  // column; -1: no entry
+        float top = -__builtin_inff();
+        bool any = false, bad = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const bool in = i * 64 + lane < a.k && index[i] >= 0;
+            if (!in) p[i] = -__builtin_inff();
+            any = any || !(p[i] == -__builtin_inff());
+            bad = bad || (in && index[i] >= a.cols);
+            at[i] = in && index[i] < a.cols ? static_cast<int>(index[i]) : -1;
+            top = max_of(top, p[i]);
+        }
+        any = __any(any);
+        bad = __any(bad);
+        top = wave_max(top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            p[i] = p[i] == -__builtin_inff() ? 0.0f
+                                             : __builtin_amdgcn_exp2f((p[i] - top) * a.scale);
+            sum += p[i];
+        }
+        sum = group_sum<64>(sum);
+
+        const float c = bad ? __builtin_nanf("") : any ? weight * a.temperature : 0.0f;
         const float l2 = st.y * kLog2e;
         auto grad = [&](float v) {
             return c * __builtin_amdgcn_exp2f(__builtin_fmaf(v - st.x, a.scale, -l2));
         };
-        // What the named columns need of z and the old dz is read before any of dz is
-        // written.
-        float own_z[PER], own_old[PER];
-        int own_at[PER], twice = 0;
+        float f[kSlots][W];
+        float eg = grad(ez);
+#pragma unroll
+        for (int u = 0; u < kSlots; ++u) {
+            S::unpack(raw[u], f[u]);
+#pragma unroll
+            for (int e = 0; e < W; ++e) f[u][e] = grad(f[u][e]);
+        }
+        const int first = q.head + chunk * kChunk * W;  // the chunk's columns but the edges
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int j = static_cast<int>(threadIdx.x) + i * kLanes;
-            const int64_t r = t.index[i] - c0;
-            own_at[i] = t.index[i] >= 0 && r >= 0 && r < n ? static_cast<int>(r) : -1;
-            own_z[i] = own_old[i] = 0.0f;
-            if (own_at[i] >= 0) {
-                own_z[i] = S::get(z + own_at[i]);
-                if constexpr (ACC) own_old[i] = S::get(dz + own_at[i]);
-                const unsigned bit = static_cast<unsigned>(own_at[i]) % kMapBits;
-                if (atomicOr(&map[bit / 32], 1u << (bit % 32)) >> (bit % 32) & 1u) twice = 1;
-            }
-            if (j < a.k) {
-                at[j] = own_at[i];
-                prob[j] = t.p[i];
+            const int r = at[i] - first;
+            const bool mine = at[i] >= 0 && ((r >= 0 && r < kChunk * W) ||
+                                             (chunk == 0 && r < 0) ||
+                                             (chunk == chunks - 1 && at[i] >= q.tail0));
+            unsigned long long todo = __ballot(mine);
+            while (todo) {
+                const int l = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                const int col = __builtin_amdgcn_readlane(at[i], l);
+                const float d =
+                    c * (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(p[i]), l)) / sum);
+                if (col == ec) eg -= d;
+                const int rel = col - first;
+                if (rel < 0 || col >= q.tail0) continue;
+                const int slot = rel / W, elem = rel % W;
+                const float mine_d = lane == (slot & 63) ? d : 0.0f;
+#pragma unroll
+                for (int u = 0; u < kSlots; ++u)
+                    if (u == slot / 64) {
+#pragma unroll
+                        for (int e = 0; e < W; ++e)
+                            if (e == elem) f[u][e] -= mine_d;
+                    }
             }
         }
-        twice = __syncthreads_or(twice);
-        const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
-        if (c == 0.0f) {
-            if constexpr (!ACC) {
-                const Parts q = parts_of<S>(dz, n);
-                u32x4* const db = reinterpret_cast<u32x4*>(dz + q.head);
-                for (int v = threadIdx.x; v < q.slots; v += kLanes)
-                    __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, db + v);
-                if (const int e = edge(q, n); e >= 0) S::put(dz + e, 0.0f);
-            }
-        } else if (!same) {  // z and dz at different offsets from a 16-byte boundary
-            for (int e = threadIdx.x; e < n; e += kLanes) {
-                const float g = grad(S::get(z + e));
-                S::put(dz + e, ACC ? acc_add(S::get(dz + e), g) : g);
-            }
-        } else {
-            const Parts q = parts_of<S>(z, n);
-            const u32x4* const zb = reinterpret_cast<const u32x4*>(z + q.head);
-            u32x4* const db = reinterpret_cast<u32x4*>(dz + q.head);
-            auto slot = [&](int v, u32x4 raw, u32x4 old) {
-                float f[W];
-                S::unpack(raw, f);
+        // a row without a teacher or weight: zeros, whatever z holds
+        const bool zero = c == 0.0f;
 #pragma unroll
-                for (int e = 0; e < W; ++e) f[e] = grad(f[e]);
-                if constexpr (ACC) {
-                    float o[W];
-                    S::unpack(old, o);
+        for (int u = 0; u < kSlots; ++u) {
+            const int v = chunk * kChunk + u * 64 + lane;
 #pragma unroll
-                    for (int e = 0; e < W; ++e) f[e] = acc_add(o[e], f[e]);
-                }
-                __builtin_nontemporal_store(S::pack(f), db + v);
-            };
-            int v = static_cast<int>(threadIdx.x);
-            for (; v + (kBatch - 1) * kLanes < q.slots; v += kLanes * kBatch) {
-                u32x4 raw[kBatch], old[kBatch] = {};
+            for (int e = 0; e < W; ++e) f[u][e] = zero ? 0.0f : f[u][e];
+            if constexpr (ACC) {
+                float o[W];
+                S::unpack(old[u], o);
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    raw[u] = __builtin_nontemporal_load(zb + v + u * kLanes);
-                    if constexpr (ACC) old[u] = __builtin_nontemporal_load(db + v + u * kLanes);
-                }
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) slot(v + u * kLanes, raw[u], old[u]);
+                for (int e = 0; e < W; ++e) f[u][e] = acc_add(o[e], f[u][e]);
             }
-            for (; v < q.slots; v += kLanes)
-                slot(v, __builtin_nontemporal_load(zb + v),
-                     ACC ? __builtin_nontemporal_load(db + v) : u32x4{0u, 0u, 0u, 0u});
-            if (const int e = edge(q, n); e >= 0) {
-                const float g = grad(S::get(z + e));
-                S::put(dz + e, ACC ? acc_add(S::get(dz + e), g) : g);
-            }
+            if (v < q.slots) store16_any_stream<S>(db + static_cast<int64_t>(v) * W, S::pack(f[u]));
         }
-        // Entries of one column all write the same value.
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (c != 0.0f) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (own_at[i] < 0) continue;
-                float p = t.p[i];
-                if (twice) {
-                    p = 0.0f;
-                    for (int j = 0; j < a.k; ++j) p += at[j] == own_at[i] ? prob[j] : 0.0f;
-                }
-                const float g = grad(own_z[i]) - c * p;
-                S::put(dz + own_at[i], ACC ? acc_add(own_old[i], g) : g);
-            }
+        if (ec >= 0) {
+            eg = zero ? 0.0f : eg;
+            S::put(dz + ec, ACC ? acc_add(eold, eg) : eg);
         }
-        __syncthreads();
     }
 }
 
@@ -496,12 +529,26 @@ int forward(const Args& a, float* loss, float2* stats, float2* part, hipStream_t
 }
 
 template <class S, int PER>
+int backward_per(const Args& a, const float2* stats, const float* dloss, void* dz, bool acc,
+                 hipStream_t st) {
+    const int64_t n = a.cols / S::kVec;  // slots at most
+    const int chunks = static_cast<int>(std::max<int64_t>((n + kChunk - 1) / kChunk, 1));
+    const int64_t groups = (a.rows * chunks + kWaves - 1) / kWaves;
+    const dim3 grid(capped_blocks(groups, kLanes)), block(kLanes);
+    if (acc)
+        hipLaunchKernelGGL((distill_bwd<S, PER, true>), grid, block, 0, st, a, stats, dloss, dz,
+                           chunks);
+    else
+        hipLaunchKernelGGL((distill_bwd<S, PER, false>), grid, block, 0, st, a, stats, dloss, dz,
+                           chunks);
+    return check_launch();
+}
+template <class S>
 int backward(const Args& a, const float2* stats, const float* dloss, void* dz, bool acc,
              hipStream_t st) {
-    const dim3 grid(capped_blocks(a.rows * a.segs, kLanes)), block(kLanes);
-    if (acc) hipLaunchKernelGGL((distill_bwd<S, PER, true>), grid, block, 0, st, a, stats, dloss, dz);
-    else hipLaunchKernelGGL((distill_bwd<S, PER, false>), grid, block, 0, st, a, stats, dloss, dz);
-    return check_launch();
+    if (a.k <= 64) return backward_per<S, 1>(a, stats, dloss, dz, acc, st);
+    if (a.k <= 256) return backward_per<S, 4>(a, stats, dloss, dz, acc, st);
+    return backward_per<S, kMaxK / 64>(a, stats, dloss, dz, acc, st);
 }
 
 constexpr int kMostPer = kMaxK / kLanes;
@@ -562,11 +609,8 @@ int agk_distill_topk_bwd(const void* z, const int64_t* index, const void* t, con
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const float2* const in = reinterpret_cast<const float2*>(stats);
     const bool acc = accumulate != 0;
-    if (dtype == AGK_F32)
-        return k <= kLanes ? backward<agk::F32, 1>(a, in, dloss, dz, acc, st)
-                           : backward<agk::F32, kMostPer>(a, in, dloss, dz, acc, st);
-    return k <= kLanes ? backward<agk::BF16, 1>(a, in, dloss, dz, acc, st)
-                       : backward<agk::BF16, kMostPer>(a, in, dloss, dz, acc, st);
+    return dtype == AGK_F32 ? backward<agk::F32>(a, in, dloss, dz, acc, st)
+                            : backward<agk::BF16>(a, in, dloss, dz, acc, st);
 }
 
 }  // extern "C"

@@ -4,8 +4,8 @@
 //   dx (+)= rstd * (h - sum(h)/cols - xhat * sum(h * xhat)/cols)
 //   dgamma (+)= sum_rows dy * xhat,  dbeta (+)= sum_rows dy
 //
-// One pass: a workgroup of 1024 lanes takes every nblk-th group of G rows, each row held in
-// registers by TPR lanes (NV 16-byte slots of x and of dy per lane), and the next
+// One pass: a workgroup of up to 1024 lanes takes every nblk-th group of G rows, each row held
+// in registers by TPR lanes (NV 16-byte slots of x and of dy per lane), and the next
 // rows' loads are issued before the current rows are reduced.  Each lane adds its
 // columns' dgamma and dbeta terms in fp32 over its rows; the workgroup's sums are one
 // partial row of each, and a second kernel adds the partial rows in fp64 in a fixed
@@ -29,10 +29,12 @@ namespace layernorm {
 constexpr int kLanes = 1024;
 constexpr int kBlocks = 256;  // workgroups, one per CU, and partial rows
 
-// (TPR, NV): lanes of a row and 16-byte slots per lane; 1024 / TPR rows at a time.
+// (TPR, NV): lanes of a row and 16-byte slots per lane; 1024 / TPR rows at a time.  Rows of
+// more than a wave take the fewest whole waves that hold them, of the steps below: with
+// powers of two 4099 f32 rows of 1030 columns (258 slots) left half of the lanes idle.
 #define AGK_LN_SHAPES(X)                                                                 \
-    X(1, 1) X(2, 1) X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(256, 1)       \
-    X(512, 1) X(1024, 1) X(1024, 2) X(1024, 4)
+    X(1, 1) X(2, 1) X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(192, 1)       \
+    X(256, 1) X(320, 1) X(512, 1) X(640, 1) X(768, 1) X(1024, 1) X(1024, 2) X(1024, 4)
 
 // The widest shape's 32 columns of bf16 a lane do not fit its registers.
 template <class S>
@@ -87,7 +89,7 @@ struct Set {
 };
 
 template <class S, int TPR, int NV, bool RAG>
-__global__ __launch_bounds__(kLanes) void ln_bwd(const Args<typename S::T> p) {
+__global__ __launch_bounds__(kLanes / TPR * TPR) void ln_bwd(const Args<typename S::T> p) {
     using T = typename S::T;
     constexpr int W = S::kVec;
     constexpr int G = kLanes / TPR;
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(kLanes) void ln_bwd(const Args<typename S::T> p) {
                         if (e >= dup[k]) part[grp * cols + col[k] + e] = which ? db[k][e] : dg[k][e];
                 }
             __syncthreads();
-            for (int c = threadIdx.x; c < cols; c += kLanes) {  // in group order
+            for (int c = threadIdx.x; c < cols; c += TPR * G) {  // in group order
                 float v = part[c];
                 for (int q = 1; q < G; ++q) v += part[q * cols + c];
                 out[which][c] = v;
@@ -325,8 +327,15 @@ inline Shape pick(int64_t cols) {
     if (cols < S::kVec || slots > 4096) return s;
     const int nv = slots <= 1024 ? 1 : slots <= 2048 ? 2 : 4;
     if (!enabled<S>(nv)) return s;
+    constexpr int kTpr[] = {1, 2, 4, 8, 16, 32, 64, 128, 192, 256, 320, 512, 640, 768, 1024};
     s.nv = nv;
-    s.tpr = nv == 1 ? pow2_at_least(slots) : 1024;
+    s.tpr = 1024;
+    for (int tpr : kTpr)
+        if (static_cast<int64_t>(tpr) * nv >= slots) {
+            s.tpr = tpr;
+            break;
+        }
+    if (nv > 1) s.tpr = 1024;
     return s;
 }
 
@@ -350,7 +359,7 @@ int launch(const Args<typename S::T>& a, int64_t* nblk, hipStream_t st) {
     const int g = kLanes / s.tpr;
     *nblk = blocks(a.rows, g);
     const size_t lds = g > 1 && a.partial ? static_cast<size_t>(g) * a.cols * 4 : 0;
-    const dim3 grid(static_cast<unsigned>(*nblk)), block(kLanes);
+    const dim3 grid(static_cast<unsigned>(*nblk)), block(g * s.tpr);
 #define AGK_X(TPR, NV)                                                                      \
     if constexpr (enabled<S>(NV)) {                                                         \
         if (s.tpr == TPR && s.nv == NV) {                                                   \
