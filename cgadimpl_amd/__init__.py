@@ -102,7 +102,7 @@ SIGNATURES = {
     "agk_linear_xent_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, ctypes.c_int,
                                            _P, ctypes.c_size_t, _I64, _I64, _I64, _I64,
                                            ctypes.c_int, ctypes.c_int, _P]),
-    "agk_distill_topk_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "agk_distill_topk_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, ctypes.c_int]),
     "agk_distill_topk_fwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, ctypes.c_size_t, _I64, _I64,
                                             _I64, ctypes.c_float, ctypes.c_int, ctypes.c_int, _P]),
     "agk_distill_topk_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64,
@@ -1036,10 +1036,11 @@ def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, sta
     float32 [...] and [..., 2]."""
     dev, rows, cols, k = _distill_sizes(z, index, teacher)
     loss, stats = _loss_and_stats(z.shape[:-1], rows, dev, z, loss, stats)
-    ws, ws_bytes = _scratch(workspace, lib().agk_distill_topk_workspace_bytes(rows, cols), z)
+    dt = _dtype_code(z)
+    ws, ws_bytes = _scratch(workspace, lib().agk_distill_topk_workspace_bytes(rows, cols, dt), z)
     rc = lib().agk_distill_topk_fwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(loss), _ptr(stats),
-                                    _ptr(ws), ws_bytes, rows, cols, k, float(temperature),
-                                    _dtype_code(z), _dtype_code(teacher), _stream(stream))
+                                    _ptr(ws), ws_bytes, rows, cols, k, float(temperature), dt,
+                                    _dtype_code(teacher), _stream(stream))
     _check(rc, "agk_distill_topk_fwd")
     return loss, stats
 

@@ -33,29 +33,9 @@ __device__ __forceinline__ float max_of(float a, float b) {  // one v_max_f32; d
     return r;
 }
 
-// Reductions over the workgroup; every lane gets the result.  `red` is free again
-// after the barrier of the next call, so calls alternate between two arrays.
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int h = 32; h > 0; h /= 2) v = max_of(v, __shfl_xor(v, h));
-    return v;
-}
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v = max_of(v, red[w]);
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = group_sum<64>(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += red[w];
     return v;
 }
 
@@ -66,63 +46,64 @@ struct Args {
     int t_bf16;
     int64_t rows, cols;
     int k;
-    int segs;          // segments per row
+    int segs;          // segments per row (the forward of very wide rows; else 1)
     int64_t seg_cols;  // columns of a segment (a multiple of 8; the last may have fewer)
     float temperature, scale;  // scale = log2(e) / T
 };
 
-// A row's teacher as the lanes hold it: PER entries, j = lane + i * kLanes.  Kernels are built
-// for PER = 1 (k <= 256) and for the most entries: the rest of a kernel then keeps the registers.
+// A row's teacher, held by one wave: PER entries per lane, entry j in lane j % 64.  A wave works
+// it out by itself, without a barrier: two loads, a maximum and a sum over 64 lanes.
 template <int PER>
 struct Teacher {
-    int64_t index[PER];  // < 0: no entry
-    float p[PER], logp[PER];
-    bool any, bad;  // an entry with a probability; a column past the last
-};
+    int64_t index[PER];  // as loaded
+    int at[PER];         // column; -1: no entry
+    float p[PER];        // t, after exponentials() exp((t - top) / T); p = that / sum
+    float top, sum;
+    bool any, bad;       // an entry with a probability; a column past the last
 
-// red: three arrays of kWaves floats.
-template <int PER>
-__device__ __forceinline__ void load_teacher(const Args& a, int64_t row, Teacher<PER>& o,
-                                             float (*red)[kWaves]) {
-    float t[PER];
-    float top = -__builtin_inff();
-    int flags = 0;
-    const int64_t base = row * a.k;
+    __device__ __forceinline__ void load(const Args& a, int64_t row) {
+        const int lane = static_cast<int>(threadIdx.x & 63);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int j = static_cast<int>(threadIdx.x) + i * kLanes;
-        o.index[i] = -1;
-        t[i] = -__builtin_inff();
-        if (j < a.k) {
-            o.index[i] = a.index[base + j];
-            const float v = a.t_bf16 ? BF16::get(static_cast<const uint16_t*>(a.t) + base + j)
-                                     : static_cast<const float*>(a.t)[base + j];
-            if (o.index[i] >= 0) {
-                t[i] = v;
-                if (!(v == -__builtin_inff())) flags |= 1;
-                if (o.index[i] >= a.cols) flags |= 2;
+        for (int i = 0; i < PER; ++i) {
+            const int j = i * 64 + lane;
+            index[i] = -1;
+            p[i] = 0.0f;
+            if (a.k) {  // uniform; lanes past the entries load the first one
+                const int64_t e = row * a.k + (j < a.k ? j : 0);
+                index[i] = a.index[e];
+                p[i] = a.t_bf16 ? BF16::get(static_cast<const uint16_t*>(a.t) + e)
+                                : static_cast<const float*>(a.t)[e];
             }
         }
-        top = max_of(top, t[i]);
     }
-    const bool any = __syncthreads_or(flags & 1), bad = __syncthreads_or(flags & 2);
-    o.any = any;
-    o.bad = bad;
-    top = block_max(top, red[0]);
-    float e[PER], sum = 0.0f;
+    __device__ __forceinline__ void place(const Args& a) {
+        const int lane = static_cast<int>(threadIdx.x & 63);
+        top = -__builtin_inff();
+        any = bad = false;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        e[i] = t[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((t[i] - top) * a.scale);
-        sum += e[i];
+        for (int i = 0; i < PER; ++i) {
+            const bool in = i * 64 + lane < a.k && index[i] >= 0;
+            if (!in) p[i] = -__builtin_inff();
+            any = any || !(p[i] == -__builtin_inff());
+            bad = bad || (in && index[i] >= a.cols);
+            at[i] = in && index[i] < a.cols ? static_cast<int>(index[i]) : -1;
+            top = max_of(top, p[i]);
+        }
+        any = __any(any);
+        bad = __any(bad);
+        top = wave_max(top);
     }
-    sum = block_sum(sum, red[1]);
-    const float logs = logf(sum);
+    __device__ __forceinline__ void exponentials(const Args& a) {
+        sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        o.p[i] = e[i] / sum;
-        o.logp[i] = (t[i] - top) / a.temperature - logs;
+        for (int i = 0; i < PER; ++i) {
+            p[i] = p[i] == -__builtin_inff() ? 0.0f
+                                             : __builtin_amdgcn_exp2f((p[i] - top) * a.scale);
+            sum += p[i];
+        }
+        sum = group_sum<64>(sum);
     }
-}
+};
 
 __device__ __forceinline__ void seg_range(const Args& a, int seg, int64_t& c0, int& n) {
     c0 = static_cast<int64_t>(seg) * a.seg_cols;
@@ -197,9 +178,9 @@ struct Lse {
     }
 };
 
-// {max, sum} of a segment, in every lane.
+// {max, sum} of a segment, in every lane of a workgroup of LANES.
 constexpr int kBatch = 4;  // 16-byte loads in flight per lane
-template <class S>
+template <class S, int LANES>
 __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, float& m, float& s,
                                         float2* red) {
     using T = typename S::T;
@@ -212,10 +193,10 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
     const u32x4* const body = reinterpret_cast<const u32x4*>(z + q.head);
     Lse r{-__builtin_inff(), 0.0f};
     int v = static_cast<int>(threadIdx.x);
-    for (; v + (kBatch - 1) * kLanes < q.slots; v += kLanes * kBatch) {
+    for (; v + (kBatch - 1) * LANES < q.slots; v += LANES * kBatch) {
         u32x4 raw[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) raw[u] = __builtin_nontemporal_load(body + v + u * kLanes);
+        for (int u = 0; u < kBatch; ++u) raw[u] = __builtin_nontemporal_load(body + v + u * LANES);
         float f[kBatch * W];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
@@ -226,7 +207,7 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
         }
         r.add(f, a.scale);
     }
-    for (; v < q.slots; v += kLanes) {
+    for (; v < q.slots; v += LANES) {
         float f[W];
         S::unpack(__builtin_nontemporal_load(body + v), f);
         r.add(f, a.scale);
@@ -247,42 +228,59 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
     m = red[0].x;
     s = red[0].y;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) join(m, s, red[w].x, red[w].y, a.scale);
+    for (int w = 1; w < LANES / 64; ++w) join(m, s, red[w].x, red[w].y, a.scale);
 }
 
-// The row's loss from its {max, sum}; called by the whole workgroup.
+// The named columns' z, loaded before the row is streamed; then the row's loss from its
+// {max, sum}.  Both by one wave.
 template <class S, int PER>
-__device__ __forceinline__ void row_loss(const Args& a, int64_t row, float m, float s, float* loss,
-                                         float2* stats, float (*red)[kWaves]) {
-    using T = typename S::T;
-    const T* const z = static_cast<const T*>(a.z) + row * a.cols;
-    const float l = logf(s);
-    Teacher<PER> t;
-    load_teacher(a, row, t, red);
+__device__ __forceinline__ void named_z(const Args& a, int64_t row, const Teacher<PER>& t,
+                                        float (&zt)[PER]) {
+    const typename S::T* const z = static_cast<const typename S::T*>(a.z) + row * a.cols;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) zt[i] = t.at[i] >= 0 ? S::get(z + t.at[i]) : 0.0f;
+}
+template <int PER>
+__device__ __forceinline__ void row_loss(const Args& a, int64_t row, float m, float s,
+                                         Teacher<PER>& t, const float (&zt)[PER], float* loss,
+                                         float2* stats) {
+    float logp[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) logp[i] = (t.p[i] - t.top) / a.temperature;
+    t.exponentials(a);
+    const float l = logf(s), logs = logf(t.sum);
     float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (t.index[i] >= 0 && t.index[i] < a.cols && !(t.p[i] == 0.0f)) {
-            const float logq = (S::get(z + t.index[i]) - m) / a.temperature - l;
-            v += t.p[i] * (t.logp[i] - logq);
-        }
-    v = block_sum(v, red[2]);
-    if (threadIdx.x == 0) {
+    for (int i = 0; i < PER; ++i) {
+        const float p = t.p[i] / t.sum;
+        const float logq = (zt[i] - m) / a.temperature - l;
+        v += t.at[i] >= 0 && !(p == 0.0f) ? p * (logp[i] - logs - logq) : 0.0f;
+    }
+    v = group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) {
         stats[row] = make_float2(m, l);
         loss[row] = t.bad ? __builtin_nanf("") : t.any ? a.temperature * a.temperature * v : 0.0f;
     }
 }
 
-// One workgroup per row (segs == 1), looping over what the grid leaves.
-template <class S, int PER>
-__global__ __launch_bounds__(kLanes) void distill_fwd(const Args a, float* __restrict__ loss,
-                                                      float2* __restrict__ stats) {
-    __shared__ float2 red2[kWaves];
-    __shared__ float red[3][kWaves];
+// One workgroup per row (segs == 1), looping over what the grid leaves.  Its first wave
+// has the teacher's part.
+template <class S, int LANES, int PER>
+__global__ __launch_bounds__(LANES) void distill_fwd(const Args a, float* __restrict__ loss,
+                                                     float2* __restrict__ stats) {
+    __shared__ float2 red[LANES / 64];
+    const bool first = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)) == 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        Teacher<PER> t;
+        float zt[PER];
+        if (first) {
+            t.load(a, row);
+            t.place(a);
+            named_z<S, PER>(a, row, t, zt);
+        }
         float m, s;
-        seg_lse<S>(a, row, 0, m, s, red2);
-        row_loss<S, PER>(a, row, m, s, loss, stats, red);
+        seg_lse<S, LANES>(a, row, 0, m, s, red);
+        if (first) row_loss<PER>(a, row, m, s, t, zt, loss, stats);
         __syncthreads();
     }
 }
@@ -290,22 +288,27 @@ __global__ __launch_bounds__(kLanes) void distill_fwd(const Args a, float* __res
 // Segments: part[row * segs + seg].
 template <class S>
 __global__ __launch_bounds__(kLanes) void distill_part(const Args a, float2* __restrict__ part) {
-    __shared__ float2 red2[kWaves];
+    __shared__ float2 red[kWaves];
     const int64_t row = blockIdx.x / static_cast<unsigned>(a.segs);
     const int seg = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.segs));
     float m, s;
-    seg_lse<S>(a, row, seg, m, s, red2);
+    seg_lse<S, kLanes>(a, row, seg, m, s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = make_float2(m, s);
 }
 
+// A wave per row.
 template <class S, int PER>
-__global__ __launch_bounds__(kLanes) void distill_join(const Args a, const float2* __restrict__ part,
-                                                       float* __restrict__ loss,
-                                                       float2* __restrict__ stats) {
-    __shared__ float red[3][kWaves];
+__global__ __launch_bounds__(64) void distill_join(const Args a, const float2* __restrict__ part,
+                                                   float* __restrict__ loss,
+                                                   float2* __restrict__ stats) {
     const int64_t row = blockIdx.x;
+    Teacher<PER> t;
+    float zt[PER];
+    t.load(a, row);
+    t.place(a);
+    named_z<S, PER>(a, row, t, zt);
     float m = -__builtin_inff(), s = 0.0f;
-    for (int i = threadIdx.x & 63; i < a.segs; i += 64) {
+    for (int i = threadIdx.x; i < a.segs; i += 64) {
         const float2 v = part[row * a.segs + i];
         join(m, s, v.x, v.y, a.scale);
     }
@@ -314,7 +317,7 @@ __global__ __launch_bounds__(kLanes) void distill_join(const Args a, const float
         const float m2 = __shfl_xor(m, h), s2 = __shfl_xor(s, h);
         join(m, s, m2, s2, a.scale);
     }
-    row_loss<S, PER>(a, row, m, s, loss, stats, red);
+    row_loss<PER>(a, row, m, s, t, zt, loss, stats);
 }
 
 // ---- backward ------------------------------------------------------------------------
@@ -348,21 +351,9 @@ __global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) vo
         const Parts q = parts_of<S>(z, cols);
         const u32x4* const zb = reinterpret_cast<const u32x4*>(z + q.head);
         T* const db = dz + q.head;  // 16-byte aligned where z and dz start alike
-        // the row's teacher (loads return in order: those that are needed first, first)
-        int64_t index[PER];
-        float p[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int j = i * 64 + lane;
-            index[i] = -1;
-            p[i] = 0.0f;
-            if (a.k) {  // uniform; lanes past the entries load the first one
-                const int64_t e = row * a.k + (j < a.k ? j : 0);
-                index[i] = a.index[e];
-                p[i] = a.t_bf16 ? BF16::get(static_cast<const uint16_t*>(a.t) + e)
-                                : static_cast<const float*>(a.t)[e];
-            }
-        }
+        // loads return in order: those that are needed first, first
+        Teacher<PER> t;
+        t.load(a, row);
         const float2 st = stats[row];
         const float weight = dloss[row];
         __builtin_amdgcn_sched_barrier(0);
@@ -387,31 +378,10 @@ __global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) vo
         }
         __builtin_amdgcn_sched_barrier(0);
 
-        int at[PER];  // column; -1: no entry
-        float top = -__builtin_inff();
-        bool any = false, bad = false;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const bool in = i * 64 + lane < a.k && index[i] >= 0;
-            if (!in) p[i] = -__builtin_inff();
-            any = any || !(p[i] == -__builtin_inff());
-            bad = bad || (in && index[i] >= a.cols);
-            at[i] = in && index[i] < a.cols ? static_cast<int>(index[i]) : -1;
-            top = max_of(top, p[i]);
-        }
-        any = __any(any);
-        bad = __any(bad);
-        top = wave_max(top);
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            p[i] = p[i] == -__builtin_inff() ? 0.0f
-                                             : __builtin_amdgcn_exp2f((p[i] - top) * a.scale);
-            sum += p[i];
-        }
-        sum = group_sum<64>(sum);
-
-        const float c = bad ? __builtin_nanf("") : any ? weight * a.temperature : 0.0f;
+        t.place(a);
+        t.exponentials(a);
+        const float sum = t.sum;
+        const float c = t.bad ? __builtin_nanf("") : t.any ? weight * a.temperature : 0.0f;
         const float l2 = st.y * kLog2e;
         auto grad = [&](float v) {
             return c * __builtin_amdgcn_exp2f(__builtin_fmaf(v - st.x, a.scale, -l2));
@@ -427,17 +397,17 @@ __global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) vo
         const int first = q.head + chunk * kChunk * W;  // the chunk's columns but the edges
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int r = at[i] - first;
-            const bool mine = at[i] >= 0 && ((r >= 0 && r < kChunk * W) ||
+            const int r = t.at[i] - first;
+            const bool mine = t.at[i] >= 0 && ((r >= 0 && r < kChunk * W) ||
                                              (chunk == 0 && r < 0) ||
-                                             (chunk == chunks - 1 && at[i] >= q.tail0));
+                                             (chunk == chunks - 1 && t.at[i] >= q.tail0));
             unsigned long long todo = __ballot(mine);
             while (todo) {
                 const int l = __builtin_ctzll(todo);
                 todo &= todo - 1;
-                const int col = __builtin_amdgcn_readlane(at[i], l);
+                const int col = __builtin_amdgcn_readlane(t.at[i], l);
                 const float d =
-                    c * (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(p[i]), l)) / sum);
+                    c * (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.p[i]), l)) / sum);
                 if (col == ec) eg -= d;
                 const int rel = col - first;
                 if (rel < 0 || col >= q.tail0) continue;
@@ -474,13 +444,17 @@ __global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) vo
     }
 }
 
-// Segments of a row: enough workgroups to fill the chip (8 of 256 lanes per CU), of
-// at least kMinSeg columns.
+// Segments of a row in the forward.  A few rows of many columns are cut into kMinSeg columns and
+// more, kFill workgroups of them; else a row is one workgroup's, which reads 40 bytes a ns
+// on a CU of its own, and saves the second kernel.  MI355X, us, whole / cut: f32 32 x 32000 6.3 /
+// 8.0, 1 x 151936 15.9 / 7.9, 4 x 262144 20.6 / 8.2, bf16 96 x 131072 (256 KiB) 13.8 / 14.3.
 constexpr int64_t kFill = 2048;
 constexpr int64_t kMinSeg = 2048;
-inline int segments(int64_t rows, int64_t cols) {
+constexpr int64_t kWholeBytes = 320 << 10;
+inline int segments(int64_t rows, int64_t cols, int dtype) {
+    if (rows >= 256 || cols * (dtype == AGK_F32 ? 4 : 2) <= kWholeBytes) return 1;
     const int64_t want = (kFill + rows - 1) / rows, most = (cols + kMinSeg - 1) / kMinSeg;
-    int64_t s = std::max<int64_t>(std::min(want, most), 1);
+    const int64_t s = std::min(want, most);
     const int64_t w = ((cols + s - 1) / s + 7) / 8 * 8;
     return static_cast<int>((cols + w - 1) / w);
 }
@@ -496,7 +470,7 @@ inline int check(int64_t rows, int64_t cols, int64_t k, float temperature, int d
 }
 
 inline Args args(const void* z, const int64_t* index, const void* t, int64_t rows, int64_t cols,
-                 int64_t k, float temperature, int t_dtype) {
+                 int64_t k, float temperature, int dtype, int t_dtype) {
     Args a;
     a.z = z;
     a.index = index;
@@ -505,7 +479,7 @@ inline Args args(const void* z, const int64_t* index, const void* t, int64_t row
     a.rows = rows;
     a.cols = cols;
     a.k = static_cast<int>(k);
-    a.segs = segments(rows, cols);
+    a.segs = segments(rows, cols, dtype);
     a.seg_cols = ((cols + a.segs - 1) / a.segs + 7) / 8 * 8;
     a.temperature = temperature;
     a.scale = static_cast<float>(1.4426950408889634 / temperature);
@@ -513,19 +487,31 @@ inline Args args(const void* z, const int64_t* index, const void* t, int64_t row
 }
 
 template <class S, int PER>
-int forward(const Args& a, float* loss, float2* stats, float2* part, hipStream_t st) {
-    if (a.segs == 1) {
-        hipLaunchKernelGGL((distill_fwd<S, PER>), dim3(capped_blocks(a.rows, kLanes)), dim3(kLanes),
-                           0, st, a, loss, stats);
+int forward_per(const Args& a, float* loss, float2* stats, float2* part, hipStream_t st) {
+    if (a.segs > 1) {
+        hipLaunchKernelGGL(distill_part<S>, dim3(static_cast<unsigned>(a.rows * a.segs)),
+                           dim3(kLanes), 0, st, a, part);
+        const int rc = check_launch();
+        if (rc != AGK_OK) return rc;
+        hipLaunchKernelGGL((distill_join<S, PER>), dim3(static_cast<unsigned>(a.rows)), dim3(64), 0,
+                           st, a, part, loss, stats);
         return check_launch();
     }
-    hipLaunchKernelGGL(distill_part<S>, dim3(static_cast<unsigned>(a.rows * a.segs)), dim3(kLanes),
-                       0, st, a, part);
-    const int rc = check_launch();
-    if (rc != AGK_OK) return rc;
-    hipLaunchKernelGGL((distill_join<S, PER>), dim3(static_cast<unsigned>(a.rows)), dim3(kLanes), 0,
-                       st, a, part, loss, stats);
+    // a workgroup of 1024 lanes for rows too few to give every CU several of 256 (bf16 1000 x
+    // 50257 30.6 us against 23.1 with 256 lanes and 1100 rows; 300 rows 15.4)
+    if (a.rows < 512 && a.cols / S::kVec > 1024)
+        hipLaunchKernelGGL((distill_fwd<S, 1024, PER>), dim3(static_cast<unsigned>(a.rows)),
+                           dim3(1024), 0, st, a, loss, stats);
+    else
+        hipLaunchKernelGGL((distill_fwd<S, kLanes, PER>), dim3(capped_blocks(a.rows, kLanes)),
+                           dim3(kLanes), 0, st, a, loss, stats);
     return check_launch();
+}
+template <class S>
+int forward(const Args& a, float* loss, float2* stats, float2* part, hipStream_t st) {
+    if (a.k <= 64) return forward_per<S, 1>(a, loss, stats, part, st);
+    if (a.k <= 256) return forward_per<S, 4>(a, loss, stats, part, st);
+    return forward_per<S, kMaxK / 64>(a, loss, stats, part, st);
 }
 
 template <class S, int PER>
@@ -551,17 +537,16 @@ int backward(const Args& a, const float2* stats, const float* dloss, void* dz, b
     return backward_per<S, kMaxK / 64>(a, stats, dloss, dz, acc, st);
 }
 
-constexpr int kMostPer = kMaxK / kLanes;
-
 }  // namespace distill
 }  // namespace agk
 
 extern "C" {
 
-size_t agk_distill_topk_workspace_bytes(int64_t rows, int64_t cols) {
+size_t agk_distill_topk_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
     using namespace agk::distill;
     if (rows <= 0 || cols <= 0 || agk::check_sizes(rows, cols) != AGK_OK) return 0;
-    const int s = segments(rows, cols);
+    if (!agk::valid_dtype(dtype)) return 0;
+    const int s = segments(rows, cols, dtype);
     return s > 1 ? static_cast<size_t>(rows) * s * sizeof(float2) : 0;
 }
 
@@ -575,19 +560,16 @@ int agk_distill_topk_fwd(const void* z, const int64_t* index, const void* t, flo
     if (!z || !loss || !stats || (k > 0 && (!index || !t))) return AGK_EINVAL;
     if ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(index)) & 7u)
         return AGK_EINVAL;
-    const size_t need = agk_distill_topk_workspace_bytes(rows, cols);
+    const size_t need = agk_distill_topk_workspace_bytes(rows, cols, dtype);
     if (need && (!workspace || workspace_bytes < need)) return AGK_EWORKSPACE;
     if (need && (reinterpret_cast<uintptr_t>(workspace) & 7u)) return AGK_EINVAL;
     agk::clear_pending_error();
-    const Args a = args(z, index, t, rows, cols, k, temperature, t_dtype);
+    const Args a = args(z, index, t, rows, cols, k, temperature, dtype, t_dtype);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     float2* const out = reinterpret_cast<float2*>(stats);
     float2* const part = static_cast<float2*>(workspace);
-    if (dtype == AGK_F32)
-        return k <= kLanes ? forward<agk::F32, 1>(a, loss, out, part, st)
-                           : forward<agk::F32, kMostPer>(a, loss, out, part, st);
-    return k <= kLanes ? forward<agk::BF16, 1>(a, loss, out, part, st)
-                       : forward<agk::BF16, kMostPer>(a, loss, out, part, st);
+    return dtype == AGK_F32 ? forward<agk::F32>(a, loss, out, part, st)
+                            : forward<agk::BF16>(a, loss, out, part, st);
 }
 
 int agk_distill_topk_bwd(const void* z, const int64_t* index, const void* t, const float* stats,
@@ -605,7 +587,7 @@ int agk_distill_topk_bwd(const void* z, const int64_t* index, const void* t, con
     const int64_t bytes = rows * cols * (dtype == AGK_F32 ? 4 : 2);
     if (dz != z && !agk::disjoint(dz, z, bytes)) return AGK_EINVAL;
     agk::clear_pending_error();
-    const Args a = args(z, index, t, rows, cols, k, temperature, t_dtype);
+    const Args a = args(z, index, t, rows, cols, k, temperature, dtype, t_dtype);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const float2* const in = reinterpret_cast<const float2*>(stats);
     const bool acc = accumulate != 0;

@@ -117,6 +117,17 @@ __device__ __forceinline__ void stage_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// ---- the order of K ----------------------------------------------------------------
+// Where the direct and ring kernels find k-tile t of an operand: LinearK, K once through.
+// (A product whose operands are stored as several bf16 planes brings an order of its own.)
+struct LinearK {
+    __device__ __forceinline__ int start(int n) { return n; }  // n whole k-tiles: the tiles in all
+    __device__ __forceinline__ int a(int t, int step) const { return t * step; }  // byte offsets
+    __device__ __forceinline__ int b(int t, int step) const { return t * step; }
+    __device__ __forceinline__ int more_a() const { return 0; }  // bytes past the first n tiles
+    __device__ __forceinline__ int more_b() const { return 0; }
+};
+
 // ---- tile order ----------------------------------------------------------------
 // Workgroups are dispatched round-robin over the 8 XCDs (workgroup L runs on
 // XCD L % 8), each XCD with its own L2.  The tile order below gives each XCD

@@ -70,20 +70,20 @@ struct DirectStage {
 };
 
 // Load j of a wave (j = 0..7) fills kilobyte wave * 8 + j of one operand's half
-// of `stage`; tile t's data starts t * step bytes into the operand.
-__device__ __forceinline__ void direct_issue_a(const DirectStage& d, uint16_t* stage, int t,
+// of `stage`; the tile's data starts `at` bytes into the operand.
+__device__ __forceinline__ void direct_issue_a(const DirectStage& d, uint16_t* stage, int at,
                                                int wave) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(d.ra, (lds_ptr_t)(stage + (wave * 8 + j) * 512),
-                                                 16, d.oa[j], t * d.step_a, 0, 0);
+                                                 16, d.oa[j], at, 0, 0);
 }
-__device__ __forceinline__ void direct_issue_b(const DirectStage& d, uint16_t* stage, int t,
+__device__ __forceinline__ void direct_issue_b(const DirectStage& d, uint16_t* stage, int at,
                                                int wave) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            d.rb, (lds_ptr_t)(stage + BM * BK + (wave * 8 + j) * 512), 16, d.ob[j], t * d.step_b,
+            d.rb, (lds_ptr_t)(stage + BM * BK + (wave * 8 + j) * 512), 16, d.ob[j], at,
             0, 0);
 }
 
@@ -179,21 +179,22 @@ __device__ __forceinline__ void mfma_sub(const Frags<NB>& f, f32x16 (&acc)[TM][N
     if constexpr (NB == 4) { \
         AGK_X8(AGK_RM)     \
     }
-template <bool FIRST, bool A_TR, bool B_TR, int NB>
-__device__ __forceinline__ void direct_step(const DirectStage& d, const uint16_t* cur,
+template <bool FIRST, bool A_TR, bool B_TR, int NB, class KM>
+__device__ __forceinline__ void direct_step(const DirectStage& d, const KM& km,
+                                            const uint16_t* cur,
                                             uint16_t* other, int t, int nk,
                                             f32x16 (&acc)[TM][NB], Frags<NB>& f0, Frags<NB>& f1,
                                             int wm, int bc, int frow, int fk, int lane,
                                             int wave) {
     const int tn = t + 1 < nk ? t + 1 : nk - 1;
-    direct_issue_a(d, other, tn, wave);
+    direct_issue_a(d, other, km.a(tn, d.step_a), wave);
     read_frags<A_TR, B_TR>(f0, cur, 0, wm, bc, frow, fk, lane);
     if constexpr (!FIRST) {
         mfma_sub(f1, acc);
         AGK_SUBSTEP_LRM
     }
     __builtin_amdgcn_sched_barrier(0);
-    direct_issue_b(d, other, tn, wave);
+    direct_issue_b(d, other, km.b(tn, d.step_b), wave);
     read_frags<A_TR, B_TR>(f1, cur, 1, wm, bc, frow, fk, lane);
     mfma_sub(f0, acc);
     AGK_SUBSTEP_LRM
@@ -236,8 +237,9 @@ __device__ __forceinline__ void store_half(const f32x16 (&acc)[TM][2 * TN], cons
 // Both stage the tile's full 256 B columns (the same loads).  TAIL: K is not a
 // multiple of 64; the last K % 64 k are multiplied first, staged through
 // registers into st1 (which tile 1's loads fill only after it).
-template <bool A_TR, bool B_TR, int NB, bool TAIL, class Epi>
-__device__ __forceinline__ void direct_tile(const DirectStage& d, uint16_t* st0, uint16_t* st1,
+template <bool A_TR, bool B_TR, int NB, bool TAIL, class Epi, class KM>
+__device__ __forceinline__ void direct_tile(const DirectStage& d, const KM& km, int nk,
+                                            uint16_t* st0, uint16_t* st1,
                                             const uint16_t* __restrict__ a0, int64_t lda,
                                             int rows_a, const uint16_t* __restrict__ b0,
                                             int64_t ldb, int rows_b, int K, int m0, int n0,
@@ -251,19 +253,19 @@ __device__ __forceinline__ void direct_tile(const DirectStage& d, uint16_t* st0,
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    const int nk = K / BK;  // >= 1
+    const int whole = K / BK;  // >= 1
     const int frow = lane & 31;
     const int fk = (lane >> 5) * 8;  // MFMA operand lanes 32..63 hold k 8..15
     const int bc = half_off + wn * (NB * 32);  // the wave's first B column in the stage
     if constexpr (TAIL) {
-        stage_k_tail<A_TR, BM>(st1, a0, lda, rows_a, nk * BK, K);
-        stage_k_tail<B_TR, BN>(st1 + BM * BK, b0, ldb, rows_b, nk * BK, K);
+        stage_k_tail<A_TR, BM>(st1, a0, lda, rows_a, whole * BK, K);
+        stage_k_tail<B_TR, BN>(st1 + BM * BK, b0, ldb, rows_b, whole * BK, K);
     }
-    direct_issue_a(d, st0, 0, wave);
-    direct_issue_b(d, st0, 0, wave);
+    direct_issue_a(d, st0, km.a(0, d.step_a), wave);
+    direct_issue_b(d, st0, km.b(0, d.step_b), wave);
     if constexpr (TAIL) {
         stage_barrier<16>();  // the tail's LDS writes, every wave (tile 0 still in flight)
-        for (int s = 0; s * 16 < K - nk * BK; ++s) {
+        for (int s = 0; s * 16 < K - whole * BK; ++s) {
             Frags<NB> f;
             read_frags<A_TR, B_TR>(f, st1, s, wm, bc, frow, fk, lane);
             mfma_sub(f, acc);
@@ -274,16 +276,16 @@ __device__ __forceinline__ void direct_tile(const DirectStage& d, uint16_t* st0,
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     Frags<NB> f0, f1;
-    direct_step<true, A_TR, B_TR>(d, st0, st1, 0, nk, acc, f0, f1, wm, bc, frow, fk, lane, wave);
+    direct_step<true, A_TR, B_TR>(d, km, st0, st1, 0, nk, acc, f0, f1, wm, bc, frow, fk, lane, wave);
     int t = 1;
     for (; t + 1 < nk; t += 2) {
-        direct_step<false, A_TR, B_TR>(d, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
+        direct_step<false, A_TR, B_TR>(d, km, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
                                        wave);
-        direct_step<false, A_TR, B_TR>(d, st0, st1, t + 1, nk, acc, f0, f1, wm, bc, frow, fk,
+        direct_step<false, A_TR, B_TR>(d, km, st0, st1, t + 1, nk, acc, f0, f1, wm, bc, frow, fk,
                                        lane, wave);
     }
     if (t < nk)
-        direct_step<false, A_TR, B_TR>(d, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
+        direct_step<false, A_TR, B_TR>(d, km, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
                                        wave);
     mfma_sub(f1, acc);  // substep 3 of the last tile
 
@@ -303,12 +305,13 @@ __device__ __forceinline__ void direct_tile(const DirectStage& d, uint16_t* st0,
 // (workgroup full_tiles + 2 h + q: half q of tile full_tiles + h), so that a
 // last round of few tiles runs on twice as many CUs for half as long.  Every
 // output element is summed in the same k order either way (bit-identical).
-template <bool A_TR, bool B_TR, bool TAIL, class Epi>
+template <bool A_TR, bool B_TR, bool TAIL, class Epi, class KM = LinearK>
 __device__ __forceinline__ void direct_body(const uint16_t* __restrict__ A, int64_t lda,
                                             const uint16_t* __restrict__ B, int64_t ldb, int M,
                                             int N, int K, int tiles_m, int tiles_n, int group_m,
                                             int full_tiles, uint16_t* st0, uint16_t* st1,
-                                            const Epi& epi) {
+                                            const Epi& epi, KM km = {}) {
+    const int nk = km.start(K / BK);
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     // wave-uniform, so kept in scalar registers (LDS destinations of the loads)
@@ -332,11 +335,13 @@ __device__ __forceinline__ void direct_body(const uint16_t* __restrict__ A, int6
     // position is the scalar offset, always inside the operand)
     d.ra = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(a0), static_cast<short>(0),
-        static_cast<int>(A_TR ? ((K - 1) * lda + rows_a) * 2 : ((rows_a - 1) * lda + K) * 2),
+        static_cast<int>(A_TR ? ((K - 1) * lda + rows_a) * 2 : ((rows_a - 1) * lda + K) * 2) +
+            km.more_a(),
         0x00020000);
     d.rb = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(b0), static_cast<short>(0),
-        static_cast<int>(B_TR ? ((K - 1) * ldb + rows_b) * 2 : ((rows_b - 1) * ldb + K) * 2),
+        static_cast<int>(B_TR ? ((K - 1) * ldb + rows_b) * 2 : ((rows_b - 1) * ldb + K) * 2) +
+            km.more_b(),
         0x00020000);
     d.step_a = A_TR ? static_cast<int>(BK * lda * 2) : BK * 2;
     d.step_b = B_TR ? static_cast<int>(BK * ldb * 2) : BK * 2;
@@ -344,10 +349,10 @@ __device__ __forceinline__ void direct_body(const uint16_t* __restrict__ A, int6
     direct_offsets<B_TR>(d.ob, wave, lane, rows_b, ldb);
 
     if (!halves)
-        direct_tile<A_TR, B_TR, 4, TAIL>(d, st0, st1, a0, lda, rows_a, b0, ldb, rows_b, K, m0, n0,
+        direct_tile<A_TR, B_TR, 4, TAIL>(d, km, nk, st0, st1, a0, lda, rows_a, b0, ldb, rows_b, K, m0, n0,
                                          0, wm, wn, lane, wave, epi);
     else
-        direct_tile<A_TR, B_TR, 2, TAIL>(d, st0, st1, a0, lda, rows_a, b0, ldb, rows_b, K, m0, n0,
+        direct_tile<A_TR, B_TR, 2, TAIL>(d, km, nk, st0, st1, a0, lda, rows_a, b0, ldb, rows_b, K, m0, n0,
                                          ((L - full_tiles) & 1) * (BN / 2), wm, wn, lane, wave,
                                          epi);
 }

@@ -196,7 +196,7 @@ struct RingOperands {
     const void *a, *b;
     int bytes_a, bytes_b;  // what the tile's loads can address
     int step_a, step_b;    // bytes from one k-tile to the next
-    int nk;                // whole 64-deep k-tiles
+    int nk;                // whole 64-deep k-tiles, in all
 };
 
 struct RingRsrc {
@@ -221,30 +221,33 @@ __device__ __forceinline__ void ring_load_b(const RingRsrc& q, uint16_t* lds, ui
 
 // Loads one operand of k-tile t (nothing past the last one: a zero-byte
 // resource).
-template <class SH>
-__device__ __forceinline__ void ring_issue_a(const RingOperands& r, const RingOffsets<SH>& o,
-                                             uint16_t* stage, int t, int wave) {
+template <class SH, class KM>
+__device__ __forceinline__ void ring_issue_a(const RingOperands& r, const KM& km,
+                                             const RingOffsets<SH>& o, uint16_t* stage, int t,
+                                             int wave) {
     const bool in = t < r.nk;
     const RingRsrc q = ring_rsrc(r, in);
 #pragma unroll
     for (int j = 0; j < SH::kBM / 32; ++j)
-        ring_load_a(q, stage + (wave * (SH::kBM / 32) + j) * 512, o.a[j], in ? t * r.step_a : 0);
+        ring_load_a(q, stage + (wave * (SH::kBM / 32) + j) * 512, o.a[j], in ? km.a(t, r.step_a) : 0);
 }
-template <class SH>
-__device__ __forceinline__ void ring_issue_b(const RingOperands& r, const RingOffsets<SH>& o,
-                                             uint16_t* stage, int t, int wave) {
+template <class SH, class KM>
+__device__ __forceinline__ void ring_issue_b(const RingOperands& r, const KM& km,
+                                             const RingOffsets<SH>& o, uint16_t* stage, int t,
+                                             int wave) {
     const bool in = t < r.nk;
     const RingRsrc q = ring_rsrc(r, in);
 #pragma unroll
     for (int j = 0; j < SH::kBN / 32; ++j)
         ring_load_b(q, stage + SH::kBM * BK + (wave * (SH::kBN / 32) + j) * 512, o.b[j],
-                    in ? t * r.step_b : 0);
+                    in ? km.b(t, r.step_b) : 0);
 }
-template <class SH>
-__device__ __forceinline__ void ring_issue(const RingOperands& r, const RingOffsets<SH>& o,
-                                           uint16_t* stage, int t, int wave) {
-    ring_issue_a<SH>(r, o, stage, t, wave);
-    ring_issue_b<SH>(r, o, stage, t, wave);
+template <class SH, class KM>
+__device__ __forceinline__ void ring_issue(const RingOperands& r, const KM& km,
+                                           const RingOffsets<SH>& o, uint16_t* stage, int t,
+                                           int wave) {
+    ring_issue_a<SH>(r, km, o, stage, t, wave);
+    ring_issue_b<SH>(r, km, o, stage, t, wave);
 }
 
 // Scheduling groups of a substep: one load (if LOADS), READS fragment reads,
@@ -261,8 +264,8 @@ __device__ __forceinline__ void ring_sched() {
 
 // One k-tile out of `cur`, loading tile `ahead` into `into` (the stage the
 // previous step read).  FIRST: no straddling substep to multiply.
-template <bool FIRST, bool A_TR, bool B_TR, class SH>
-__device__ __forceinline__ void ring_step(const RingOperands& r,
+template <bool FIRST, bool A_TR, bool B_TR, class SH, class KM>
+__device__ __forceinline__ void ring_step(const RingOperands& r, const KM& km,
                                           const RingOffsets<SH>& o, const uint16_t* cur,
                                           uint16_t* into, int ahead,
                                           f32x16 (&acc)[SH::kTm][SH::kTn],
@@ -272,14 +275,14 @@ __device__ __forceinline__ void ring_step(const RingOperands& r,
     constexpr int kMfma = SH::kTm * SH::kTn;
     constexpr int kReads = SH::kTm * (A_TR ? 2 : 1) + SH::kTn * (B_TR ? 2 : 1);
     constexpr int kPer = (kReads + kMfma - 1) / kMfma;
-    ring_issue_a<SH>(r, o, into, ahead, wave);
+    ring_issue_a<SH>(r, km, o, into, ahead, wave);
     ring_read<A_TR, B_TR, SH>(f0, cur, 0, wm, wn, lane);
     if constexpr (!FIRST) {
         ring_mfma(f1, acc);
         ring_sched<kMfma, kPer, true>();
     }
     __builtin_amdgcn_sched_barrier(0);
-    ring_issue_b<SH>(r, o, into, ahead, wave);
+    ring_issue_b<SH>(r, km, o, into, ahead, wave);
     ring_read<A_TR, B_TR, SH>(f1, cur, 1, wm, wn, lane);
     ring_mfma(f0, acc);
     ring_sched<kMfma, kPer, true>();
@@ -306,11 +309,11 @@ __device__ __forceinline__ void ring_tail(const uint16_t* stage, int k_left,
     }
 }
 
-template <bool A_TR, bool B_TR, class SH, class Epi>
+template <bool A_TR, bool B_TR, class SH, class Epi, class KM = LinearK>
 __device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_t lda,
                                           const uint16_t* __restrict__ B, int64_t ldb, int M,
                                           int N, int K, int tiles_m, int tiles_n, int group_m,
-                                          const Epi& epi) {
+                                          const Epi& epi, KM km = {}) {
     constexpr int NST = SH::kStages;
     __shared__ __attribute__((aligned(16))) uint16_t st0[SH::kElems];
     __shared__ __attribute__((aligned(16))) uint16_t st1[SH::kElems];
@@ -339,7 +342,10 @@ __device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_
     r.bytes_b = static_cast<int>(B_TR ? ((K - 1) * ldb + rows_b) * 2 : ((rows_b - 1) * ldb + K) * 2);
     r.step_a = A_TR ? static_cast<int>(BK * lda * 2) : BK * 2;
     r.step_b = B_TR ? static_cast<int>(BK * ldb * 2) : BK * 2;
-    r.nk = K / BK;
+    const int whole = K / BK;
+    r.nk = km.start(whole);
+    r.bytes_a += km.more_a();
+    r.bytes_b += km.more_b();
     RingOffsets<SH> o;
     ring_offsets<A_TR, SH::kBM>(o.a, wave, lane, rows_a, lda);
     ring_offsets<B_TR, SH::kBN>(o.b, wave, lane, rows_b, ldb);
@@ -355,14 +361,14 @@ __device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_
     // The K % 64 tail goes first, through the last stage, whose own loads are
     // issued by step 0.
     uint16_t* const last = NST == 3 ? st2 : st3;
-    const int k_left = K - r.nk * BK;
+    const int k_left = K - whole * BK;
     if (k_left) {
-        stage_k_tail<A_TR, SH::kBM>(last, a0, lda, rows_a, r.nk * BK, K);
-        stage_k_tail<B_TR, SH::kBN>(last + SH::kBM * BK, b0, ldb, rows_b, r.nk * BK, K);
+        stage_k_tail<A_TR, SH::kBM>(last, a0, lda, rows_a, whole * BK, K);
+        stage_k_tail<B_TR, SH::kBN>(last + SH::kBM * BK, b0, ldb, rows_b, whole * BK, K);
     }
-    ring_issue<SH>(r, o, st0, 0, wave);
-    ring_issue<SH>(r, o, st1, 1, wave);
-    if constexpr (NST > 3) ring_issue<SH>(r, o, st2, 2, wave);
+    ring_issue<SH>(r, km, o, st0, 0, wave);
+    ring_issue<SH>(r, km, o, st1, 1, wave);
+    if constexpr (NST > 3) ring_issue<SH>(r, km, o, st2, 2, wave);
     if (k_left) {
         stage_barrier<(NST - 1) * SH::kLoads>();  // the tail's LDS writes, every wave
         ring_tail<A_TR, B_TR, SH>(last, k_left, acc, wm, wn, lane);
@@ -372,8 +378,8 @@ __device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_
     if (r.nk > 0) {
         RingFrags<SH::kTm, SH::kTn> f0, f1;
 #define AGK_RING(FIRST, CUR, INTO, t)                                                           \
-    ring_step<FIRST, A_TR, B_TR, SH>(r, o, CUR, INTO, (t) + NST - 1, acc, f0, f1, wm, wn, lane, \
-                                     wave)
+    ring_step<FIRST, A_TR, B_TR, SH>(r, km, o, CUR, INTO, (t) + NST - 1, acc, f0, f1, wm, wn,   \
+                                     lane, wave)
         AGK_RING(true, st0, last, 0);
         int t = 1;
         if constexpr (NST == 3) {

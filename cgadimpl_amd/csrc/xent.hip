@@ -7,11 +7,12 @@
 // each wave's block of z^T leaves as {max, sum of exponentials} per token, 8 bytes for 32 to
 // 128 logits, and a second kernel joins a token's blocks.  The backward makes z
 // again, a piece of the vocabulary at a time, leaving G's piece in bf16 (the matrix
-// cores' operand), and takes the two products from it.  dw's rows belong to one piece; dx adds up in fp32 over the pieces.
-// 8 tokens vocab cols flop a step, 2 of the forward and 6 of the backward (2 of them
-// the logits again: the price of not keeping them).
+// cores' operand), and takes the two products from it.  dw's rows belong to one piece;
+// dx adds up in fp32 over the pieces.  8 tokens vocab cols flop a step, 2 of the forward and
+// 6 of the backward (2 of them the logits again: the price of not keeping them).
 //
-// fp32.  The same pieces on the fp32 product of gemm_f32.hip, z^T's piece in memory.
+// fp32.  The same kernels on operands split into three bf16 planes (PlanesK), x once a call
+// and w a piece at a time; G leaves its kernel split.
 //
 // A token that is left out (a negative label, or a zero dloss) has a zero row of G
 // whatever its logits are, and the product over tokens reads its row of x as zeros,
@@ -90,32 +91,86 @@ __global__ __launch_bounds__(kJoinLanes) void xent_join(
 
 // ---- the backward's weights ---------------------------------------------------------
 
-// weight[t] = dloss[t] / *alpha for a token with a label, 0 for one without, NaN for
-// one whose label is past the vocabulary; zeros to padded.  *alpha: the largest finite
-// |dloss| of the tokens with a label (1 where that is 0), or 1 if !SCALE.  One workgroup: a few
-// thousand values.
-template <bool SCALE>
-__global__ __launch_bounds__(1024) void xent_weights(const float* __restrict__ dloss,
-                                                     const int64_t* __restrict__ labels,
-                                                     float* __restrict__ weight,
-                                                     float* __restrict__ alpha, int64_t tokens,
-                                                     int64_t padded, int64_t vocab) {
+// Row `row` of an fp32 matrix (NULL: zeros) as three bf16 planes of kp values, by `lanes`
+// lanes; zeros past cols.
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void split_row(const float* __restrict__ src, int cols, int kp,
+                                          uint16_t* __restrict__ dst, int lane, int lanes) {
+    for (int c = lane * 4; c < kp; c += lanes * 4) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (src && c + 4 <= cols) {
+            const f32x4_a4 q = *reinterpret_cast<const f32x4_a4*>(src + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = q[e];
+        } else if (src) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < cols) v[e] = src[c + e];
+        }
+        uint32_t lo[3], hi[3];
+        split3(v[0], v[1], lo);
+        split3(v[2], v[3], hi);
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            *reinterpret_cast<uint2*>(dst + q * kp + c) = make_uint2(lo[q], hi[q]);
+    }
+}
+
+// Rows [0, rows) of src, and zeros in those up to padded: four rows per workgroup.
+__global__ __launch_bounds__(256) void xent_split(const float* __restrict__ src, int64_t ld,
+                                                  int64_t rows, int64_t padded, int cols, int kp,
+                                                  uint16_t* __restrict__ dst) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < padded;
+         r += static_cast<int64_t>(gridDim.x) * 4)
+        split_row(r < rows ? src + r * ld : nullptr, cols, kp, dst + r * (3 * static_cast<int64_t>(kp)),
+                  static_cast<int>(threadIdx.x & 63), 64);
+}
+
+// The first workgroup: weight[t] = dloss[t] / *alpha for a token with a label, 0 for one
+// without, NaN for one whose label is past the vocabulary; zeros to padded.  *alpha: the
+// largest finite |dloss| of the tokens with a label (1 where that is 0) for bf16, 1 for fp32.
+// The others: a token's row each, x[t], or zeros for one that is left out, as the products'
+// operand: a copy of cols values (bf16), or three planes of kp (fp32; rows to padded64 of zeros).
+template <bool BF16>
+__global__ __launch_bounds__(1024) void xent_tokens(const float* __restrict__ dloss,
+                                                    const int64_t* __restrict__ labels,
+                                                    float* __restrict__ weight,
+                                                    float* __restrict__ alpha, int64_t tokens,
+                                                    int64_t padded, int64_t vocab,
+                                                    const void* __restrict__ x, int64_t ldx,
+                                                    uint16_t* __restrict__ dst, int cols, int kp,
+                                                    int64_t padded64) {
+    if (blockIdx.x > 0) {
+        const int lane = static_cast<int>(threadIdx.x & 255);
+        for (int64_t t = (static_cast<int64_t>(blockIdx.x) - 1) * 4 + (threadIdx.x >> 8);
+             t < (BF16 ? tokens : padded64); t += (static_cast<int64_t>(gridDim.x) - 1) * 4) {
+            const bool keep = t < tokens && labels[t] >= 0 && dloss[t] != 0.0f;
+            if constexpr (BF16) {
+                const agk::u32x4* const from = reinterpret_cast<const agk::u32x4*>(
+                    static_cast<const uint16_t*>(x) + t * ldx);
+                agk::u32x4* const to = reinterpret_cast<agk::u32x4*>(dst + t * cols);
+                for (int c = lane; c < cols / 8; c += 256)
+                    to[c] = keep ? from[c] : agk::u32x4{0u, 0u, 0u, 0u};
+            } else {
+                split_row(keep ? static_cast<const float*>(x) + t * ldx : nullptr, cols, kp,
+                          dst + t * (3 * static_cast<int64_t>(kp)), lane, 256);
+            }
+        }
+        return;
+    }
     float c = 1.0f;
-    if constexpr (SCALE) {
-        __shared__ float red[1024];
+    if constexpr (BF16) {
+        __shared__ float red[16];
         float m = 0.0f;
         for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
             const float d = fabsf(dloss[t]);
             if (labels[t] >= 0 && d < __builtin_inff()) m = fmaxf(m, d);
         }
-        red[threadIdx.x] = m;
-        for (int h = 512; h > 0; h /= 2) {
-            __syncthreads();
-            if (static_cast<int>(threadIdx.x) < h)
-                red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + h]);
-        }
+        for (int h = 32; h > 0; h /= 2) m = fmaxf(m, __shfl_xor(m, h));
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
         __syncthreads();
-        c = red[0] > 0.0f ? red[0] : 1.0f;
+        for (int w = 0; w < 16; ++w) m = fmaxf(m, red[w]);
+        c = m > 0.0f ? m : 1.0f;
     }
     for (int64_t t = threadIdx.x; t < padded; t += 1024) {
         float w = 0.0f;
@@ -129,18 +184,6 @@ __global__ __launch_bounds__(1024) void xent_weights(const float* __restrict__ d
     if (threadIdx.x == 0) *alpha = c;
 }
 
-// dst[t] = x[t], or zeros for a token that is left out; rows of cols (T: 16 bytes of
-// bf16, or one float).
-template <class T>
-__global__ __launch_bounds__(256) void xent_keep_rows(const T* __restrict__ x, int64_t ldx,
-                                                      const float* __restrict__ weight,
-                                                      T* __restrict__ dst, int cols) {
-    const int64_t t = blockIdx.x;
-    const bool keep = weight[t] != 0.0f;
-    for (int c = threadIdx.x; c < cols; c += 256)
-        dst[t * cols + c] = keep ? x[t * ldx + c] : T{};
-}
-
 // dx (+)= alpha * (the K slices' sums, added in order), rounded to bf16 once.
 __global__ __launch_bounds__(256) void xent_dx_out(const float* __restrict__ acc, int slices,
                                                    int64_t slice, const float* __restrict__ alpha,
@@ -150,17 +193,21 @@ __global__ __launch_bounds__(256) void xent_dx_out(const float* __restrict__ acc
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= n8) return;
     const float a = *alpha;
-    float v[8];
-    const float4* p = reinterpret_cast<const float4*>(acc + i * 8);
-    *reinterpret_cast<float4*>(v) = p[0];
-    *reinterpret_cast<float4*>(v + 4) = p[1];
-    for (int s = 1; s < slices; ++s) {
-        float u[8];
-        const float4* q = reinterpret_cast<const float4*>(acc + s * slice + i * 8);
-        *reinterpret_cast<float4*>(u) = q[0];
-        *reinterpret_cast<float4*>(u + 4) = q[1];
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < slices; s0 += 4) {  // four slices' loads before they are added
+        float u[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += u[e];
+        for (int s = 0; s < 4; ++s) {
+            const float4* q = reinterpret_cast<const float4*>(
+                acc + (s0 + s < slices ? s0 + s : slices - 1) * slice + i * 8);
+            *reinterpret_cast<float4*>(u[s]) = q[0];
+            *reinterpret_cast<float4*>(u[s] + 4) = q[1];
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s0 + s < slices)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += u[s][e];
     }
     const bool keep = weight[i / cols8] != 0.0f;
 #pragma unroll
@@ -175,57 +222,39 @@ __global__ __launch_bounds__(256) void xent_dx_out(const float* __restrict__ acc
     *out = agk::BF16::pack(v);
 }
 
-// ---- fp32: z^T's piece in memory ------------------------------------------------------
-
-// A piece's blocks of kZRows vocabulary rows: {max, sum} per token and the labels'
-// logits, as LseEpi leaves them.
-constexpr int kZRows = 32;
-__global__ __launch_bounds__(256) void xent_piece_lse(const float* __restrict__ z, int rows,
-                                                      int64_t v0, int64_t tokens,
-                                                      const int64_t* __restrict__ labels,
-                                                      float2* __restrict__ part,
-                                                      float* __restrict__ picked) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (t >= tokens) return;
-    const int r0 = static_cast<int>(blockIdx.y) * kZRows;
-    float v[kZRows];
+// The same for fp32: dx (+)= the slices' sums (rows of cols8), four columns per lane.
+__global__ __launch_bounds__(256) void xent_dx_out32(const float* __restrict__ acc, int slices,
+                                                     int64_t slice,
+                                                     const float* __restrict__ weight,
+                                                     float* __restrict__ dx, int64_t rows, int cols,
+                                                     int cols8, int accumulate) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = i / (cols8 / 4);
+    const int c = static_cast<int>(i - row * (cols8 / 4)) * 4;
+    if (row >= rows) return;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < slices; s0 += 4) {
+        float4 u[4];
 #pragma unroll
-    for (int r = 0; r < kZRows; ++r)
-        v[r] = r0 + r < rows ? z[static_cast<int64_t>(r0 + r) * tokens + t] : -__builtin_inff();
-    float m = v[0];
+        for (int s = 0; s < 4; ++s)
+            u[s] = *reinterpret_cast<const float4*>(
+                acc + (s0 + s < slices ? s0 + s : slices - 1) * slice + i * 4);
 #pragma unroll
-    for (int r = 1; r < kZRows; ++r) m = max_of(m, v[r]);
-    const float shift = m == -__builtin_inff() ? 0.0f : m;
-    float s = 0.0f;
+        for (int s = 0; s < 4; ++s)
+            if (s0 + s < slices) {
+                v[0] += u[s].x;
+                v[1] += u[s].y;
+                v[2] += u[s].z;
+                v[3] += u[s].w;
+            }
+    }
+    const bool keep = weight[row] != 0.0f;
 #pragma unroll
-    for (int r = 0; r < kZRows; ++r) s += exp_of(v[r] - shift);
-    part[(v0 / kZRows + blockIdx.y) * tokens + t] = make_float2(m, s);
-    const int at = label_row(labels[t], v0 + r0, kZRows);
-    if (at >= 0 && r0 + at < rows) picked[t] = z[static_cast<int64_t>(r0 + at) * tokens + t];
-}
-
-// z^T's piece becomes G^T's.
-__global__ __launch_bounds__(256) void xent_piece_grad(float* __restrict__ z, int rows, int64_t v0,
-                                                       int64_t tokens,
-                                                       const int64_t* __restrict__ labels,
-                                                       const float2* __restrict__ stats,
-                                                       const float* __restrict__ weight) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (t >= tokens) return;
-    const int r0 = static_cast<int>(blockIdx.y) * kZRows;
-    const float2 st = stats[t];
-    const float w = weight[t];
-    const int at = label_row(labels[t], v0 + r0, kZRows);
-    float v[kZRows];
-#pragma unroll
-    for (int r = 0; r < kZRows; ++r)
-        if (r0 + r < rows) v[r] = z[static_cast<int64_t>(r0 + r) * tokens + t];
-#pragma unroll
-    for (int r = 0; r < kZRows; ++r)
-        if (r0 + r < rows) {
-            float p = exp_of((v[r] - st.x) - st.y);
-            p -= at == r ? 1.0f : 0.0f;
-            z[static_cast<int64_t>(r0 + r) * tokens + t] = w != 0.0f ? w * p : 0.0f;
+    for (int e = 0; e < 4; ++e)
+        if (c + e < cols) {
+            float* const p = dx + row * cols + c + e;
+            const float g = keep ? v[e] : 0.0f;
+            *p = accumulate ? agk::acc_add(*p, g) : g;
         }
 }
 
@@ -245,7 +274,6 @@ __global__ __launch_bounds__(256) void xent_zero(uint32_t* __restrict__ out, int
 // 8192 / 16384 / 32768 rows, one piece) 2843 / 2805 / 2698 / 2444.
 constexpr int64_t kPieceBytes = 512LL << 20;
 constexpr int64_t kMaxOperand = 1LL << 30;    // values a product's 31-bit offsets reach
-constexpr int64_t kMaxPiece = 1LL << 20;      // vocabulary rows, 32 per grid row of the fp32 kernels
 constexpr int64_t kMaxTokens = 1LL << 24;     // a workgroup per token within a grid
 
 // G's rows are padded to whole 128-byte lines of bf16: the products fetch 128 bytes of
@@ -256,13 +284,13 @@ inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 inline size_t region(int64_t bytes) { return static_cast<size_t>(up(bytes, 256)); }
 
 // The vocabulary rows of a piece: `asked`, or what fills kPieceBytes, cut to equal
-// pieces of whole 256-row tiles that the products' offsets reach.
-inline int64_t piece_rows(int64_t rows, int64_t vocab, int64_t ldw, int size, int64_t asked) {
-    const int64_t row_bytes = up(rows, kLine) * size;
-    int64_t p = asked > 0 ? up(std::min(asked, vocab), 256) : kPieceBytes / row_bytes;
-    p = std::min(p, kMaxPiece);
-    if (size == 2) p = std::min(p, std::min(kMaxOperand / ldw, kMaxOperand / up(rows, kLine)));
-    p = std::max<int64_t>(p / 256 * 256, 256);
+// pieces of whole 256-row tiles that the products' offsets reach.  per_row: values of the
+// operands' longest row (G's or w's, in all planes).
+inline int64_t piece_rows(int64_t vocab, int64_t ldg, int64_t ldw, int planes, int64_t asked) {
+    const int64_t most = kMaxOperand / (planes * std::max(ldg, ldw));
+    int64_t p = asked > 0 ? up(std::min(asked, vocab), 256)
+                          : kPieceBytes / (2 * planes * (planes == 1 ? ldg : std::max(ldg, ldw)));
+    p = std::max<int64_t>(std::min(p, most) / 256 * 256, 256);
     if (p >= vocab) return vocab;
     const int64_t n = (vocab + p - 1) / p;
     return up((vocab + n - 1) / n, 256);
@@ -291,10 +319,10 @@ inline int lse_block(int shape) {
         default: return 32;
     }
 }
-// Blocks per token that the workspace holds, whatever tile a device's compute units give.
-inline int64_t max_blocks(int64_t rows, int64_t vocab, int dtype) {
-    const int64_t least = dtype == AGK_BF16 && rows > kFewTokens ? 64 : 32;
-    return (vocab + least - 1) / least;
+// Blocks per token that the workspace holds, whatever tiles a device's compute units give.
+inline int64_t max_blocks(int64_t rows, int64_t vocab, int64_t piece) {
+    const int64_t least = rows > kFewTokens ? 64 : 32;
+    return ((vocab + piece - 1) / piece) * ((piece + least - 1) / least);
 }
 
 // The tile and K slices of dx = G w.  K is the piece's vocabulary rows, far longer than
@@ -305,7 +333,7 @@ inline int64_t max_blocks(int64_t rows, int64_t vocab, int dtype) {
 struct DxPlan {
     int shape, slices, k_slice;
 };
-inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k) {
+inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks) {
     using namespace agk_gemm;
     const int64_t cus = device_cus();
     DxPlan best{pick_shape(rows8, cols, k, device_cus()), 1, static_cast<int>(up(k, 64))};
@@ -313,14 +341,14 @@ inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k) {
     for (const RingCost& s : kRingCosts) {
         const int64_t tiles = ((rows8 + s.bm - 1) / s.bm) * ((cols + s.bn - 1) / s.bn);
         const double slots = static_cast<double>(cus * s.per_cu);
-        for (int64_t n = 1; n <= kMaxSlices && (n == 1 || n * kMinSlice <= k); ++n) {
+        for (int64_t n = 1; n <= kMaxSlices && (n == 1 || n * kMinSlice <= k * walks); ++n) {
             if (k < BK || !agk::grid_fits(tiles, 256)) break;
             const int64_t ks = up((k + n - 1) / n, 64), m = (k + ks - 1) / ks;
             if (m != n || k - (n - 1) * ks < BK) continue;  // every slice has a whole k-tile
             const double load = static_cast<double>(tiles * n) / slots;
             const double rounds = static_cast<double>(static_cast<int64_t>(load));
             const double fill = load - rounds;
-            const double steps = static_cast<double>(ks) / 64;
+            const double steps = static_cast<double>(ks) / 64 * walks;
             // the 256 x 256 kernel on two k-strided operands and a long K: 1.36 us a step at 53 %
             // fill, 1.64-1.70 full
             const double light = s.id == 0 ? 1.25 : s.light, full = s.id == 0 ? 1.65 : s.full;
@@ -349,28 +377,51 @@ inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
     return d;
 }
 
-// The backward's workspace.
-struct Layout {
-    int64_t piece, rows8, ldg;
-    size_t weight, alpha, keep, g, acc, total;
+// The workspaces.  `cols` of the operands as staged: kp for planes (whole k-tiles).
+struct FwdLayout {
+    int64_t kp, piece;
+    size_t picked, part, x3, w3, total;
 };
-inline Layout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t ldw, int dtype,
-                         int64_t piece) {
-    Layout o;
-    const int size = dtype == AGK_F32 ? 4 : 2;
+inline FwdLayout fwd_layout(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
+    FwdLayout o;
+    const bool bf16 = dtype == AGK_BF16;
+    o.kp = up(cols, 64);
+    o.piece = bf16 ? vocab : piece_rows(vocab, 64, o.kp, 3, 0);
+    o.picked = 0;
+    o.part = o.picked + region(rows * 4);
+    o.x3 = o.part + region(max_blocks(rows, vocab, o.piece) * rows * 8);
+    o.w3 = o.x3 + (bf16 ? 0 : region(rows * o.kp * 6));
+    o.total = o.w3 + (bf16 ? 0 : region(o.piece * o.kp * 6));
+    return o;
+}
+
+struct BwdLayout {
+    int planes;
+    int64_t piece, padded;             // vocabulary rows of a piece, and of its operands
+    int64_t rows8, rows64, ldg, kp, cols8;
+    DxPlan dx;
+    size_t weight, alpha, x, w3, g, acc, total;
+};
+inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t ldw, int dtype,
+                            int64_t piece) {
+    BwdLayout o;
+    const bool bf16 = dtype == AGK_BF16;
+    o.planes = bf16 ? 1 : 3;
     o.rows8 = up(rows, 8);
-    o.ldg = dtype == AGK_F32 ? rows : up(rows, kLine);
-    o.piece = piece_rows(rows, vocab, ldw, size, piece);
+    o.rows64 = up(rows, 64);
+    o.ldg = up(rows, kLine);
+    o.kp = up(cols, 64);
+    o.cols8 = up(cols, 8);
+    o.piece = piece_rows(vocab, o.ldg, bf16 ? ldw : o.kp, o.planes, piece);
+    o.padded = bf16 ? o.piece : up(o.piece, 64);
+    o.dx = dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : 6);
     o.weight = 0;
     o.alpha = o.weight + region(o.rows8 * 4);
-    o.keep = o.alpha + region(4);
-    o.g = o.keep + region(rows * cols * size);
-    o.acc = o.g + region(o.piece * o.ldg * size);
-    o.total = o.acc;
-    if (dtype == AGK_BF16) {
-        const DxPlan d = dx_plan(o.rows8, cols, o.piece);
-        o.total += region(static_cast<int64_t>(d.slices) * o.rows8 * cols * 4);
-    }
+    o.x = o.alpha + region(4);
+    o.w3 = o.x + region(bf16 ? rows * cols * 2 : o.rows64 * o.kp * 6);
+    o.g = o.w3 + (bf16 ? 0 : region(o.padded * o.kp * 6));
+    o.acc = o.g + region(o.padded * o.ldg * 2 * o.planes);
+    o.total = o.acc + region(static_cast<int64_t>(o.dx.slices) * o.rows8 * o.cols8 * 4);
     return o;
 }
 
@@ -388,7 +439,8 @@ inline int check_args(const void* x, int64_t ldx, const void* w, int64_t ldw, in
     if (dtype == AGK_BF16) {
         if (cols % 8 || ldx % 8 || ldw % 8 || !aligned16(x) || !aligned16(w)) return AGK_EINVAL;
         if (256 * ldw > kMaxOperand || 256 * ldx > kMaxOperand) return AGK_EINVAL;
-    } else if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 3u) {
+    } else if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 3u) ||
+               cols > kMaxOperand / 1024) {  // 256 rows of three planes
         return AGK_EINVAL;
     }
     return AGK_OK;
@@ -407,6 +459,15 @@ int launch_join(const float2* part, int64_t blocks, const float* picked, const i
     return check_launch();
 }
 
+// Launches a matrix's split: rows of three planes of kp.
+int launch_split(const float* src, int64_t ld, int64_t rows, int64_t padded, int64_t cols,
+                 int64_t kp, uint16_t* dst, hipStream_t st) {
+    const int64_t groups = std::min<int64_t>((padded + 3) / 4, 65536);
+    hipLaunchKernelGGL(xent_split, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, src, ld,
+                       rows, padded, static_cast<int>(cols), static_cast<int>(kp), dst);
+    return check_launch();
+}
+
 }  // namespace agk_xent
 
 extern "C" {
@@ -414,9 +475,7 @@ extern "C" {
 size_t agk_linear_xent_fwd_workspace_bytes(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
     using namespace agk_xent;
     if (rows <= 0 || vocab <= 0 || cols <= 0 || !agk::valid_dtype(dtype)) return 0;
-    size_t b = region(rows * 4) + region(max_blocks(rows, vocab, dtype) * rows * 8);
-    if (dtype == AGK_F32) b += region(piece_rows(rows, vocab, cols, 4, 0) * rows * 4);
-    return b;
+    return fwd_layout(rows, vocab, cols, dtype).total;
 }
 
 int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
@@ -424,51 +483,50 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
                         size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t cols,
                         int dtype, agk_stream_t stream) {
     using namespace agk_xent;
-    const int rc = check_args(x, ldx, w, ldw, rows, vocab, cols, dtype);
+    int rc = check_args(x, ldx, w, ldw, rows, vocab, cols, dtype);
     if (rc != AGK_OK || rows == 0) return rc;
-    if (!labels || !loss || !stats || ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(labels)) & 7u))
+    if (!labels || !loss || !stats ||
+        ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(labels)) & 7u))
         return AGK_EINVAL;
-    if (!workspace ||
-        workspace_bytes < agk_linear_xent_fwd_workspace_bytes(rows, vocab, cols, dtype))
-        return AGK_EWORKSPACE;
+    const FwdLayout o = fwd_layout(rows, vocab, cols, dtype);
+    if (!workspace || workspace_bytes < o.total) return AGK_EWORKSPACE;
     if (!aligned16(workspace)) return AGK_EINVAL;
     agk::clear_pending_error();
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     char* const ws = static_cast<char*>(workspace);
-    float* const picked = reinterpret_cast<float*>(ws);
-    float2* const part = reinterpret_cast<float2*>(ws + region(rows * 4));
-    float2* const out = reinterpret_cast<float2*>(stats);
-    if (dtype == AGK_BF16) {
-        const int shape = lse_shape(rows, vocab, cols);
-        const int block = lse_block(shape);
-        const Product p{static_cast<const uint16_t*>(w), ldw, static_cast<const uint16_t*>(x), ldx,
-                        static_cast<int>(vocab), static_cast<int>(rows), static_cast<int>(cols), 1,
-                        0, st};
-        const LseEpi e{part, picked, labels, static_cast<int>(vocab), static_cast<int>(rows)};
-        const int r = launch_lse(shape, p, e);
-        if (r != AGK_OK) return r;
-        return launch_join(part, (vocab + block - 1) / block, picked, labels, loss, out, rows,
-                           vocab, st);
+    float* const picked = reinterpret_cast<float*>(ws + o.picked);
+    float2* const part = reinterpret_cast<float2*>(ws + o.part);
+    uint16_t* const x3 = reinterpret_cast<uint16_t*>(ws + o.x3);
+    uint16_t* const w3 = reinterpret_cast<uint16_t*>(ws + o.w3);
+    const bool bf16 = dtype == AGK_BF16;
+    const int m = static_cast<int>(rows), kp = static_cast<int>(o.kp);
+    int64_t blocks = 0;
+    if (!bf16 && (rc = launch_split(static_cast<const float*>(x), ldx, rows, rows, cols, kp, x3,
+                                    st)) != AGK_OK)
+        return rc;
+    for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
+        const int64_t n = std::min(o.piece, vocab - v0);
+        const int shape = lse_shape(rows, n, bf16 ? cols : o.kp);
+        const LseEpi e{part + blocks * rows, picked, labels, v0, static_cast<int>(n), m};
+        if (bf16) {
+            rc = launch_lse(shape,
+                            Product{static_cast<const uint16_t*>(w), ldw,
+                                    static_cast<const uint16_t*>(x), ldx, static_cast<int>(n), m,
+                                    static_cast<int>(cols), 1, 0, st},
+                            e);
+        } else {
+            rc = launch_split(static_cast<const float*>(w) + v0 * ldw, ldw, n, n, cols, kp, w3, st);
+            if (rc != AGK_OK) return rc;
+            rc = launch_lse(shape,
+                            Product{w3, 3 * o.kp, x3, 3 * o.kp, static_cast<int>(n), m, kp, 1, 0,
+                                    st},
+                            e, PlanesK{kp * 2, kp * 2, 0});
+        }
+        if (rc != AGK_OK) return rc;
+        blocks += (n + lse_block(shape) - 1) / lse_block(shape);
     }
-    const int64_t piece = piece_rows(rows, vocab, cols, 4, 0);
-    float* const z = reinterpret_cast<float*>(
-        ws + region(rows * 4) + region(max_blocks(rows, vocab, dtype) * rows * 8));
-    for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
-        const int64_t n = std::min(piece, vocab - v0);
-        int r = agk_gemm_f32(static_cast<const float*>(w) + v0 * ldw, ldw, 0,
-                             static_cast<const float*>(x), ldx, 1, z, rows, n, rows, cols, 0,
-                             stream);
-        if (r != AGK_OK) return r;
-        hipLaunchKernelGGL(xent_piece_lse,
-                           dim3(static_cast<unsigned>((rows + 255) / 256),
-                                static_cast<unsigned>((n + kZRows - 1) / kZRows)),
-                           dim3(256), 0, st, z, static_cast<int>(n), v0, rows, labels, part,
-                           picked);
-        r = check_launch();
-        if (r != AGK_OK) return r;
-    }
-    return launch_join(part, (vocab + kZRows - 1) / kZRows, picked, labels, loss, out, rows, vocab,
-                       st);
+    return launch_join(part, blocks, picked, labels, loss, reinterpret_cast<float2*>(stats), rows,
+                       vocab, st);
 }
 
 size_t agk_linear_xent_bwd_workspace_bytes(int64_t rows, int64_t vocab, int64_t cols, int dtype,
@@ -497,7 +555,7 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         if (!dw || acc_dw) return AGK_OK;
         if (vocab > INT64_MAX / 16 / cols) return AGK_EINVAL;
         agk::clear_pending_error();
-        const int64_t n = vocab * cols * dw_size / 4;
+        const int64_t n = vocab * cols * dw_size / 4;  // bf16: cols is even
         hipLaunchKernelGGL(xent_zero, dim3(agk::capped_blocks((n + 255) / 256, 256)), dim3(256), 0,
                            st, static_cast<uint32_t*>(dw), n);
         return check_launch();
@@ -506,114 +564,101 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(labels)) & 7u))
         return AGK_EINVAL;
     if (!dx && !dw) return AGK_OK;
-    if (dtype == AGK_BF16) {
-        if (dx && !aligned16(dx)) return AGK_EINVAL;
-        if (rows > kMaxOperand / std::max(ldx, cols)) return AGK_EINVAL;
-    } else if (dx && (reinterpret_cast<uintptr_t>(dx) & 3u)) {
+    const bool bf16 = dtype == AGK_BF16;
+    if (dx && (reinterpret_cast<uintptr_t>(dx) & (bf16 ? 15u : 3u))) return AGK_EINVAL;
+    // 31-bit offsets of the products over tokens
+    if (bf16 ? rows > kMaxOperand / ldx : up(rows, 64) > kMaxOperand / (3 * up(cols, 64)))
         return AGK_EINVAL;
-    }
-    Layout o = bwd_layout(rows, vocab, cols, cols, dtype, piece);
+    BwdLayout o = bwd_layout(rows, vocab, cols, cols, dtype, piece);
     if (!workspace || workspace_bytes < o.total) return AGK_EWORKSPACE;
     if (!aligned16(workspace)) return AGK_EINVAL;
-    // a wider ldw may need smaller pieces than the workspace was sized for
-    if (dtype == AGK_BF16) o.piece = std::min(o.piece, piece_rows(rows, vocab, ldw, 2, piece));
+    if (bf16) {  // a wider ldw may need smaller pieces than the workspace was sized for
+        const int64_t p = piece_rows(vocab, o.ldg, ldw, 1, piece);
+        if (p < o.piece) {
+            o.piece = p;
+            const int64_t had = o.dx.slices;
+            o.dx = dx_plan(o.rows8, o.cols8, p, 1);
+            if (o.dx.slices > had) o.dx = last_piece(DxPlan{o.dx.shape, static_cast<int>(had), 0}, p);
+        }
+    }
     agk::clear_pending_error();
     char* const ws = static_cast<char*>(workspace);
     float* const weight = reinterpret_cast<float*>(ws + o.weight);
     float* const alpha = reinterpret_cast<float*>(ws + o.alpha);
     float* const acc = reinterpret_cast<float*>(ws + o.acc);
+    uint16_t* const xk = reinterpret_cast<uint16_t*>(ws + o.x);
+    uint16_t* const w3 = reinterpret_cast<uint16_t*>(ws + o.w3);
+    uint16_t* const g = reinterpret_cast<uint16_t*>(ws + o.g);
     const float2* const in = reinterpret_cast<const float2*>(stats);
-    const bool bf16 = dtype == AGK_BF16;
-    if (bf16)
-        hipLaunchKernelGGL(xent_weights<true>, dim3(1), dim3(1024), 0, st, dloss, labels, weight,
-                           alpha, rows, o.rows8, vocab);
-    else
-        hipLaunchKernelGGL(xent_weights<false>, dim3(1), dim3(1024), 0, st, dloss, labels, weight,
-                           alpha, rows, o.rows8, vocab);
-    if ((rc = check_launch()) != AGK_OK) return rc;
-    if (dw) {
-        const dim3 grid(static_cast<unsigned>(rows));
-        if (bf16)
-            hipLaunchKernelGGL(xent_keep_rows<agk::u32x4>, grid, dim3(256), 0, st,
-                               static_cast<const agk::u32x4*>(x), ldx / 8, weight,
-                               reinterpret_cast<agk::u32x4*>(ws + o.keep),
-                               static_cast<int>(cols / 8));
-        else
-            hipLaunchKernelGGL(xent_keep_rows<float>, grid, dim3(256), 0, st,
-                               static_cast<const float*>(x), ldx, weight,
-                               reinterpret_cast<float*>(ws + o.keep), static_cast<int>(cols));
-        if ((rc = check_launch()) != AGK_OK) return rc;
-    }
+    const int m = static_cast<int>(rows), m8 = static_cast<int>(o.rows8);
+    const int ldg = static_cast<int>(o.ldg), kp = static_cast<int>(o.kp);
+    const int c1 = static_cast<int>(cols), c8 = static_cast<int>(o.cols8);
     const int cus = agk_gemm::device_cus();
-    const int64_t slice = o.rows8 * cols;
-    DxPlan plan{0, 1, 0};
-    if (bf16) plan = dx_plan(o.rows8, cols, o.piece);
+    const int64_t slice = o.rows8 * o.cols8;
+    const int64_t copied = bf16 ? (dw ? rows : 0) : o.rows64;
+    const dim3 grid(1 + agk::capped_blocks((copied + 3) / 4, 1 << 20)), block(1024);
+    if (bf16)
+        hipLaunchKernelGGL(xent_tokens<true>, grid, block, 0, st, dloss, labels, weight, alpha, rows,
+                           o.rows8, vocab, x, ldx, xk, c1, kp, o.rows64);
+    else
+        hipLaunchKernelGGL(xent_tokens<false>, grid, block, 0, st, dloss, labels, weight, alpha,
+                           rows, o.rows8, vocab, x, ldx, xk, c1, kp, o.rows64);
+    if ((rc = check_launch()) != AGK_OK) return rc;
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
-        if (!bf16) {
-            float* const z = reinterpret_cast<float*>(ws + o.g);
-            const float* const wp = static_cast<const float*>(w) + v0 * ldw;
-            rc = agk_gemm_f32(wp, ldw, 0, static_cast<const float*>(x), ldx, 1, z, rows, n, rows,
-                              cols, 0, stream);
+        const int nv = static_cast<int>(n), np = static_cast<int>(bf16 ? n : up(n, 64));
+        const DxPlan d = n == o.piece ? o.dx : last_piece(o.dx, np);
+        const AddEpi<true> de{acc, c8, slice, nullptr, m8, c8, v0 > 0};
+        char* const out = static_cast<char*>(dw) + v0 * cols * dw_size;
+        if (bf16) {
+            const uint16_t* const wp = static_cast<const uint16_t*>(w) + v0 * ldw;
+            rc = launch_grad(agk_gemm::pick_shape(n, rows, cols, cus),
+                             Product{wp, ldw, static_cast<const uint16_t*>(x), ldx, nv, m, c1, 1, 0,
+                                     st},
+                             GradEpi<1>{g, in, weight, labels, v0, ldg, nv, nv, m});
             if (rc != AGK_OK) return rc;
-            hipLaunchKernelGGL(xent_piece_grad,
-                               dim3(static_cast<unsigned>((rows + 255) / 256),
-                                    static_cast<unsigned>((n + kZRows - 1) / kZRows)),
-                               dim3(256), 0, st, z, static_cast<int>(n), v0, rows, labels, in,
-                               weight);
-            if ((rc = check_launch()) != AGK_OK) return rc;
-            if (dx) {
-                rc = agk_gemm_f32(z, rows, 1, wp, ldw, 0, static_cast<float*>(dx), cols, rows,
-                                  cols, n, acc_dx || v0 > 0, stream);
-                if (rc != AGK_OK) return rc;
-            }
-            if (dw) {
-                rc = agk_gemm_f32(z, rows, 0, reinterpret_cast<const float*>(ws + o.keep), cols, 0,
-                                  static_cast<float*>(dw) + v0 * cols, cols, n, cols, rows, acc_dw,
-                                  stream);
-                if (rc != AGK_OK) return rc;
-            }
-            continue;
-        }
-        const uint16_t* const wp = static_cast<const uint16_t*>(w) + v0 * ldw;
-        uint16_t* const g = reinterpret_cast<uint16_t*>(ws + o.g);
-        const int ldg = static_cast<int>(o.ldg), m = static_cast<int>(n);
-        const Product zp{wp, ldw, static_cast<const uint16_t*>(x), ldx, m, static_cast<int>(rows),
-                         static_cast<int>(cols), 1, 0, st};
-        const GradEpi ge{g, in, weight, labels, v0, ldg, m, static_cast<int>(rows)};
-        rc = launch_grad(agk_gemm::pick_shape(n, rows, cols, cus), zp, ge);
-        if (rc != AGK_OK) return rc;
-        if (dx) {
-            DxPlan d = plan;
-            if (n != o.piece) d = last_piece(plan, n);
-            const int m8 = static_cast<int>(o.rows8);
-            const Product dp{g, ldg, wp, ldw, m8, static_cast<int>(cols), m, d.slices, d.k_slice,
-                             st};
-            const AddEpi<true> de{acc, cols, slice, nullptr, m8, static_cast<int>(cols), v0 > 0};
-            if ((rc = launch_dx(d.shape, dp, de)) != AGK_OK) return rc;
-        }
-        if (dw) {
-            const Product wpd{g, ldg, reinterpret_cast<const uint16_t*>(ws + o.keep), cols, m,
-                              static_cast<int>(cols), static_cast<int>(rows), 1, 0, st};
+            if (dx)
+                rc = launch_dx(d.shape,
+                               Product{g, ldg, wp, ldw, m8, c1, nv, d.slices, d.k_slice, st}, de);
+            if (rc != AGK_OK) return rc;
+            const Product wt{g, ldg, xk, cols, nv, c1, m, 1, 0, st};
             const int shape = agk_gemm::pick_shape(n, cols, rows, cus);
-            char* const out = static_cast<char*>(dw) + v0 * cols * dw_size;
-            if (dw_dtype == AGK_F32)
-                rc = launch_dw(shape, wpd, AddEpi<true>{out, cols, 0, alpha, m,
-                                                        static_cast<int>(cols), acc_dw});
-            else
-                rc = launch_dw(shape, wpd, AddEpi<false>{out, cols, 0, alpha, m,
-                                                         static_cast<int>(cols), acc_dw});
+            if (dw && dw_dtype == AGK_F32)
+                rc = launch_dw(shape, wt, AddEpi<true>{out, cols, 0, alpha, nv, c1, acc_dw});
+            else if (dw)
+                rc = launch_dw(shape, wt, AddEpi<false>{out, cols, 0, alpha, nv, c1, acc_dw});
+        } else {
+            rc = launch_split(static_cast<const float*>(w) + v0 * ldw, ldw, n, np, cols, kp, w3, st);
             if (rc != AGK_OK) return rc;
+            rc = launch_grad(agk_gemm::pick_shape(np, rows, kp, cus),
+                             Product{w3, 3 * o.kp, xk, 3 * o.kp, np, m, kp, 1, 0, st},
+                             GradEpi<3>{g, in, weight, labels, v0, ldg, nv, np, m},
+                             PlanesK{kp * 2, kp * 2, 0});
+            if (rc != AGK_OK) return rc;
+            if (dx)
+                rc = launch_dx(d.shape,
+                               Product{g, 3 * o.ldg, w3, 3 * o.kp, m8, c8, np, d.slices, d.k_slice,
+                                       st},
+                               de, PlanesK{ldg * 2, kp * 2, 0});
+            if (rc != AGK_OK) return rc;
+            if (dw)
+                rc = launch_dw(agk_gemm::pick_shape(np, c8, ldg, cus),
+                               Product{g, 3 * o.ldg, xk, 3 * o.kp, np, c8, ldg, 1, 0, st},
+                               AddEpi<true>{out, cols, 0, nullptr, nv, c1, acc_dw},
+                               PlanesK{ldg * 2, kp * 2, 0});
         }
+        if (rc != AGK_OK) return rc;
     }
-    if (bf16 && dx) {
-        const int64_t n8 = rows * cols / 8;
-        hipLaunchKernelGGL(xent_dx_out, dim3(static_cast<unsigned>((n8 + 255) / 256)), dim3(256), 0,
-                           st, acc, plan.slices, slice, alpha, weight, static_cast<uint16_t*>(dx), n8,
-                           static_cast<int>(cols / 8), acc_dx);
-        return check_launch();
-    }
-    return AGK_OK;
+    if (!dx) return AGK_OK;
+    const int64_t lanes = rows * o.cols8 / (bf16 ? 8 : 4);
+    const dim3 out_grid(static_cast<unsigned>((lanes + 255) / 256));
+    if (bf16)
+        hipLaunchKernelGGL(xent_dx_out, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice, alpha,
+                           weight, static_cast<uint16_t*>(dx), lanes, c8 / 8, acc_dx);
+    else
+        hipLaunchKernelGGL(xent_dx_out32, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice,
+                           weight, static_cast<float*>(dx), rows, c1, c8, acc_dx);
+    return check_launch();
 }
 
 }  // extern "C"

@@ -12,5 +12,8 @@ int launch_dw(int shape, const Product& p, const AddEpi<true>& e) {
 int launch_dw(int shape, const Product& p, const AddEpi<false>& e) {
     return launch_product<false, true>(shape, p, e);
 }
+int launch_dw(int shape, const Product& p, const AddEpi<true>& e, const PlanesK& k) {
+    return launch_product<false, true>(shape, p, e, k);
+}
 
 }  // namespace agk_xent

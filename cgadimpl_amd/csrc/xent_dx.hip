@@ -8,5 +8,8 @@ namespace agk_xent {
 int launch_dx(int shape, const Product& p, const AddEpi<true>& e) {
     return launch_product<true, true>(shape, p, e);
 }
+int launch_dx(int shape, const Product& p, const AddEpi<true>& e, const PlanesK& k) {
+    return launch_product<true, true>(shape, p, e, k);
+}
 
 }  // namespace agk_xent

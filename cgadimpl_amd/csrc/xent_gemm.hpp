@@ -11,6 +11,8 @@
 // 5-step exchange over 32 lanes for every row of the tile.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_common.hpp"
 #include "gemm_direct.hpp"
 #include "gemm_ring.hpp"
@@ -20,6 +22,46 @@ namespace agk_xent {
 using agk_gemm::f32x16;
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// fp32 operands.  A value is stored as three bf16 whose sum it is to 2^-27 of it: x = a + b +
+// c, a = bf16(x), b = bf16(x - a), c = bf16(x - a - b), in three planes side by side in each
+// row.  A product of two is aa' + ab' + ba' + bb' + ac' + ca', six bf16 products summed in
+// fp32 by walking K six times over different planes; what is left out (bc', cb', cc') is
+// below 2^-25 of the product, half of what rounding it to fp32 costs.  Six bf16 matrix instructions at
+// 1250 TFLOP/s are 208 TFLOP/s of fp32; the fp32 matrix instruction gives 113-135 (of
+// 157).  Measured, MI355X: see xent.hip.
+struct PlanesK {
+    int plane_a, plane_b;  // bytes from one plane to the next
+    int n;                 // k-tiles of a plane
+    static constexpr uint32_t kOrderA = 0x201100u, kOrderB = 0x021010u;  // plane of walk s: nibble s
+
+    __device__ __forceinline__ int start(int tiles) {
+        n = tiles;
+        return 6 * tiles;
+    }
+    __device__ __forceinline__ int walk(int t) const {
+        return (t >= n) + (t >= 2 * n) + (t >= 3 * n) + (t >= 4 * n) + (t >= 5 * n);
+    }
+    __device__ __forceinline__ int a(int t, int step) const {
+        const int s = walk(t);
+        return (t - s * n) * step + static_cast<int>(kOrderA >> (4 * s) & 3u) * plane_a;
+    }
+    __device__ __forceinline__ int b(int t, int step) const {
+        const int s = walk(t);
+        return (t - s * n) * step + static_cast<int>(kOrderB >> (4 * s) & 3u) * plane_b;
+    }
+    __device__ __forceinline__ int more_a() const { return 2 * plane_a; }
+    __device__ __forceinline__ int more_b() const { return 2 * plane_b; }
+};
+// x's three planes, two neighbouring values at a time.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&plane)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        plane[i] = agk_gemm::pack_bf16(x, y);
+        x -= agk_gemm::bf16_lo(plane[i]);
+        y -= agk_gemm::bf16_hi(plane[i]);
+    }
+}
 
 // exp(x) on v_exp_f32; see fast_exp in rowops.hip for its error.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -64,6 +106,7 @@ struct LseEpi {
     float2* part;
     float* picked;
     const int64_t* labels;
+    int64_t v0;  // the first vocabulary row of the operand, which has `vocab` of them
     int vocab, tokens;
 
     template <bool INNER, int TMW, int TNW>
@@ -107,7 +150,7 @@ struct LseEpi {
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
             const bool in = col < tokens;
-            const int at = in ? label_row(labels[col], row0, TMW * 32) : -1;
+            const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
             const float2 v = inner ? reduce<true>(acc, j, 0, half)
                                    : reduce<false>(acc, j, vocab - row0, half);
             if (in && half == 0) out[col] = v;
@@ -123,25 +166,26 @@ struct LseEpi {
     }
 };
 
-// Backward: G^T, weight * (softmax - [label]), rounded to bf16: rows v0 .. of the
-// vocabulary as rows of ldg tokens, zeros in the columns from `tokens` to ldg (the
-// padding of G's rows: the product over tokens reads up to 7 of them).
+// Backward: G^T, weight * (softmax - [label]), rows v0 .. of the vocabulary as rows of ldg
+// tokens, zeros in the columns from `tokens` to ldg (the padding of G's rows) and in the rows
+// from `rows` to padded_rows: what the products that follow read of them.  PLANES = 1: rounded
+// to bf16; 3: G's three planes, ldg apart.
 //
-// One fma, one exponential and one product per logit; exp(z - m - l) takes m + l rounded once
-// (2^-24 of its size: far below G's rounding to bf16).  Lanes c and c + 1 exchange rows e
+// One fma, one exponential and one product per logit.  Lanes c and c + 1 exchange rows e
 // and e + 1, so that a store is 4 bytes of two neighbouring tokens.
+template <int PLANES>
 struct GradEpi {
     uint16_t* G;
     const float2* stats;
     const float* weight;  // 0: a token that is left out
     const int64_t* labels;
     int64_t v0;
-    int ldg, rows, tokens;
+    int ldg, rows, padded_rows, tokens;
 
     template <int TMW, int TNW>
     __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
                                                int lane) const {
-        if (row0 >= rows) return;
+        if (row0 >= padded_rows) return;
         const int half = lane >> 5, odd = lane & 1;
         const bool inner = row0 + TMW * 32 <= rows;
         // even lanes: {own low, neighbour's low}; odd lanes: {neighbour's high, own high}
@@ -155,9 +199,13 @@ struct GradEpi {
             const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
             const bool hit = __any(at >= 0);
             const bool some_out = __any(w == 0.0f);
-            const float shift = (st.x + st.y) * kLog2e;
+            // bf16: exp(z - (m + l)), m + l rounded once (2^-24 of its size: far below G's
+            // rounding); fp32: the difference z - m first
+            const float m = PLANES == 1 ? 0.0f : st.x;
+            const float shift = (PLANES == 1 ? st.x + st.y : st.y) * kLog2e;
             const bool store = col < ldg;  // ldg is even: a pair is in or out
-            uint16_t* const out = G + (col & ~1) + static_cast<int64_t>(row0 + odd) * ldg;
+            uint16_t* const out =
+                G + (col & ~1) + static_cast<int64_t>(row0 + odd) * (PLANES * ldg);
 #pragma unroll
             for (int i = 0; i < TMW; ++i)
 #pragma unroll
@@ -166,18 +214,25 @@ struct GradEpi {
                     float g[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        float p = __builtin_amdgcn_exp2f(
-                            __builtin_fmaf(acc[i][j][e + u], kLog2e, -shift));
+                        const float z = PLANES == 1 ? acc[i][j][e + u] : acc[i][j][e + u] - m;
+                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -shift));
                         if (hit) p -= at == r + u ? 1.0f : 0.0f;
                         g[u] = w * p;
                         if (some_out) g[u] = w != 0.0f ? g[u] : 0.0f;  // z may be NaN there
+                        if (!inner) g[u] = row0 + r + u < rows ? g[u] : 0.0f;
                     }
-                    const uint32_t own = agk_gemm::pack_bf16(g[0], g[1]);
-                    const uint32_t other = static_cast<uint32_t>(
-                        __builtin_amdgcn_mov_dpp(static_cast<int>(own), 0xb1, 0xf, 0xf, true));
-                    const uint32_t v = __builtin_amdgcn_perm(own, other, pick);
-                    if (store && (inner || row0 + r + odd < rows))
-                        *reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(r) * ldg) = v;
+                    uint32_t own[3];
+                    if constexpr (PLANES == 1) own[0] = agk_gemm::pack_bf16(g[0], g[1]);
+                    else split3(g[0], g[1], own);
+#pragma unroll
+                    for (int q = 0; q < PLANES; ++q) {
+                        const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(
+                            static_cast<int>(own[q]), 0xb1, 0xf, 0xf, true));
+                        const uint32_t v = __builtin_amdgcn_perm(own[q], other, pick);
+                        if (store && (inner || row0 + r + odd < padded_rows))
+                            *reinterpret_cast<uint32_t*>(
+                                out + static_cast<int64_t>(r) * (PLANES * ldg) + q * ldg) = v;
+                    }
                 }
         }
     }
@@ -251,11 +306,16 @@ struct Product {
     hipStream_t st;
 };
 
+// bf16 operands, and fp32 ones as planes (ldX: three planes' worth).
 int launch_lse(int shape, const Product& p, const LseEpi& e);
-int launch_grad(int shape, const Product& p, const GradEpi& e);
+int launch_lse(int shape, const Product& p, const LseEpi& e, const PlanesK& k);
+int launch_grad(int shape, const Product& p, const GradEpi<1>& e);
+int launch_grad(int shape, const Product& p, const GradEpi<3>& e, const PlanesK& k);
 int launch_dx(int shape, const Product& p, const AddEpi<true>& e);
+int launch_dx(int shape, const Product& p, const AddEpi<true>& e, const PlanesK& k);
 int launch_dw(int shape, const Product& p, const AddEpi<true>& e);
 int launch_dw(int shape, const Product& p, const AddEpi<false>& e);
+int launch_dw(int shape, const Product& p, const AddEpi<true>& e, const PlanesK& k);
 
 }  // namespace agk_xent
 
@@ -276,49 +336,54 @@ __device__ __forceinline__ int slice_of(const uint16_t* __restrict__& A, int64_t
     return blockIdx.y + 1 < gridDim.y ? k_slice : K - k0;
 }
 
-template <bool A_TR, bool B_TR, bool TAIL, class Epi>
+template <bool A_TR, bool B_TR, bool TAIL, class Epi, class KM>
 __global__ __launch_bounds__(agk_gemm::kDirectThreads) void xent_direct_kernel(
     const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
-    int N, int K, int k_slice, const Epi epi, int tiles_m, int tiles_n, int full_tiles) {
+    int N, int K, int k_slice, const Epi epi, const KM km, int tiles_m, int tiles_n, int full_tiles) {
     __shared__ __attribute__((aligned(16))) uint16_t st0[agk_gemm::kStageElems];
     __shared__ __attribute__((aligned(16))) uint16_t st1[agk_gemm::kStageElems];
     const int k = slice_of<A_TR, B_TR>(A, lda, B, ldb, K, k_slice);
     agk_gemm::direct_body<A_TR, B_TR, TAIL>(A, lda, B, ldb, M, N, k, tiles_m, tiles_n,
-                                            agk_gemm::kGroupM, full_tiles, st0, st1, epi);
+                                            agk_gemm::kGroupM, full_tiles, st0, st1, epi, km);
 }
 
-template <bool A_TR, bool B_TR, class SH, class Epi>
+template <bool A_TR, bool B_TR, class SH, class Epi, class KM>
 __global__ __launch_bounds__(256, SH::kPerCu) void xent_ring_kernel(
     const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
-    int N, int K, int k_slice, const Epi epi, int tiles_m, int tiles_n) {
+    int N, int K, int k_slice, const Epi epi, const KM km, int tiles_m, int tiles_n) {
     const int k = slice_of<A_TR, B_TR>(A, lda, B, ldb, K, k_slice);
     agk_gemm::ring_body<A_TR, B_TR, SH>(A, lda, B, ldb, M, N, k, tiles_m, tiles_n,
-                                        agk_gemm::kGroupM, epi);
+                                        agk_gemm::kGroupM, epi, km);
 }
 
-template <bool A_TR, bool B_TR, class Epi>
-int launch_product(int shape, const Product& p, const Epi& e) {
+template <bool A_TR, bool B_TR, class Epi, class KM = agk_gemm::LinearK>
+int launch_product(int shape, const Product& p, const Epi& e, const KM& km = {}) {
     using namespace agk_gemm;
     if (shape == 0) {
         const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
         const int tiles = tiles_m * tiles_n;
         const int full = p.slices > 1 ? tiles : direct_full_tiles(tiles, device_cus());
         const dim3 grid(full + 2 * (tiles - full), p.slices), block(kDirectThreads);
-        if (p.K % BK != 0)
-            hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, true, Epi>), grid, block, 0, p.st,
-                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, tiles_m, tiles_n, full);
-        else
-            hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, false, Epi>), grid, block, 0, p.st,
-                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, tiles_m, tiles_n, full);
+#define AGK_XENT_DIRECT(TAIL)                                                                    \
+    hipLaunchKernelGGL((xent_direct_kernel<A_TR, B_TR, TAIL, Epi, KM>), grid, block, 0, p.st,    \
+                       p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, km, tiles_m, tiles_n, \
+                       full)
+        if constexpr (std::is_same<KM, LinearK>::value) {  // planes have no K tail
+            if (p.K % BK != 0) AGK_XENT_DIRECT(true);
+            else AGK_XENT_DIRECT(false);
+        } else {
+            AGK_XENT_DIRECT(false);
+        }
+#undef AGK_XENT_DIRECT
         return agk::check_launch();
     }
 #define AGK_XENT_CASE(ID, BM_, BN_, WVM, NST)                                                    \
     case ID: {                                                                                   \
         using SH = RingShape<BM_, BN_, WVM, NST>;                                                \
         const int tiles_m = (p.M + BM_ - 1) / BM_, tiles_n = (p.N + BN_ - 1) / BN_;              \
-        hipLaunchKernelGGL((xent_ring_kernel<A_TR, B_TR, SH, Epi>),                              \
+        hipLaunchKernelGGL((xent_ring_kernel<A_TR, B_TR, SH, Epi, KM>),                          \
                            dim3(tiles_m * tiles_n, p.slices), dim3(256), 0, p.st, p.A, p.lda,    \
-                           p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, tiles_m, tiles_n);           \
+                           p.B, p.ldb, p.M, p.N, p.K, p.k_slice, e, km, tiles_m, tiles_n);       \
         break;                                                                                   \
     }
     switch (shape) { AGK_RING_SHAPES(AGK_XENT_CASE) }

@@ -5,8 +5,11 @@
 
 namespace agk_xent {
 
-int launch_grad(int shape, const Product& p, const GradEpi& e) {
+int launch_grad(int shape, const Product& p, const GradEpi<1>& e) {
     return launch_product<false, false>(shape, p, e);
+}
+int launch_grad(int shape, const Product& p, const GradEpi<3>& e, const PlanesK& k) {
+    return launch_product<false, false>(shape, p, e, k);
 }
 
 }  // namespace agk_xent

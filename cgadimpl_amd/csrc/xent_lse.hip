@@ -8,5 +8,8 @@ namespace agk_xent {
 int launch_lse(int shape, const Product& p, const LseEpi& e) {
     return launch_product<false, false>(shape, p, e);
 }
+int launch_lse(int shape, const Product& p, const LseEpi& e, const PlanesK& k) {
+    return launch_product<false, false>(shape, p, e, k);
+}
 
 }  // namespace agk_xent

@@ -89,12 +89,12 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
  * stats [rows][2] fp32, 8-byte aligned, receives max(z) and
  * log(sum(exp((z - max) / T))), for the backward.
  * 0 <= k <= AGK_DISTILL_MAX_K (AGK_EINVAL); any alignment and cols.
- * workspace: agk_distill_topk_workspace_bytes bytes (rows spread over several
- * workgroups), 8-byte aligned, scratch; NULL where that is 0.  Calls that share
+ * workspace: agk_distill_topk_workspace_bytes bytes (a few wide rows are spread
+ * over several workgroups each), 8-byte aligned, scratch; NULL where that is 0.  Calls that share
  * one must not overlap in time.
  * rows == 0 is a no-op; cols == 0 with rows > 0 is AGK_EINVAL.               */
 #define AGK_DISTILL_MAX_K 1024
-size_t agk_distill_topk_workspace_bytes(int64_t rows, int64_t cols);
+size_t agk_distill_topk_workspace_bytes(int64_t rows, int64_t cols, int dtype);
 
 int agk_distill_topk_fwd(const void* z, const int64_t* index, const void* t, float* loss,
                          float* stats, void* workspace, size_t workspace_bytes, int64_t rows,

@@ -82,7 +82,7 @@ def run(z, index, t, dloss, T, **kw):
 
 
 SIZES = [(1, 1, 1), (1, 1000, 8), (2, 7, 3), (3, 130, 5), (33, 32001, 64), (2100, 515, 7),
-         (5, 131072, 1024), (9, 2049, 256), (300, 4096, 20), (4, 50257, 257), (40, 8, 300)]
+         (5, 131072, 1024), (3, 300001, 70), (9, 2049, 256), (300, 4096, 20), (4, 50257, 257), (40, 8, 300)]
 
 
 @pytest.mark.parametrize("dtype", [F, BF])
@@ -218,7 +218,7 @@ def test_empty_and_refusals(cuda):
         agk.distill_topk_bwd(wide[:4], index, t, stats, dloss, dz=wide[2:6])
 
 
-@pytest.mark.parametrize("rows,cols", [(40, 9000), (2100, 300)])
+@pytest.mark.parametrize("rows,cols", [(40, 9000), (2100, 300), (4, 270001)])
 def test_graph_and_streams(cuda, rows, cols):
     z, index, t, dloss = inputs(rows, cols, 12, BF)
 

@@ -148,16 +148,17 @@ def test_distill_validation():
         assert call(rows=0, z=None) == OK
         assert call(rows=0, cols=0) == OK
     assert fwd(loss=None) == EINVAL
-    need = lib.agk_distill_topk_workspace_bytes(4, 100000)
+    need = lib.agk_distill_topk_workspace_bytes(4, 1000000, F32)
     assert need > 0
-    assert fwd(cols=100000, ws=None) == EWORKSPACE
-    assert fwd(cols=100000, ws_bytes=need - 1) == EWORKSPACE
-    assert fwd(cols=100000, ws=FAKE + 4) == EINVAL
+    assert fwd(cols=1000000, ws=None) == EWORKSPACE
+    assert fwd(cols=1000000, ws_bytes=need - 1) == EWORKSPACE
+    assert fwd(cols=1000000, ws=FAKE + 4) == EINVAL
     assert bwd(dloss=None) == EINVAL and bwd(dz=None) == EINVAL
     assert bwd(acc=2) == EINVAL
     assert bwd(dz=FAKE + 16) == EINVAL               # overlaps z without being it
     ws = lib.agk_distill_topk_workspace_bytes
-    assert ws(0, 100) == 0 and ws(100, 0) == 0 and ws(100000, 50000) == 0
+    assert ws(0, 100, F32) == 0 and ws(100, 0, F32) == 0 and ws(100, 100, 2) == 0
+    assert ws(100000, 500000, F32) == 0 and ws(4, 100000, BF16) == 0 and ws(4, 100000, F32) > 0
     assert agk.AGK_DISTILL_MAX_K == 1024 and agk.AGK_ACCUM_DBETA == 4
 
 
