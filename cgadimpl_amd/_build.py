@@ -8,7 +8,8 @@ Outputs (in-tree, git-ignored, shipped with the source tree):
   cgadimpl_amd/lib/libagk_synth.so     seeded synthetic input generator (host)
   cgadimpl_amd/lib/libag.so            the C++ graph layer (ag::Value, rms, rms_norm,
                                        mul, backward) over the C ABI (host C++)
-  cgadimpl_amd/lib/test_ag_layer       its GPU test program (tests/cpp/)
+  cgadimpl_amd/lib/test_ag_layer       its GPU test programs (tests/cpp/)
+  cgadimpl_amd/lib/test_ag_losses
   cgadimpl_amd/lib/rmsnorm_layer       the RMSNorm layer benchmark through the graph layer
                                        (cgadimpl_amd/ag/bench/rmsnorm_layer.cpp)
 
@@ -150,6 +151,9 @@ def build_sanitized(out_dir: str, verbose: bool = True) -> list[str]:
         outs.append(ag_program("test_ag_layer", os.path.join(ROOT, "tests", "cpp",
                                                              "test_ag_layer.cpp"),
                                clang, [*SAN_HOST_FLAGS, "-g"]))
+        outs.append(ag_program("test_ag_losses", os.path.join(ROOT, "tests", "cpp",
+                                                              "test_ag_losses.cpp"),
+                               clang, [*SAN_HOST_FLAGS, "-g"]))
         outs.append(ag_program("rmsnorm_layer", os.path.join(AG_DIR, "bench",
                                                              "rmsnorm_layer.cpp"),
                                clang, [*SAN_HOST_FLAGS, "-g"]))
@@ -176,6 +180,8 @@ def build_all(verbose: bool = True) -> list[str]:
     outs.append(ag_library())
     outs.append(ag_program("test_ag_layer", os.path.join(ROOT, "tests", "cpp",
                                                          "test_ag_layer.cpp")))
+    outs.append(ag_program("test_ag_losses", os.path.join(ROOT, "tests", "cpp",
+                                                          "test_ag_losses.cpp")))
     outs.append(ag_program("rmsnorm_layer", os.path.join(AG_DIR, "bench", "rmsnorm_layer.cpp")))
     if verbose:
         for o in outs:

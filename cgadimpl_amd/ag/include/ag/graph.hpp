@@ -80,6 +80,8 @@ struct Node : std::enable_shared_from_this<Node> {
     Op op = Op::Leaf;
     bool is_leaf = false;
     float eps = 0.0f;  // RMSNorm / RMSNormAffine: the eps of the forward pass
+    Indices index;             // LinearCrossEntropy: labels; DistillTopK: the teacher's columns
+    float temperature = 1.0f;  // DistillTopK
     // Value(float): the literal's value, so an op can take it in another dtype
     bool is_scalar_literal = false;
     float literal_value = 0.0f;

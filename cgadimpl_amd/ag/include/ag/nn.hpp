@@ -1,10 +1,10 @@
-// nn.hpp -- the RMSNorm layer as a module.
+// nn.hpp -- the RMSNorm and LayerNorm layers as modules.
 //
 // The reference has nn::Module / nn::Linear (cgadimpl/include/nn/nn.hpp:9-54)
 // but no RMSNorm module, and its benchmark's RMSNormLayer is an empty stub
 // (Benchmark/RMSNormLayer.cpp:1-5).  This is the layer those would define:
 // a learned per-channel gain gamma (initialised to ones) applied with the
-// fused rms_norm op.
+// fused rms_norm op.  LayerNorm is the same for layer_norm (gamma ones, beta zeros).
 #pragma once
 
 #include <vector>
@@ -28,6 +28,16 @@ class RMSNorm : public Module {
     std::vector<Value> parameters() override { return {gamma}; }
 
     Value gamma;
+    float eps;
+};
+
+class LayerNorm : public Module {
+  public:
+    explicit LayerNorm(int64_t dim, float eps = 1e-5f, Dtype dt = Dtype::Float32);
+    Value operator()(const Value& x) const;
+    std::vector<Value> parameters() override { return {gamma, beta}; }
+
+    Value gamma, beta;
     float eps;
 };
 

@@ -7,7 +7,7 @@
 // include/agk_rmsnorm.h, plus the fused layer rms_norm(x, gamma, eps), one node
 // whose forward and backward are one kernel call each.  matmul, laynor,
 // softmax_row and logsumexp_row (ops.hpp:62,78,96-97) run on the GEMM and the
-// row kernels of include/agk_rowops.h.
+// row kernels of include/agk_rowops.h, the losses on those of include/agk_losses.h.
 #pragma once
 
 #include <memory>
@@ -60,6 +60,25 @@ Value softmax_row(const Value& z);
 // Row log-sum-exp over the last axis, [..., D] -> [..., 1] (reduction.cpp:54-66).
 Value logsumexp_row(const Value& z);
 
+// LayerNorm with weight and bias: (x - mean) / sqrt(var + eps) * gamma + beta, gamma and
+// beta of shape [D] or [1, D] and x's dtype.  One kernel call forward, one pass and a
+// column reduction backward.  Their gradients are fp32.  Tape: {mean, rstd}.
+Value layer_norm(const Value& x, const Value& gamma, const Value& beta, float eps = 1e-5f);
+
+// The softmax cross entropy of x w^T against labels, per row: x [..., D], w [V, D] (a linear
+// layer's layout, x's dtype), labels [...], to an fp32 loss [..., 1].  The logits are never
+// in memory whole (include/agk_losses.h).  A negative label is a row without a loss or
+// gradient; one of V or more gives a NaN.  x's gradient has its dtype, w's is fp32.
+// Weights of the rows (1/n for a mean) go into backward's seed, or a mul of the loss.
+// bfloat16: D a multiple of 8.
+Value linear_cross_entropy(const Value& x, const Value& w, const Indices& labels);
+
+// T^2 KL(p || q) per row, q = softmax(z / T) over z [..., V], p = softmax(teacher / T) over the
+// row's k columns index [..., k] (a negative one is an empty entry), teacher [..., k] fp32 or
+// bf16: the student's distance from the teacher's top logits, fp32 [..., 1].
+Value distill_topk(const Value& z, const Indices& index, const Tensor& teacher,
+                   float temperature = 1.0f);
+
 namespace detail {
 std::shared_ptr<Node> rms_nodeops(const std::shared_ptr<Node>& x);
 std::shared_ptr<Node> rms_norm_nodeops(const std::shared_ptr<Node>& x,
@@ -74,6 +93,14 @@ std::shared_ptr<Node> linear_nodeops(const std::shared_ptr<Node>& x,
 std::shared_ptr<Node> laynor_nodeops(const std::shared_ptr<Node>& x);
 std::shared_ptr<Node> softmax_row_nodeops(const std::shared_ptr<Node>& z);
 std::shared_ptr<Node> logsumexp_row_nodeops(const std::shared_ptr<Node>& z);
+std::shared_ptr<Node> layer_norm_nodeops(const std::shared_ptr<Node>& x,
+                                         const std::shared_ptr<Node>& gamma,
+                                         const std::shared_ptr<Node>& beta, float eps);
+std::shared_ptr<Node> linear_cross_entropy_nodeops(const std::shared_ptr<Node>& x,
+                                                   const std::shared_ptr<Node>& w,
+                                                   const Indices& labels);
+std::shared_ptr<Node> distill_topk_nodeops(const std::shared_ptr<Node>& z, const Indices& index,
+                                           const Tensor& teacher, float temperature);
 }  // namespace detail
 
 }  // namespace ag

@@ -186,4 +186,25 @@ class Tensor {
     std::shared_ptr<Storage> storage_;
 };
 
+// A device array of int64: the labels and column indices that a loss reads.  It
+// takes no gradient; its memory is a Storage, as a Tensor's.
+class Indices {
+  public:
+    Indices() = default;  // undefined
+    static Indices from_host(const std::vector<int64_t>& src, const std::vector<int64_t>& shape);
+    // New values in the same memory (a captured graph reads them at its next replay).
+    void set_from_host(const std::vector<int64_t>& src);
+
+    bool defined() const { return static_cast<bool>(storage_); }
+    const std::vector<int64_t>& shape() const { return shape_; }
+    int64_t numel() const;
+    const int64_t* data() const {
+        return storage_ ? static_cast<const int64_t*>(storage_->data()) : nullptr;
+    }
+
+  private:
+    std::vector<int64_t> shape_;
+    std::shared_ptr<Storage> storage_;
+};
+
 }  // namespace ag

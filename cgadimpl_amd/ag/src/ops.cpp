@@ -1,6 +1,6 @@
 // ops.cpp -- forward ops, VJP and JVP rules of the RMSNorm layer path and its
-// neighbours, on the HIP kernels behind include/agk_rmsnorm.h and
-// include/agk_rowops.h.
+// neighbours, on the HIP kernels behind include/agk_rmsnorm.h,
+// include/agk_rowops.h and include/agk_losses.h.
 //
 // Reference behaviour (paths relative to the reference tree):
 //   rms_nodeops      cgadimpl/src/ops/normalization.cpp:23-35
@@ -30,6 +30,7 @@
 
 #include "ag/autodiff.hpp"
 #include "ag/ops.hpp"
+#include "agk_losses.h"
 #include "agk_rowops.h"
 #include "check.hpp"
 
@@ -411,6 +412,119 @@ std::shared_ptr<Node> logsumexp_row_nodeops(const std::shared_ptr<Node>& z) {
     return n;
 }
 
+std::shared_ptr<Node> layer_norm_nodeops(const std::shared_ptr<Node>& x,
+                                         const std::shared_ptr<Node>& gamma,
+                                         const std::shared_ptr<Node>& beta, float eps) {
+    require_value(x, "layer_norm");
+    require_value(gamma, "layer_norm");
+    require_value(beta, "layer_norm");
+    if (x == gamma || x == beta || gamma == beta)
+        fail("layer_norm: x, gamma and beta must be different nodes");
+    const Tensor& xv = x->value;
+    const Tensor& gv = gamma->value;
+    const Tensor& bv = beta->value;
+    if (xv.dim() < 1) fail("layer_norm: input needs at least one axis");
+    if (!is_row_vector(gv, xv.cols()) || !is_row_vector(bv, xv.cols()))
+        fail("layer_norm: gamma and beta must have shape [D] or [1, D] with D = x.shape[-1]");
+    if (gv.dtype() != xv.dtype() || bv.dtype() != xv.dtype())
+        fail("layer_norm: x, gamma and beta must have the same dtype");
+    Tensor y = Tensor::empty(xv.shape(), xv.dtype());
+    auto mean = std::make_shared<Tensor>(Tensor::empty(row_stat_shape(xv), Dtype::Float32));
+    auto rstd = std::make_shared<Tensor>(Tensor::empty(row_stat_shape(xv), Dtype::Float32));
+    agk_check(agk_layernorm_affine_fwd(xv.data(), gv.data(), bv.data(), y.data(),
+                                       static_cast<float*>(mean->data()),
+                                       static_cast<float*>(rstd->data()), xv.rows(), xv.cols(), eps,
+                                       agk_dtype_of(xv.dtype()), stream_arg()),
+              "layer_norm");
+    auto n = std::make_shared<Node>(
+        y, Op::LayerNormAffine,
+        x->requires_grad() || gamma->requires_grad() || beta->requires_grad(), "layer_norm");
+    n->eps = eps;
+    n->tape.push_back(mean);
+    n->tape.push_back(rstd);
+    link_inputs(n, {x, gamma, beta});
+    return n;
+}
+
+// Device scratch of `bytes` from the pool (or the capture arena); null for none.
+static std::unique_ptr<Storage> scratch(size_t bytes) {
+    return bytes ? std::make_unique<Storage>(bytes, current_stream()) : nullptr;
+}
+
+// [..., 2] of a [..., D] tensor: the statistics a loss keeps per row.
+static std::vector<int64_t> pair_shape(const Tensor& t) {
+    std::vector<int64_t> s = t.shape();
+    s.back() = 2;
+    return s;
+}
+
+static bool same_lead(const std::vector<int64_t>& idx, const Tensor& t, size_t extra) {
+    return idx.size() + 1 == t.shape().size() + extra &&
+           std::equal(t.shape().begin(), t.shape().end() - 1, idx.begin());
+}
+
+std::shared_ptr<Node> linear_cross_entropy_nodeops(const std::shared_ptr<Node>& x,
+                                                   const std::shared_ptr<Node>& w,
+                                                   const Indices& labels) {
+    require_value(x, "linear_cross_entropy");
+    require_value(w, "linear_cross_entropy");
+    if (x == w) fail("linear_cross_entropy: x and w must be different nodes");
+    const Tensor& xv = x->value;
+    const Tensor& wv = w->value;
+    if (xv.dtype() != wv.dtype()) fail("linear_cross_entropy: x and w must have the same dtype");
+    if (wv.dim() != 2 || xv.dim() < 1 || xv.cols() != wv.shape()[1])
+        fail("linear_cross_entropy: expects x [..., D] and w [V, D]");
+    if (!labels.defined() || !same_lead(labels.shape(), xv, 0))
+        fail("linear_cross_entropy: expects one label for each row of x");
+    const int64_t rows = lead_rows(xv), V = wv.shape()[0], D = xv.cols();
+    const int dt = agk_dtype_of(xv.dtype());
+    Tensor loss = Tensor::empty(row_stat_shape(xv), Dtype::Float32);
+    auto stats = std::make_shared<Tensor>(Tensor::empty(pair_shape(xv), Dtype::Float32));
+    const size_t bytes = agk_linear_xent_fwd_workspace_bytes(rows, V, D, dt);
+    const std::unique_ptr<Storage> ws = scratch(bytes);
+    agk_check(agk_linear_xent_fwd(xv.data(), D, wv.data(), D, labels.data(),
+                                  static_cast<float*>(loss.data()),
+                                  static_cast<float*>(stats->data()), ws ? ws->data() : nullptr,
+                                  bytes, rows, V, D, dt, stream_arg()),
+              "linear_cross_entropy");
+    auto n = std::make_shared<Node>(loss, Op::LinearCrossEntropy,
+                                    x->requires_grad() || w->requires_grad(),
+                                    "linear_cross_entropy");
+    n->index = labels;
+    n->tape.push_back(stats);
+    link_inputs(n, {x, w});
+    return n;
+}
+
+std::shared_ptr<Node> distill_topk_nodeops(const std::shared_ptr<Node>& z, const Indices& index,
+                                           const Tensor& teacher, float temperature) {
+    require_value(z, "distill_topk");
+    const Tensor& zv = z->value;
+    if (zv.dim() < 1) fail("distill_topk: input needs at least one axis");
+    if (!index.defined() || !teacher.defined() || !same_lead(index.shape(), zv, 1) ||
+        index.shape() != teacher.shape())
+        fail("distill_topk: expects z [..., V], index [..., k] and teacher [..., k]");
+    const int64_t rows = lead_rows(zv), V = zv.cols(), k = index.shape().back();
+    const int dt = agk_dtype_of(zv.dtype());
+    Tensor loss = Tensor::empty(row_stat_shape(zv), Dtype::Float32);
+    auto stats = std::make_shared<Tensor>(Tensor::empty(pair_shape(zv), Dtype::Float32));
+    const size_t bytes = agk_distill_topk_workspace_bytes(rows, V, dt);
+    const std::unique_ptr<Storage> ws = scratch(bytes);
+    agk_check(agk_distill_topk_fwd(zv.data(), index.data(), teacher.data(),
+                                   static_cast<float*>(loss.data()),
+                                   static_cast<float*>(stats->data()), ws ? ws->data() : nullptr,
+                                   bytes, rows, V, k, temperature, dt,
+                                   agk_dtype_of(teacher.dtype()), stream_arg()),
+              "distill_topk");
+    auto n = std::make_shared<Node>(loss, Op::DistillTopK, z->requires_grad(), "distill_topk");
+    n->index = index;
+    n->temperature = temperature;
+    n->tape.push_back(stats);
+    n->tape.push_back(std::make_shared<Tensor>(teacher));
+    link_inputs(n, {z});
+    return n;
+}
+
 // ---- VJP rules --------------------------------------------------------------
 
 void vjp_Leaf(Node*, const Tensor&) {}
@@ -743,6 +857,96 @@ void vjp_LogSumExpRow(Node* n, const Tensor& gy) {
               "vjp_LogSumExpRow");
 }
 
+// The three gradients in one pass over the rows (agk_layernorm_affine_bwd).
+void vjp_LayerNormAffine(Node* n, const Tensor& gy) {
+    Node* X = n->inputs[0].get();
+    Node* G = n->inputs[1].get();
+    Node* B = n->inputs[2].get();
+    const bool want_x = X->requires_grad(), want_g = G->requires_grad(),
+               want_b = B->requires_grad();
+    if (!want_x && !want_g && !want_b) return;
+    check_upstream(n, gy, "vjp_LayerNormAffine");
+    const Tensor& x = X->value;
+    GradLocks lock(X, G, B);
+    int acc = AGK_ACCUM_NONE;
+    bool a = false;
+    void* dx = nullptr;
+    float *dg = nullptr, *db = nullptr;
+    if (want_x) {
+        dx = X->grad_for_write(x.dtype(), &a).data();
+        if (a) acc |= AGK_ACCUM_DX;
+    }
+    if (want_g) {
+        dg = static_cast<float*>(G->grad_for_write(Dtype::Float32, &a).data());
+        if (a) acc |= AGK_ACCUM_DGAMMA;
+    }
+    if (want_b) {
+        db = static_cast<float*>(B->grad_for_write(Dtype::Float32, &a).data());
+        if (a) acc |= AGK_ACCUM_DBETA;
+    }
+    const size_t bytes =
+        want_g || want_b ? agk_layernorm_affine_bwd_workspace_bytes(x.rows(), x.cols()) : 0;
+    const std::unique_ptr<Storage> ws = scratch(bytes);
+    agk_check(agk_layernorm_affine_bwd(x.data(), G->value.data(),
+                                       static_cast<const float*>(n->tape[0]->data()),
+                                       static_cast<const float*>(n->tape[1]->data()), gy.data(), dx,
+                                       dg, db, ws ? ws->data() : nullptr, bytes, x.rows(), x.cols(),
+                                       agk_dtype_of(x.dtype()), acc, stream_arg()),
+              "vjp_LayerNormAffine");
+}
+
+// X.grad += G W, W.grad += G^T X, G = gy (softmax - [label]), a piece of the vocabulary at a
+// time (agk_linear_xent_bwd).
+void vjp_LinearCrossEntropy(Node* n, const Tensor& gy) {
+    Node* X = n->inputs[0].get();
+    Node* W = n->inputs[1].get();
+    if (!X->requires_grad() && !W->requires_grad()) return;
+    check_upstream(n, gy, "vjp_LinearCrossEntropy");
+    const Tensor& x = X->value;
+    const Tensor& w = W->value;
+    const int64_t rows = lead_rows(x), V = w.shape()[0], D = x.cols();
+    const int dt = agk_dtype_of(x.dtype());
+    GradLocks lock(X, W);
+    int acc = AGK_ACCUM_NONE;
+    bool a = false;
+    void *dx = nullptr, *dw = nullptr;
+    if (X->requires_grad()) {
+        dx = X->grad_for_write(x.dtype(), &a).data();
+        if (a) acc |= AGK_ACCUM_DX;
+    }
+    if (W->requires_grad()) {
+        dw = W->grad_for_write(Dtype::Float32, &a).data();
+        if (a) acc |= AGK_ACCUM_DGAMMA;
+    }
+    const size_t bytes = agk_linear_xent_bwd_workspace_bytes(rows, V, D, dt, 0);
+    const std::unique_ptr<Storage> ws = scratch(bytes);
+    agk_check(agk_linear_xent_bwd(x.data(), D, w.data(), D, n->index.data(),
+                                  static_cast<const float*>(n->tape[0]->data()),
+                                  static_cast<const float*>(gy.data()), dx, dw, AGK_F32,
+                                  ws ? ws->data() : nullptr, bytes, rows, V, D, 0, dt, acc,
+                                  stream_arg()),
+              "vjp_LinearCrossEntropy");
+}
+
+// Z.grad += gy T (q - p at the teacher's columns)
+void vjp_DistillTopK(Node* n, const Tensor& gy) {
+    Node* Z = n->inputs[0].get();
+    if (!Z->requires_grad()) return;
+    check_upstream(n, gy, "vjp_DistillTopK");
+    const Tensor& z = Z->value;
+    const Tensor& teacher = *n->tape[1];
+    GradLocks lock(Z, nullptr);
+    bool acc = false;
+    Tensor& dz = Z->grad_for_write(z.dtype(), &acc);
+    agk_check(agk_distill_topk_bwd(z.data(), n->index.data(), teacher.data(),
+                                   static_cast<const float*>(n->tape[0]->data()),
+                                   static_cast<const float*>(gy.data()), dz.data(), lead_rows(z),
+                                   z.cols(), n->index.shape().back(), n->temperature,
+                                   agk_dtype_of(z.dtype()), agk_dtype_of(teacher.dtype()),
+                                   acc ? AGK_ACCUM_DX : AGK_ACCUM_NONE, stream_arg()),
+              "vjp_DistillTopK");
+}
+
 // ---- JVP rules ------------------------------------------------------------------
 // Each returns the tangent of n, or an undefined Tensor when every input
 // tangent is zero.  `tan(p)` is the tangent of input p (undefined: zero).
@@ -959,6 +1163,60 @@ Tensor jvp_LogSumExpRow(Node* n, const TangentOf& tan) {
     return out;
 }
 
+// gamma * LN'(x) tx + tgamma * xhat + tbeta, LN' symmetric: its VJP kernel applied to tx
+Tensor jvp_LayerNormAffine(Node* n, const TangentOf& tan) {
+    Node* X = n->inputs[0].get();
+    Node* G = n->inputs[1].get();
+    Node* B = n->inputs[2].get();
+    const Tensor &tx = tan(X), &tg = tan(G), &tb = tan(B);
+    if (!tx.defined() && !tg.defined() && !tb.defined()) return Tensor();
+    check_tangent(tx, X->value, "jvp_LayerNormAffine");
+    check_tangent(tg, G->value, "jvp_LayerNormAffine");
+    check_tangent(tb, B->value, "jvp_LayerNormAffine");
+    const Tensor& x = X->value;
+    const int dt = agk_dtype_of(x.dtype());
+    Tensor out = Tensor::empty(x.shape(), x.dtype());
+    bool first = true;
+    // out (+)= a * b[cols] over rows
+    auto add = [&](const Tensor& a, const Tensor& b) {
+        const int64_t as[2] = {x.rows(), a.cols()}, bs[2] = {1, x.cols()};
+        agk_check(agk_mul_bcast_fwd(a.data(), as, 2, b.data(), bs, 2, out.data(), dt, first ? 0 : 1,
+                                    stream_arg()),
+                  "jvp_LayerNormAffine");
+        first = false;
+    };
+    if (tx.defined()) {
+        Tensor t = Tensor::empty(x.shape(), x.dtype());
+        agk_check(agk_layernorm_bwd(x.data(), static_cast<const float*>(n->tape[0]->data()),
+                                    static_cast<const float*>(n->tape[1]->data()), tx.data(),
+                                    t.data(), x.rows(), x.cols(), dt, AGK_ACCUM_NONE,
+                                    stream_arg()),
+                  "jvp_LayerNormAffine");
+        add(t, G->value);
+    }
+    if (tg.defined()) {
+        Tensor xhat = Tensor::empty(x.shape(), x.dtype());
+        Tensor mean = Tensor::empty(row_stat_shape(x)), rstd = Tensor::empty(row_stat_shape(x));
+        agk_check(agk_layernorm_fwd(x.data(), xhat.data(), static_cast<float*>(mean.data()),
+                                    static_cast<float*>(rstd.data()), x.rows(), x.cols(), n->eps,
+                                    dt, stream_arg()),
+                  "jvp_LayerNormAffine");
+        add(xhat, tg);
+    }
+    if (tb.defined()) add(Tensor::full(row_stat_shape(x), 1.0f, x.dtype()), tb);
+    return out;
+}
+
+Tensor jvp_LinearCrossEntropy(Node* n, const TangentOf& tan) {
+    if (!tan(n->inputs[0].get()).defined() && !tan(n->inputs[1].get()).defined()) return Tensor();
+    fail("jvp_LinearCrossEntropy: this loss has no forward-mode rule");
+}
+
+Tensor jvp_DistillTopK(Node* n, const TangentOf& tan) {
+    if (!tan(n->inputs[0].get()).defined()) return Tensor();
+    fail("jvp_DistillTopK: this loss has no forward-mode rule");
+}
+
 }  // namespace detail
 
 Value rms(const Value& x) { return Value(detail::rms_nodeops(x.node)); }
@@ -982,5 +1240,18 @@ Value laynor(const Value& x) { return Value(detail::laynor_nodeops(x.node)); }
 Value softmax_row(const Value& z) { return Value(detail::softmax_row_nodeops(z.node)); }
 
 Value logsumexp_row(const Value& z) { return Value(detail::logsumexp_row_nodeops(z.node)); }
+
+Value layer_norm(const Value& x, const Value& gamma, const Value& beta, float eps) {
+    return Value(detail::layer_norm_nodeops(x.node, gamma.node, beta.node, eps));
+}
+
+Value linear_cross_entropy(const Value& x, const Value& w, const Indices& labels) {
+    return Value(detail::linear_cross_entropy_nodeops(x.node, w.node, labels));
+}
+
+Value distill_topk(const Value& z, const Indices& index, const Tensor& teacher,
+                   float temperature) {
+    return Value(detail::distill_topk_nodeops(z.node, index, teacher, temperature));
+}
 
 }  // namespace ag

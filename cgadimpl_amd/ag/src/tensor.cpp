@@ -442,6 +442,28 @@ Tensor Tensor::from_host_f32(const std::vector<float>& src, const std::vector<in
     return from_host(src.data(), shape, Dtype::Float32);
 }
 
+Indices Indices::from_host(const std::vector<int64_t>& src, const std::vector<int64_t>& shape) {
+    Indices x;
+    x.shape_ = shape;
+    x.storage_ = std::make_shared<Storage>(static_cast<size_t>(count(shape)) * sizeof(int64_t),
+                                           current_stream());
+    x.set_from_host(src);
+    return x;
+}
+
+void Indices::set_from_host(const std::vector<int64_t>& src) {
+    if (!defined()) fail("ag::Indices::set_from_host: undefined");
+    if (static_cast<int64_t>(src.size()) != numel())
+        fail("ag::Indices: element count does not match the shape");
+    if (src.empty()) return;
+    hip_check(hipMemcpyAsync(storage_->data(), src.data(), src.size() * sizeof(int64_t),
+                             hipMemcpyHostToDevice, current_stream()),
+              "hipMemcpyAsync H2D");
+    hip_check(hipStreamSynchronize(current_stream()), "hipStreamSynchronize");
+}
+
+int64_t Indices::numel() const { return count(shape_); }
+
 void Tensor::copy_to_host(void* dst) const {
     if (!defined()) fail("ag::Tensor::copy_to_host: undefined tensor");
     if (!nbytes()) return;
