@@ -117,10 +117,22 @@ __device__ __forceinline__ void stage_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// The 32 x 32 x 16 product of bf16 (or, F16, fp16) operands.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma16(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
 // ---- the order of K ----------------------------------------------------------------
 // Where the direct and ring kernels find k-tile t of an operand: LinearK, K once through.
-// (A product whose operands are stored as several bf16 planes brings an order of its own.)
+// (A product whose operands are stored as several planes brings an order of its own.)
 struct LinearK {
+    static constexpr bool kF16 = false;  // bf16 operands
     __device__ __forceinline__ int start(int n) { return n; }  // n whole k-tiles: the tiles in all
     __device__ __forceinline__ int a(int t, int step) const { return t * step; }  // byte offsets
     __device__ __forceinline__ int b(int t, int step) const { return t * step; }

@@ -145,13 +145,13 @@ __device__ __forceinline__ void read_frags(Frags<NB>& f, const uint16_t* stage, 
     }
 }
 
-template <int NB>
+template <bool F16, int NB>
 __device__ __forceinline__ void mfma_sub(const Frags<NB>& f, f32x16 (&acc)[TM][NB]) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = mfma16<F16>(f.a[i], f.b[j], acc[i][j]);
 }
 
 // Scheduling groups: one load, one fragment read, two MFMAs (AGK_LRM); one
@@ -190,21 +190,21 @@ __device__ __forceinline__ void direct_step(const DirectStage& d, const KM& km,
     direct_issue_a(d, other, km.a(tn, d.step_a), wave);
     read_frags<A_TR, B_TR>(f0, cur, 0, wm, bc, frow, fk, lane);
     if constexpr (!FIRST) {
-        mfma_sub(f1, acc);
+        mfma_sub<KM::kF16>(f1, acc);
         AGK_SUBSTEP_LRM
     }
     __builtin_amdgcn_sched_barrier(0);
     direct_issue_b(d, other, km.b(tn, d.step_b), wave);
     read_frags<A_TR, B_TR>(f1, cur, 1, wm, bc, frow, fk, lane);
-    mfma_sub(f0, acc);
+    mfma_sub<KM::kF16>(f0, acc);
     AGK_SUBSTEP_LRM
     __builtin_amdgcn_sched_barrier(0);
     read_frags<A_TR, B_TR>(f0, cur, 2, wm, bc, frow, fk, lane);
-    mfma_sub(f1, acc);
+    mfma_sub<KM::kF16>(f1, acc);
     AGK_SUBSTEP_RM
     __builtin_amdgcn_sched_barrier(0);
     read_frags<A_TR, B_TR>(f1, cur, 3, wm, bc, frow, fk, lane);
-    mfma_sub(f0, acc);
+    mfma_sub<KM::kF16>(f0, acc);
     AGK_SUBSTEP_RM
     __builtin_amdgcn_sched_barrier(0);
     // This wave's loads of tile t + 1 have landed and its reads of tile t are
@@ -268,7 +268,7 @@ __device__ __forceinline__ void direct_tile(const DirectStage& d, const KM& km, 
         for (int s = 0; s * 16 < K - whole * BK; ++s) {
             Frags<NB> f;
             read_frags<A_TR, B_TR>(f, st1, s, wm, bc, frow, fk, lane);
-            mfma_sub(f, acc);
+            mfma_sub<KM::kF16>(f, acc);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -287,7 +287,7 @@ __device__ __forceinline__ void direct_tile(const DirectStage& d, const KM& km, 
     if (t < nk)
         direct_step<false, A_TR, B_TR>(d, km, st1, st0, t, nk, acc, f0, f1, wm, bc, frow, fk, lane,
                                        wave);
-    mfma_sub(f1, acc);  // substep 3 of the last tile
+    mfma_sub<KM::kF16>(f1, acc);  // substep 3 of the last tile
 
     if constexpr (NB == 4) {
         // the wave's 128 x 128 block leaves as two 128 x 64 halves

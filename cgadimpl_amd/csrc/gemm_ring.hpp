@@ -178,13 +178,13 @@ __device__ __forceinline__ void ring_read(RingFrags<SH::kTm, SH::kTn>& f, const 
         f.b[j] = ring_frag<B_TR, SH::kBN>(stage + SH::kBM * BK, (wn * SH::kTn + j) * 32, s, lane);
 }
 
-template <int TMW, int TNW>
+template <bool F16, int TMW, int TNW>
 __device__ __forceinline__ void ring_mfma(const RingFrags<TMW, TNW>& f, f32x16 (&acc)[TMW][TNW]) {
 #pragma unroll
     for (int i = 0; i < TMW; ++i)
 #pragma unroll
         for (int j = 0; j < TNW; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = mfma16<F16>(f.a[i], f.b[j], acc[i][j]);
 }
 
 template <class SH>
@@ -278,34 +278,34 @@ __device__ __forceinline__ void ring_step(const RingOperands& r, const KM& km,
     ring_issue_a<SH>(r, km, o, into, ahead, wave);
     ring_read<A_TR, B_TR, SH>(f0, cur, 0, wm, wn, lane);
     if constexpr (!FIRST) {
-        ring_mfma(f1, acc);
+        ring_mfma<KM::kF16>(f1, acc);
         ring_sched<kMfma, kPer, true>();
     }
     __builtin_amdgcn_sched_barrier(0);
     ring_issue_b<SH>(r, km, o, into, ahead, wave);
     ring_read<A_TR, B_TR, SH>(f1, cur, 1, wm, wn, lane);
-    ring_mfma(f0, acc);
+    ring_mfma<KM::kF16>(f0, acc);
     ring_sched<kMfma, kPer, true>();
     __builtin_amdgcn_sched_barrier(0);
     ring_read<A_TR, B_TR, SH>(f0, cur, 2, wm, wn, lane);
-    ring_mfma(f1, acc);
+    ring_mfma<KM::kF16>(f1, acc);
     ring_sched<kMfma, kPer, false>();
     __builtin_amdgcn_sched_barrier(0);
     ring_read<A_TR, B_TR, SH>(f1, cur, 3, wm, wn, lane);
-    ring_mfma(f0, acc);
+    ring_mfma<KM::kF16>(f0, acc);
     ring_sched<kMfma, kPer, false>();
     stage_barrier<(SH::kStages - 2) * SH::kLoads>();
 }
 
 // The K % 64 tail out of `stage` (zeros past K), all four substeps.
-template <bool A_TR, bool B_TR, class SH>
+template <bool A_TR, bool B_TR, class SH, class KM>
 __device__ __forceinline__ void ring_tail(const uint16_t* stage, int k_left,
                                           f32x16 (&acc)[SH::kTm][SH::kTn], int wm, int wn,
                                           int lane) {
     for (int s = 0; s * 16 < k_left; ++s) {
         RingFrags<SH::kTm, SH::kTn> f;
         ring_read<A_TR, B_TR, SH>(f, stage, s, wm, wn, lane);
-        ring_mfma(f, acc);
+        ring_mfma<KM::kF16>(f, acc);
     }
 }
 
@@ -371,7 +371,7 @@ __device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_
     if constexpr (NST > 3) ring_issue<SH>(r, km, o, st2, 2, wave);
     if (k_left) {
         stage_barrier<(NST - 1) * SH::kLoads>();  // the tail's LDS writes, every wave
-        ring_tail<A_TR, B_TR, SH>(last, k_left, acc, wm, wn, lane);
+        ring_tail<A_TR, B_TR, SH, KM>(last, k_left, acc, wm, wn, lane);
     }
     stage_barrier<(NST - 2) * SH::kLoads>();  // tile 0 has landed; the tail's reads are done
 
@@ -408,7 +408,7 @@ __device__ __forceinline__ void ring_body(const uint16_t* __restrict__ A, int64_
             }
         }
 #undef AGK_RING
-        ring_mfma(f1, acc);  // substep 3 of the last tile
+        ring_mfma<KM::kF16>(f1, acc);  // substep 3 of the last tile
     }
     // the empty loads of the last steps still name this workgroup's LDS
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

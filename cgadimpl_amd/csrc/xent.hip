@@ -11,8 +11,9 @@
 // dx adds up in fp32 over the pieces.  8 tokens vocab cols flop a step, 2 of the forward and
 // 6 of the backward (2 of them the logits again: the price of not keeping them).
 //
-// fp32.  The same kernels on operands split into three bf16 planes (PlanesK), x once a call
-// and w a piece at a time; G leaves its kernel split.
+// fp32.  The same kernels on operands split into two fp16 planes (PlanesK), x once a call
+// and w a piece at a time, after a pass over them for their largest values; G leaves its
+// kernel split.
 //
 // A token that is left out (a negative label, or a zero dloss) has a zero row of G
 // whatever its logits are, and the product over tokens reads its row of x as zeros,
@@ -91,87 +92,184 @@ __global__ __launch_bounds__(kJoinLanes) void xent_join(
 
 // ---- the backward's weights ---------------------------------------------------------
 
-// Row `row` of an fp32 matrix (NULL: zeros) as three bf16 planes of kp values, by `lanes`
-// lanes; zeros past cols.
+// What the kernels of one call pass on in device memory.
+struct Scalars {
+    float alpha;  // the backward's weights are dloss / alpha
+    float z;      // fp32: the logits, dx and dw as factors of their products (powers of two;
+    float dx;     // dw's with alpha)
+    float dw;
+};
+
+// Largest finite |value| of `rows` rows, one wave to a row; rows are left out where keep says so.
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
-__device__ __forceinline__ void split_row(const float* __restrict__ src, int cols, int kp,
-                                          uint16_t* __restrict__ dst, int lane, int lanes) {
-    for (int c = lane * 4; c < kp; c += lanes * 4) {
+template <class Keep>
+__device__ __forceinline__ float rows_max(const float* __restrict__ src, int64_t ld, int64_t rows,
+                                          int cols, int64_t first, int64_t stride, Keep keep) {
+    const int lane = static_cast<int>(threadIdx.x & 63);
+    float m = 0.0f;
+    auto take = [&](float v) {
+        v = __builtin_fabsf(v);
+        if (v < __builtin_inff()) m = v > m ? v : m;
+    };
+    for (int64_t r = first; r < rows; r += stride) {
+        if (!keep(r)) continue;
+        const float* const p = src + r * ld;
+        int c = lane * 4;
+        for (; c + 4 <= cols; c += 256) {
+            const f32x4_a4 q = *reinterpret_cast<const f32x4_a4*>(p + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) take(q[e]);
+        }
+        for (int e = c; e < cols && e < c + 4; ++e) take(p[e]);
+    }
+    return m;
+}
+// 2^(14 - e) for a largest value of 2^e ..: the matrix's scale.
+__device__ __forceinline__ int top_exponent(float m) {
+    const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+    return m > 0.0f ? (e < -100 ? -100 : e) : 0;
+}
+__device__ __forceinline__ float pow2(int e) {
+    e = e < -126 ? -126 : e > 127 ? 127 : e;
+    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+constexpr int kMaxParts = 1024;  // workgroups of the maximum's pass, per matrix
+
+// A call's matrices: x (NULL: not in this launch) by the first x_groups workgroups, w by the rest.
+struct Matrices {
+    const float* x;
+    const float* w;
+    int64_t ldx, ldw, rows, wrows;
+    int cols, x_groups;
+    const int64_t* labels;  // NULL: every row of x; else those of tokens that are not left out
+    const float* dloss;
+    __device__ __forceinline__ bool keep(int64_t t) const {
+        return !labels || (labels[t] >= 0 && dloss[t] != 0.0f);
+    }
+};
+// parts[0 .. kMaxParts): x's maxima by workgroup, parts[kMaxParts ..): w's.
+__global__ __launch_bounds__(256) void xent_max(const Matrices a, float* __restrict__ parts) {
+    __shared__ float red[4];
+    const int g = static_cast<int>(blockIdx.x);
+    const bool is_x = g < a.x_groups;
+    const int k = is_x ? g : g - a.x_groups;
+    const int64_t groups = is_x ? a.x_groups : static_cast<int>(gridDim.x) - a.x_groups;
+    const int64_t first = static_cast<int64_t>(k) * 4 + (threadIdx.x >> 6);
+    float m = is_x ? rows_max(a.x, a.ldx, a.rows, a.cols, first, groups * 4,
+                              [&](int64_t t) { return a.keep(t); })
+                   : rows_max(a.w, a.ldw, a.wrows, a.cols, first, groups * 4,
+                              [](int64_t) { return true; });
+    for (int h = 32; h > 0; h /= 2) m = fmaxf(m, __shfl_xor(m, h));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        parts[(is_x ? 0 : kMaxParts) + k] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// Row of an fp32 matrix (NULL: zeros) times s as two fp16 planes of kp values, by one wave;
+// zeros past cols.
+__device__ __forceinline__ void split_row(const float* __restrict__ src, int cols, int kp, float s,
+                                          uint16_t* __restrict__ dst, int lane) {
+    for (int c = lane * 4; c < kp; c += 256) {
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (src && c + 4 <= cols) {
             const f32x4_a4 q = *reinterpret_cast<const f32x4_a4*>(src + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = q[e];
+            for (int e = 0; e < 4; ++e) v[e] = q[e] * s;
         } else if (src) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < cols) v[e] = src[c + e];
+                if (c + e < cols) v[e] = src[c + e] * s;
         }
-        uint32_t lo[3], hi[3];
-        split3(v[0], v[1], lo);
-        split3(v[2], v[3], hi);
+        uint32_t lo[2], hi[2];
+        split2(v[0], v[1], lo);
+        split2(v[2], v[3], hi);
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
+        for (int q = 0; q < 2; ++q)
             *reinterpret_cast<uint2*>(dst + q * kp + c) = make_uint2(lo[q], hi[q]);
     }
 }
 
-// Rows [0, rows) of src, and zeros in those up to padded: four rows per workgroup.
-__global__ __launch_bounds__(256) void xent_split(const float* __restrict__ src, int64_t ld,
-                                                  int64_t rows, int64_t padded, int cols, int kp,
-                                                  uint16_t* __restrict__ dst) {
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < padded;
-         r += static_cast<int64_t>(gridDim.x) * 4)
-        split_row(r < rows ? src + r * ld : nullptr, cols, kp, dst + r * (3 * static_cast<int64_t>(kp)),
-                  static_cast<int>(threadIdx.x & 63), 64);
+// The planes of x (rows to x_padded, zeros past the last and for tokens left out) and of w (rows
+// to w_padded), from the maxima of xent_max's x_parts and w_parts workgroups; four rows per
+// workgroup at a time.  The first workgroup leaves the products' factors.
+__global__ __launch_bounds__(256) void xent_split(const Matrices a, const float* __restrict__ parts,
+                                                  int x_parts, int w_parts, int kp,
+                                                  int64_t x_padded, int64_t w_padded,
+                                                  uint16_t* __restrict__ x2,
+                                                  uint16_t* __restrict__ w2,
+                                                  Scalars* __restrict__ sc) {
+    __shared__ float red[2][4];
+    float mx = 0.0f, mw = 0.0f;
+    for (int i = threadIdx.x; i < x_parts; i += 256) mx = fmaxf(mx, parts[i]);
+    for (int i = threadIdx.x; i < w_parts; i += 256) mw = fmaxf(mw, parts[kMaxParts + i]);
+    for (int h = 32; h > 0; h /= 2) {
+        mx = fmaxf(mx, __shfl_xor(mx, h));
+        mw = fmaxf(mw, __shfl_xor(mw, h));
+    }
+    const int wave = static_cast<int>(threadIdx.x >> 6), lane = static_cast<int>(threadIdx.x & 63);
+    if (lane == 0) {
+        red[0][wave] = mx;
+        red[1][wave] = mw;
+    }
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    mw = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+    const int ex = top_exponent(mx), ew = top_exponent(mw);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        sc->z = pow2(ex + ew - 28);
+        sc->dx = pow2(ew - 28);
+        sc->dw = sc->alpha * pow2(ex - 28);
+    }
+    const int64_t pitch = 2 * static_cast<int64_t>(kp);
+    if (static_cast<int>(blockIdx.x) < a.x_groups) {
+        for (int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + wave; t < x_padded;
+             t += static_cast<int64_t>(a.x_groups) * 4)
+            split_row(t < a.rows && a.keep(t) ? a.x + t * a.ldx : nullptr, a.cols, kp, pow2(14 - ex),
+                      x2 + t * pitch, lane);
+    } else {
+        const int64_t groups = static_cast<int>(gridDim.x) - a.x_groups;
+        for (int64_t v = (static_cast<int64_t>(blockIdx.x) - a.x_groups) * 4 + wave; v < w_padded;
+             v += groups * 4)
+            split_row(v < a.wrows ? a.w + v * a.ldw : nullptr, a.cols, kp, pow2(14 - ew),
+                      w2 + v * pitch, lane);
+    }
 }
 
-// The first workgroup: weight[t] = dloss[t] / *alpha for a token with a label, 0 for one
-// without, NaN for one whose label is past the vocabulary; zeros to padded.  *alpha: the
-// largest finite |dloss| of the tokens with a label (1 where that is 0) for bf16, 1 for fp32.
-// The others: a token's row each, x[t], or zeros for one that is left out, as the products'
-// operand: a copy of cols values (bf16), or three planes of kp (fp32; rows to padded64 of zeros).
-template <bool BF16>
+// The first workgroup: weight[t] = dloss[t] / alpha for a token with a label, 0 for one
+// without, NaN for one whose label is past the vocabulary; zeros to padded.  alpha: the
+// largest finite |dloss| of the tokens with a label (1 where that is 0).
+// The others (bf16): a token's row each, dst[t] = x[t], or zeros for one that is left out.
 __global__ __launch_bounds__(1024) void xent_tokens(const float* __restrict__ dloss,
                                                     const int64_t* __restrict__ labels,
                                                     float* __restrict__ weight,
-                                                    float* __restrict__ alpha, int64_t tokens,
+                                                    Scalars* __restrict__ sc, int64_t tokens,
                                                     int64_t padded, int64_t vocab,
-                                                    const void* __restrict__ x, int64_t ldx,
-                                                    uint16_t* __restrict__ dst, int cols, int kp,
-                                                    int64_t padded64) {
+                                                    const uint16_t* __restrict__ x, int64_t ldx,
+                                                    uint16_t* __restrict__ dst, int cols) {
     if (blockIdx.x > 0) {
-        const int lane = static_cast<int>(threadIdx.x & 255);
         for (int64_t t = (static_cast<int64_t>(blockIdx.x) - 1) * 4 + (threadIdx.x >> 8);
-             t < (BF16 ? tokens : padded64); t += (static_cast<int64_t>(gridDim.x) - 1) * 4) {
-            const bool keep = t < tokens && labels[t] >= 0 && dloss[t] != 0.0f;
-            if constexpr (BF16) {
-                const agk::u32x4* const from = reinterpret_cast<const agk::u32x4*>(
-                    static_cast<const uint16_t*>(x) + t * ldx);
-                agk::u32x4* const to = reinterpret_cast<agk::u32x4*>(dst + t * cols);
-                for (int c = lane; c < cols / 8; c += 256)
-                    to[c] = keep ? from[c] : agk::u32x4{0u, 0u, 0u, 0u};
-            } else {
-                split_row(keep ? static_cast<const float*>(x) + t * ldx : nullptr, cols, kp,
-                          dst + t * (3 * static_cast<int64_t>(kp)), lane, 256);
-            }
+             t < tokens; t += (static_cast<int64_t>(gridDim.x) - 1) * 4) {
+            const bool keep = labels[t] >= 0 && dloss[t] != 0.0f;
+            const agk::u32x4* const from = reinterpret_cast<const agk::u32x4*>(x + t * ldx);
+            agk::u32x4* const to = reinterpret_cast<agk::u32x4*>(dst + t * cols);
+            for (int c = static_cast<int>(threadIdx.x & 255); c < cols / 8; c += 256)
+                to[c] = keep ? from[c] : agk::u32x4{0u, 0u, 0u, 0u};
         }
         return;
     }
-    float c = 1.0f;
-    if constexpr (BF16) {
-        __shared__ float red[16];
-        float m = 0.0f;
-        for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
-            const float d = fabsf(dloss[t]);
-            if (labels[t] >= 0 && d < __builtin_inff()) m = fmaxf(m, d);
-        }
-        for (int h = 32; h > 0; h /= 2) m = fmaxf(m, __shfl_xor(m, h));
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-        __syncthreads();
-        for (int w = 0; w < 16; ++w) m = fmaxf(m, red[w]);
-        c = m > 0.0f ? m : 1.0f;
+    __shared__ float red[16];
+    float m = 0.0f;
+    for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
+        const float d = fabsf(dloss[t]);
+        if (labels[t] >= 0 && d < __builtin_inff()) m = fmaxf(m, d);
     }
+    for (int h = 32; h > 0; h /= 2) m = fmaxf(m, __shfl_xor(m, h));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, red[w]);
+    const float c = m > 0.0f ? m : 1.0f;
     for (int64_t t = threadIdx.x; t < padded; t += 1024) {
         float w = 0.0f;
         if (t < tokens) {
@@ -181,18 +279,18 @@ __global__ __launch_bounds__(1024) void xent_tokens(const float* __restrict__ dl
         }
         weight[t] = w;
     }
-    if (threadIdx.x == 0) *alpha = c;
+    if (threadIdx.x == 0) sc->alpha = c;
 }
 
 // dx (+)= alpha * (the K slices' sums, added in order), rounded to bf16 once.
 __global__ __launch_bounds__(256) void xent_dx_out(const float* __restrict__ acc, int slices,
-                                                   int64_t slice, const float* __restrict__ alpha,
+                                                   int64_t slice, const Scalars* __restrict__ sc,
                                                    const float* __restrict__ weight,
                                                    uint16_t* __restrict__ dx, int64_t n8, int cols8,
                                                    int accumulate) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= n8) return;
-    const float a = *alpha;
+    const float a = sc->alpha;
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < slices; s0 += 4) {  // four slices' loads before they are added
         float u[4][8];
@@ -222,9 +320,9 @@ __global__ __launch_bounds__(256) void xent_dx_out(const float* __restrict__ acc
     *out = agk::BF16::pack(v);
 }
 
-// The same for fp32: dx (+)= the slices' sums (rows of cols8), four columns per lane.
+// The same for fp32 (rows of cols8), four columns per lane.
 __global__ __launch_bounds__(256) void xent_dx_out32(const float* __restrict__ acc, int slices,
-                                                     int64_t slice,
+                                                     int64_t slice, const Scalars* __restrict__ sc,
                                                      const float* __restrict__ weight,
                                                      float* __restrict__ dx, int64_t rows, int cols,
                                                      int cols8, int accumulate) {
@@ -249,11 +347,12 @@ __global__ __launch_bounds__(256) void xent_dx_out32(const float* __restrict__ a
             }
     }
     const bool keep = weight[row] != 0.0f;
+    const float a = sc->alpha;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (c + e < cols) {
             float* const p = dx + row * cols + c + e;
-            const float g = keep ? v[e] : 0.0f;
+            const float g = keep ? v[e] * a : 0.0f;
             *p = accumulate ? agk::acc_add(*p, g) : g;
         }
 }
@@ -380,18 +479,20 @@ inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
 // The workspaces.  `cols` of the operands as staged: kp for planes (whole k-tiles).
 struct FwdLayout {
     int64_t kp, piece;
-    size_t picked, part, x3, w3, total;
+    size_t scalars, parts, picked, part, x2, w2, total;
 };
 inline FwdLayout fwd_layout(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
     FwdLayout o;
     const bool bf16 = dtype == AGK_BF16;
     o.kp = up(cols, 64);
-    o.piece = bf16 ? vocab : piece_rows(vocab, 64, o.kp, 3, 0);
-    o.picked = 0;
+    o.piece = bf16 ? vocab : piece_rows(vocab, 64, o.kp, 2, 0);
+    o.scalars = 0;
+    o.parts = o.scalars + region(sizeof(Scalars));
+    o.picked = o.parts + (bf16 ? 0 : region(2 * kMaxParts * 4));
     o.part = o.picked + region(rows * 4);
-    o.x3 = o.part + region(max_blocks(rows, vocab, o.piece) * rows * 8);
-    o.w3 = o.x3 + (bf16 ? 0 : region(rows * o.kp * 6));
-    o.total = o.w3 + (bf16 ? 0 : region(o.piece * o.kp * 6));
+    o.x2 = o.part + region(max_blocks(rows, vocab, o.piece) * rows * 8);
+    o.w2 = o.x2 + (bf16 ? 0 : region(rows * o.kp * 4));
+    o.total = o.w2 + (bf16 ? 0 : region(o.piece * o.kp * 4));
     return o;
 }
 
@@ -400,13 +501,13 @@ struct BwdLayout {
     int64_t piece, padded;             // vocabulary rows of a piece, and of its operands
     int64_t rows8, rows64, ldg, kp, cols8;
     DxPlan dx;
-    size_t weight, alpha, x, w3, g, acc, total;
+    size_t weight, scalars, parts, x, w2, g, acc, total;
 };
 inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t ldw, int dtype,
                             int64_t piece) {
     BwdLayout o;
     const bool bf16 = dtype == AGK_BF16;
-    o.planes = bf16 ? 1 : 3;
+    o.planes = bf16 ? 1 : 2;
     o.rows8 = up(rows, 8);
     o.rows64 = up(rows, 64);
     o.ldg = up(rows, kLine);
@@ -414,12 +515,13 @@ inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t l
     o.cols8 = up(cols, 8);
     o.piece = piece_rows(vocab, o.ldg, bf16 ? ldw : o.kp, o.planes, piece);
     o.padded = bf16 ? o.piece : up(o.piece, 64);
-    o.dx = dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : 6);
+    o.dx = dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : PlanesK::kWalks);
     o.weight = 0;
-    o.alpha = o.weight + region(o.rows8 * 4);
-    o.x = o.alpha + region(4);
-    o.w3 = o.x + region(bf16 ? rows * cols * 2 : o.rows64 * o.kp * 6);
-    o.g = o.w3 + (bf16 ? 0 : region(o.padded * o.kp * 6));
+    o.scalars = o.weight + region(o.rows8 * 4);
+    o.parts = o.scalars + region(sizeof(Scalars));
+    o.x = o.parts + (bf16 ? 0 : region(2 * kMaxParts * 4));
+    o.w2 = o.x + region(bf16 ? rows * cols * 2 : o.rows64 * o.kp * 4);
+    o.g = o.w2 + (bf16 ? 0 : region(o.padded * o.kp * 4));
     o.acc = o.g + region(o.padded * o.ldg * 2 * o.planes);
     o.total = o.acc + region(static_cast<int64_t>(o.dx.slices) * o.rows8 * o.cols8 * 4);
     return o;
@@ -440,7 +542,7 @@ inline int check_args(const void* x, int64_t ldx, const void* w, int64_t ldw, in
         if (cols % 8 || ldx % 8 || ldw % 8 || !aligned16(x) || !aligned16(w)) return AGK_EINVAL;
         if (256 * ldw > kMaxOperand || 256 * ldx > kMaxOperand) return AGK_EINVAL;
     } else if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 3u) ||
-               cols > kMaxOperand / 1024) {  // 256 rows of three planes
+               cols > kMaxOperand / 1024) {  // 256 rows of two planes
         return AGK_EINVAL;
     }
     return AGK_OK;
@@ -459,12 +561,23 @@ int launch_join(const float2* part, int64_t blocks, const float* picked, const i
     return check_launch();
 }
 
-// Launches a matrix's split: rows of three planes of kp.
-int launch_split(const float* src, int64_t ld, int64_t rows, int64_t padded, int64_t cols,
-                 int64_t kp, uint16_t* dst, hipStream_t st) {
-    const int64_t groups = std::min<int64_t>((padded + 3) / 4, 65536);
-    hipLaunchKernelGGL(xent_split, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, src, ld,
-                       rows, padded, static_cast<int>(cols), static_cast<int>(kp), dst);
+// The maxima's pass and the split of x (where a.x) and of a piece of w: rows to x_padded and
+// w_padded.  x's maxima and planes stay for the pieces after the first.
+int launch_planes(Matrices a, float* parts, int64_t kp, int64_t x_padded, int64_t w_padded,
+                  uint16_t* x2, uint16_t* w2, Scalars* sc, int* x_parts, hipStream_t st) {
+    auto groups = [](int64_t rows, int64_t most) {
+        return static_cast<int>(std::min<int64_t>((rows + 3) / 4, most));
+    };
+    a.x_groups = a.x ? groups(a.rows, kMaxParts / 4) : 0;
+    if (a.x) *x_parts = a.x_groups;
+    const int w_parts = groups(a.wrows, kMaxParts);
+    hipLaunchKernelGGL(xent_max, dim3(a.x_groups + w_parts), dim3(256), 0, st, a, parts);
+    const int rc = check_launch();
+    if (rc != AGK_OK) return rc;
+    a.x_groups = a.x ? groups(x_padded, 4096) : 0;
+    hipLaunchKernelGGL(xent_split, dim3(a.x_groups + groups(w_padded, 16384)), dim3(256), 0, st, a,
+                       parts, *x_parts, w_parts, static_cast<int>(kp), x_padded, w_padded, x2, w2,
+                       sc);
     return check_launch();
 }
 
@@ -496,31 +609,34 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     char* const ws = static_cast<char*>(workspace);
     float* const picked = reinterpret_cast<float*>(ws + o.picked);
     float2* const part = reinterpret_cast<float2*>(ws + o.part);
-    uint16_t* const x3 = reinterpret_cast<uint16_t*>(ws + o.x3);
-    uint16_t* const w3 = reinterpret_cast<uint16_t*>(ws + o.w3);
+    uint16_t* const x2 = reinterpret_cast<uint16_t*>(ws + o.x2);
+    uint16_t* const w2 = reinterpret_cast<uint16_t*>(ws + o.w2);
+    Scalars* const sc = reinterpret_cast<Scalars*>(ws + o.scalars);
     const bool bf16 = dtype == AGK_BF16;
     const int m = static_cast<int>(rows), kp = static_cast<int>(o.kp);
     int64_t blocks = 0;
-    if (!bf16 && (rc = launch_split(static_cast<const float*>(x), ldx, rows, rows, cols, kp, x3,
-                                    st)) != AGK_OK)
-        return rc;
+    int x_parts = 0;
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
+        const int nv = static_cast<int>(n);
         const int shape = lse_shape(rows, n, bf16 ? cols : o.kp);
-        const LseEpi e{part + blocks * rows, picked, labels, v0, static_cast<int>(n), m};
+        float2* const to = part + blocks * rows;
         if (bf16) {
             rc = launch_lse(shape,
                             Product{static_cast<const uint16_t*>(w), ldw,
-                                    static_cast<const uint16_t*>(x), ldx, static_cast<int>(n), m,
+                                    static_cast<const uint16_t*>(x), ldx, nv, m,
                                     static_cast<int>(cols), 1, 0, st},
-                            e);
+                            LseEpi<false>{to, picked, labels, v0, nv, m, nullptr});
         } else {
-            rc = launch_split(static_cast<const float*>(w) + v0 * ldw, ldw, n, n, cols, kp, w3, st);
+            const Matrices a{v0 ? nullptr : static_cast<const float*>(x),
+                             static_cast<const float*>(w) + v0 * ldw, ldx, ldw, rows, n,
+                             static_cast<int>(cols), 0, nullptr, nullptr};
+            rc = launch_planes(a, reinterpret_cast<float*>(ws + o.parts), kp, rows, n, x2, w2, sc,
+                               &x_parts, st);
             if (rc != AGK_OK) return rc;
-            rc = launch_lse(shape,
-                            Product{w3, 3 * o.kp, x3, 3 * o.kp, static_cast<int>(n), m, kp, 1, 0,
-                                    st},
-                            e, PlanesK{kp * 2, kp * 2, 0});
+            rc = launch_lse(shape, Product{w2, 2 * o.kp, x2, 2 * o.kp, nv, m, kp, 1, 0, st},
+                            LseEpi<true>{to, picked, labels, v0, nv, m, &sc->z},
+                            PlanesK{kp * 2, kp * 2, 0});
         }
         if (rc != AGK_OK) return rc;
         blocks += (n + lse_block(shape) - 1) / lse_block(shape);
@@ -567,7 +683,7 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const bool bf16 = dtype == AGK_BF16;
     if (dx && (reinterpret_cast<uintptr_t>(dx) & (bf16 ? 15u : 3u))) return AGK_EINVAL;
     // 31-bit offsets of the products over tokens
-    if (bf16 ? rows > kMaxOperand / ldx : up(rows, 64) > kMaxOperand / (3 * up(cols, 64)))
+    if (bf16 ? rows > kMaxOperand / ldx : up(rows, 64) > kMaxOperand / (2 * up(cols, 64)))
         return AGK_EINVAL;
     BwdLayout o = bwd_layout(rows, vocab, cols, cols, dtype, piece);
     if (!workspace || workspace_bytes < o.total) return AGK_EWORKSPACE;
@@ -584,10 +700,10 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     agk::clear_pending_error();
     char* const ws = static_cast<char*>(workspace);
     float* const weight = reinterpret_cast<float*>(ws + o.weight);
-    float* const alpha = reinterpret_cast<float*>(ws + o.alpha);
+    Scalars* const sc = reinterpret_cast<Scalars*>(ws + o.scalars);
     float* const acc = reinterpret_cast<float*>(ws + o.acc);
     uint16_t* const xk = reinterpret_cast<uint16_t*>(ws + o.x);
-    uint16_t* const w3 = reinterpret_cast<uint16_t*>(ws + o.w3);
+    uint16_t* const w2 = reinterpret_cast<uint16_t*>(ws + o.w2);
     uint16_t* const g = reinterpret_cast<uint16_t*>(ws + o.g);
     const float2* const in = reinterpret_cast<const float2*>(stats);
     const int m = static_cast<int>(rows), m8 = static_cast<int>(o.rows8);
@@ -595,27 +711,24 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const int c1 = static_cast<int>(cols), c8 = static_cast<int>(o.cols8);
     const int cus = agk_gemm::device_cus();
     const int64_t slice = o.rows8 * o.cols8;
-    const int64_t copied = bf16 ? (dw ? rows : 0) : o.rows64;
+    const int64_t copied = bf16 && dw ? rows : 0;
     const dim3 grid(1 + agk::capped_blocks((copied + 3) / 4, 1 << 20)), block(1024);
-    if (bf16)
-        hipLaunchKernelGGL(xent_tokens<true>, grid, block, 0, st, dloss, labels, weight, alpha, rows,
-                           o.rows8, vocab, x, ldx, xk, c1, kp, o.rows64);
-    else
-        hipLaunchKernelGGL(xent_tokens<false>, grid, block, 0, st, dloss, labels, weight, alpha,
-                           rows, o.rows8, vocab, x, ldx, xk, c1, kp, o.rows64);
+    hipLaunchKernelGGL(xent_tokens, grid, block, 0, st, dloss, labels, weight, sc, rows, o.rows8,
+                       vocab, static_cast<const uint16_t*>(x), ldx, xk, c1);
     if ((rc = check_launch()) != AGK_OK) return rc;
+    int x_parts = 0;
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
         const int nv = static_cast<int>(n), np = static_cast<int>(bf16 ? n : up(n, 64));
         const DxPlan d = n == o.piece ? o.dx : last_piece(o.dx, np);
-        const AddEpi<true> de{acc, c8, slice, nullptr, m8, c8, v0 > 0};
+        const AddEpi<true> de{acc, c8, slice, bf16 ? nullptr : &sc->dx, m8, c8, v0 > 0};
         char* const out = static_cast<char*>(dw) + v0 * cols * dw_size;
         if (bf16) {
             const uint16_t* const wp = static_cast<const uint16_t*>(w) + v0 * ldw;
             rc = launch_grad(agk_gemm::pick_shape(n, rows, cols, cus),
                              Product{wp, ldw, static_cast<const uint16_t*>(x), ldx, nv, m, c1, 1, 0,
                                      st},
-                             GradEpi<1>{g, in, weight, labels, v0, ldg, nv, nv, m});
+                             GradEpi<1>{g, in, weight, labels, v0, ldg, nv, nv, m, nullptr});
             if (rc != AGK_OK) return rc;
             if (dx)
                 rc = launch_dx(d.shape,
@@ -624,27 +737,31 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
             const Product wt{g, ldg, xk, cols, nv, c1, m, 1, 0, st};
             const int shape = agk_gemm::pick_shape(n, cols, rows, cus);
             if (dw && dw_dtype == AGK_F32)
-                rc = launch_dw(shape, wt, AddEpi<true>{out, cols, 0, alpha, nv, c1, acc_dw});
+                rc = launch_dw(shape, wt, AddEpi<true>{out, cols, 0, &sc->alpha, nv, c1, acc_dw});
             else if (dw)
-                rc = launch_dw(shape, wt, AddEpi<false>{out, cols, 0, alpha, nv, c1, acc_dw});
+                rc = launch_dw(shape, wt, AddEpi<false>{out, cols, 0, &sc->alpha, nv, c1, acc_dw});
         } else {
-            rc = launch_split(static_cast<const float*>(w) + v0 * ldw, ldw, n, np, cols, kp, w3, st);
+            const Matrices a{v0 ? nullptr : static_cast<const float*>(x),
+                             static_cast<const float*>(w) + v0 * ldw, ldx, ldw, rows, n, c1, 0,
+                             labels, dloss};
+            rc = launch_planes(a, reinterpret_cast<float*>(ws + o.parts), kp, o.rows64, np, xk, w2,
+                               sc, &x_parts, st);
             if (rc != AGK_OK) return rc;
             rc = launch_grad(agk_gemm::pick_shape(np, rows, kp, cus),
-                             Product{w3, 3 * o.kp, xk, 3 * o.kp, np, m, kp, 1, 0, st},
-                             GradEpi<3>{g, in, weight, labels, v0, ldg, nv, np, m},
+                             Product{w2, 2 * o.kp, xk, 2 * o.kp, np, m, kp, 1, 0, st},
+                             GradEpi<2>{g, in, weight, labels, v0, ldg, nv, np, m, &sc->z},
                              PlanesK{kp * 2, kp * 2, 0});
             if (rc != AGK_OK) return rc;
             if (dx)
                 rc = launch_dx(d.shape,
-                               Product{g, 3 * o.ldg, w3, 3 * o.kp, m8, c8, np, d.slices, d.k_slice,
+                               Product{g, 2 * o.ldg, w2, 2 * o.kp, m8, c8, np, d.slices, d.k_slice,
                                        st},
                                de, PlanesK{ldg * 2, kp * 2, 0});
             if (rc != AGK_OK) return rc;
             if (dw)
                 rc = launch_dw(agk_gemm::pick_shape(np, c8, ldg, cus),
-                               Product{g, 3 * o.ldg, xk, 3 * o.kp, np, c8, ldg, 1, 0, st},
-                               AddEpi<true>{out, cols, 0, nullptr, nv, c1, acc_dw},
+                               Product{g, 2 * o.ldg, xk, 2 * o.kp, np, c8, ldg, 1, 0, st},
+                               AddEpi<true>{out, cols, 0, &sc->dw, nv, c1, acc_dw},
                                PlanesK{ldg * 2, kp * 2, 0});
         }
         if (rc != AGK_OK) return rc;
@@ -653,10 +770,10 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const int64_t lanes = rows * o.cols8 / (bf16 ? 8 : 4);
     const dim3 out_grid(static_cast<unsigned>((lanes + 255) / 256));
     if (bf16)
-        hipLaunchKernelGGL(xent_dx_out, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice, alpha,
+        hipLaunchKernelGGL(xent_dx_out, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice, sc,
                            weight, static_cast<uint16_t*>(dx), lanes, c8 / 8, acc_dx);
     else
-        hipLaunchKernelGGL(xent_dx_out32, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice,
+        hipLaunchKernelGGL(xent_dx_out32, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice, sc,
                            weight, static_cast<float*>(dx), rows, c1, c8, acc_dx);
     return check_launch();
 }

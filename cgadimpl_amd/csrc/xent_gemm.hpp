@@ -23,44 +23,49 @@ using agk_gemm::f32x16;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// fp32 operands.  A value is stored as three bf16 whose sum it is to 2^-27 of it: x = a + b +
-// c, a = bf16(x), b = bf16(x - a), c = bf16(x - a - b), in three planes side by side in each
-// row.  A product of two is aa' + ab' + ba' + bb' + ac' + ca', six bf16 products summed in
-// fp32 by walking K six times over different planes; what is left out (bc', cb', cc') is
-// below 2^-25 of the product, half of what rounding it to fp32 costs.  Six bf16 matrix instructions at
-// 1250 TFLOP/s are 208 TFLOP/s of fp32; the fp32 matrix instruction gives 113-135 (of
-// 157).  Measured, MI355X: see xent.hip.
+// fp32 operands.  A matrix is stored scaled by a power of two that brings its largest value to
+// 2^14 .. 2^15, each value as two fp16 whose sum it is to 2^-22 of it: x = a + b, a = fp16(x), b =
+// fp16(x - a), in two planes side by side in each row.  A product of two is aa' + ab' + ba', three fp16
+// products summed in fp32 by walking K three times over different planes.  What is left out
+// (bb' and the two remainders) is at most 3 * 2^-22 of each product, 12 times an fp32 rounding
+// and of random sign: below the error of an fp32 sum of some dozens of products, and nothing
+// next to one of thousands.  Values 2^-28 of the largest and below lose relative bits
+// (fp16's smallest is 2^-24), at 2^-39 of the largest.  Three fp16 matrix instructions at 1250
+// TFLOP/s are 416 TFLOP/s of fp32; the fp32 matrix instruction gives 113-135 (of 157).  In three
+// bf16 planes (2^-25) it is six walks.  1000 tokens x 1000 x 32000, forward + backward on
+// MI355X: fp32 instruction 2.47 ms, bf16 planes 1.59, fp16 planes 0.96; relative error of dx
+// 6e-7 (fp32 products of the BLAS library: 3e-6).
 struct PlanesK {
+    static constexpr bool kF16 = true;
+    static constexpr int kWalks = 3;
     int plane_a, plane_b;  // bytes from one plane to the next
     int n;                 // k-tiles of a plane
-    static constexpr uint32_t kOrderA = 0x201100u, kOrderB = 0x021010u;  // plane of walk s: nibble s
 
     __device__ __forceinline__ int start(int tiles) {
         n = tiles;
-        return 6 * tiles;
+        return kWalks * tiles;
     }
-    __device__ __forceinline__ int walk(int t) const {
-        return (t >= n) + (t >= 2 * n) + (t >= 3 * n) + (t >= 4 * n) + (t >= 5 * n);
-    }
+    __device__ __forceinline__ int walk(int t) const { return (t >= n) + (t >= 2 * n); }
     __device__ __forceinline__ int a(int t, int step) const {
         const int s = walk(t);
-        return (t - s * n) * step + static_cast<int>(kOrderA >> (4 * s) & 3u) * plane_a;
+        return (t - s * n) * step + (s == 2 ? plane_a : 0);
     }
     __device__ __forceinline__ int b(int t, int step) const {
         const int s = walk(t);
-        return (t - s * n) * step + static_cast<int>(kOrderB >> (4 * s) & 3u) * plane_b;
+        return (t - s * n) * step + (s == 1 ? plane_b : 0);
     }
-    __device__ __forceinline__ int more_a() const { return 2 * plane_a; }
-    __device__ __forceinline__ int more_b() const { return 2 * plane_b; }
+    __device__ __forceinline__ int more_a() const { return plane_a; }
+    __device__ __forceinline__ int more_b() const { return plane_b; }
 };
-// x's three planes, two neighbouring values at a time.
-__device__ __forceinline__ void split3(float x, float y, uint32_t (&plane)[3]) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        plane[i] = agk_gemm::pack_bf16(x, y);
-        x -= agk_gemm::bf16_lo(plane[i]);
-        y -= agk_gemm::bf16_hi(plane[i]);
-    }
+constexpr float kTop = 16384.0f;  // 2^14
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// The two planes of two neighbouring (scaled) values.
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&plane)[2]) {
+    const f16x2 a = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    const f16x2 b = {static_cast<_Float16>(x - static_cast<float>(a.x)),
+                     static_cast<_Float16>(y - static_cast<float>(a.y))};
+    plane[0] = __builtin_bit_cast(uint32_t, a);
+    plane[1] = __builtin_bit_cast(uint32_t, b);
 }
 
 // exp(x) on v_exp_f32; see fast_exp in rowops.hip for its error.
@@ -101,18 +106,22 @@ __device__ __forceinline__ float max3_of(float a, float b, float c) {
 // One wave per SIMD runs this while the matrix cores wait, so it is kept short: two
 // maxima per instruction, one fma, one exponential and one addition per logit, in four
 // chains.  The fma takes z log2(e) - t, t = m log2(e) rounded; the rounding, exact as
-// another fma, goes into the sum as a factor.
+// another fma, goes into the sum as a factor.  SCALED: the accumulators are the logits over
+// *scale (a power of two).
+template <bool SCALED>
 struct LseEpi {
     float2* part;
     float* picked;
     const int64_t* labels;
     int64_t v0;  // the first vocabulary row of the operand, which has `vocab` of them
     int vocab, tokens;
+    const float* scale;
 
     template <bool INNER, int TMW, int TNW>
     __device__ __forceinline__ float2 reduce(const f32x16 (&acc)[TMW][TNW], int j, int left,
-                                             int half) const {
+                                             int half, float sc) const {
         constexpr float kNone = -__builtin_inff();
+        const float log2e = SCALED ? sc * kLog2e : kLog2e;
         // rows past the vocabulary: the smallest value, so that the sums below leave them out
         auto at = [&](int i, int e) -> float {
             if constexpr (INNER) return acc[i][j][e];
@@ -126,17 +135,17 @@ struct LseEpi {
                 m4[(e / 2) & 3] = max3_of(m4[(e / 2) & 3], at(i, e), at(i, e + 1));
         float m = max_of(max_of(m4[0], m4[1]), max_of(m4[2], m4[3]));
         m = max_of(m, other_half(m));
-        const float t = m == kNone ? 0.0f : m * kLog2e;  // no -inf - -inf
+        const float t = m == kNone ? 0.0f : m * log2e;  // no -inf - -inf
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < TMW; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                s4[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(at(i, e), kLog2e, -t));
+                s4[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(at(i, e), log2e, -t));
         float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         s += other_half(s);
-        if (m != kNone) s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -t));
-        return make_float2(m, s);
+        if (m != kNone) s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(m, log2e, -t));
+        return make_float2(SCALED ? m * sc : m, s);
     }
 
     template <int TMW, int TNW>
@@ -145,14 +154,15 @@ struct LseEpi {
         if (row0 >= vocab) return;
         const int half = lane >> 5;
         const bool inner = row0 + TMW * 32 <= vocab;
+        const float sc = SCALED ? *scale : 1.0f;
         float2* const out = part + static_cast<int64_t>(row0 / (TMW * 32)) * tokens;
 #pragma unroll
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
             const bool in = col < tokens;
             const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
-            const float2 v = inner ? reduce<true>(acc, j, 0, half)
-                                   : reduce<false>(acc, j, vocab - row0, half);
+            const float2 v = inner ? reduce<true>(acc, j, 0, half, sc)
+                                   : reduce<false>(acc, j, vocab - row0, half, sc);
             if (in && half == 0) out[col] = v;
             if (__any(at >= 0)) {
 #pragma unroll
@@ -160,7 +170,7 @@ struct LseEpi {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (at == acc_row(i, e, half) && row0 + at < vocab)
-                            picked[col] = acc[i][j][e];
+                            picked[col] = SCALED ? acc[i][j][e] * sc : acc[i][j][e];
             }
         }
     }
@@ -169,7 +179,8 @@ struct LseEpi {
 // Backward: G^T, weight * (softmax - [label]), rows v0 .. of the vocabulary as rows of ldg
 // tokens, zeros in the columns from `tokens` to ldg (the padding of G's rows) and in the rows
 // from `rows` to padded_rows: what the products that follow read of them.  PLANES = 1: rounded
-// to bf16; 3: G's three planes, ldg apart.
+// to bf16; 2: G 2^14's two fp16 planes, ldg apart, from accumulators that are the logits over
+// *scale.
 //
 // One fma, one exponential and one product per logit.  Lanes c and c + 1 exchange rows e
 // and e + 1, so that a store is 4 bytes of two neighbouring tokens.
@@ -181,6 +192,7 @@ struct GradEpi {
     const int64_t* labels;
     int64_t v0;
     int ldg, rows, padded_rows, tokens;
+    const float* scale;
 
     template <int TMW, int TNW>
     __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
@@ -190,12 +202,13 @@ struct GradEpi {
         const bool inner = row0 + TMW * 32 <= rows;
         // even lanes: {own low, neighbour's low}; odd lanes: {neighbour's high, own high}
         const uint32_t pick = odd ? 0x07060302u : 0x01000504u;
+        const float sc = PLANES == 1 ? 1.0f : *scale;
 #pragma unroll
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
             const bool in = col < tokens;
             const float2 st = in ? stats[col] : make_float2(0.0f, 0.0f);
-            const float w = in ? weight[col] : 0.0f;
+            const float w = in ? (PLANES == 1 ? weight[col] : weight[col] * kTop) : 0.0f;
             const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
             const bool hit = __any(at >= 0);
             const bool some_out = __any(w == 0.0f);
@@ -214,16 +227,17 @@ struct GradEpi {
                     float g[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const float z = PLANES == 1 ? acc[i][j][e + u] : acc[i][j][e + u] - m;
+                        const float z = PLANES == 1 ? acc[i][j][e + u]
+                                                    : __builtin_fmaf(acc[i][j][e + u], sc, -m);
                         float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -shift));
                         if (hit) p -= at == r + u ? 1.0f : 0.0f;
                         g[u] = w * p;
                         if (some_out) g[u] = w != 0.0f ? g[u] : 0.0f;  // z may be NaN there
                         if (!inner) g[u] = row0 + r + u < rows ? g[u] : 0.0f;
                     }
-                    uint32_t own[3];
+                    uint32_t own[2];
                     if constexpr (PLANES == 1) own[0] = agk_gemm::pack_bf16(g[0], g[1]);
-                    else split3(g[0], g[1], own);
+                    else split2(g[0], g[1], own);
 #pragma unroll
                     for (int q = 0; q < PLANES; ++q) {
                         const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(
@@ -306,11 +320,11 @@ struct Product {
     hipStream_t st;
 };
 
-// bf16 operands, and fp32 ones as planes (ldX: three planes' worth).
-int launch_lse(int shape, const Product& p, const LseEpi& e);
-int launch_lse(int shape, const Product& p, const LseEpi& e, const PlanesK& k);
+// bf16 operands, and fp32 ones as planes (their leading dimension: two planes' worth).
+int launch_lse(int shape, const Product& p, const LseEpi<false>& e);
+int launch_lse(int shape, const Product& p, const LseEpi<true>& e, const PlanesK& k);
 int launch_grad(int shape, const Product& p, const GradEpi<1>& e);
-int launch_grad(int shape, const Product& p, const GradEpi<3>& e, const PlanesK& k);
+int launch_grad(int shape, const Product& p, const GradEpi<2>& e, const PlanesK& k);
 int launch_dx(int shape, const Product& p, const AddEpi<true>& e);
 int launch_dx(int shape, const Product& p, const AddEpi<true>& e, const PlanesK& k);
 int launch_dw(int shape, const Product& p, const AddEpi<true>& e);

@@ -8,7 +8,7 @@ namespace agk_xent {
 int launch_grad(int shape, const Product& p, const GradEpi<1>& e) {
     return launch_product<false, false>(shape, p, e);
 }
-int launch_grad(int shape, const Product& p, const GradEpi<3>& e, const PlanesK& k) {
+int launch_grad(int shape, const Product& p, const GradEpi<2>& e, const PlanesK& k) {
     return launch_product<false, false>(shape, p, e, k);
 }
 

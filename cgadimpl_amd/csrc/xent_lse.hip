@@ -5,10 +5,10 @@
 
 namespace agk_xent {
 
-int launch_lse(int shape, const Product& p, const LseEpi& e) {
+int launch_lse(int shape, const Product& p, const LseEpi<false>& e) {
     return launch_product<false, false>(shape, p, e);
 }
-int launch_lse(int shape, const Product& p, const LseEpi& e, const PlanesK& k) {
+int launch_lse(int shape, const Product& p, const LseEpi<true>& e, const PlanesK& k) {
     return launch_product<false, false>(shape, p, e, k);
 }
 

@@ -35,7 +35,10 @@ extern "C" {
  * [rows][2] fp32, 8-byte aligned, receives m and l, which the backward reads.
  * z exists in pieces only: bf16 products leave the matrix cores as the maximum
  * and sum of exponentials of each token's logits over a few vocabulary rows, in
- * fp32 and unrounded; fp32 ones pass through a piece of the workspace.
+ * fp32 and unrounded.  fp32 operands are multiplied as two fp16 halves each (in
+ * the workspace, a piece of the vocabulary at a time), scaled by a power of two:
+ * a product is off by at most 12 * 2^-24 of itself, less than the fp32 sum of
+ * the row's products is.
  * bf16: x and w 16-byte aligned, cols, ldx and ldw multiples of 8 (as
  * agk_linear_bf16); rows and vocab are free.  fp32: any sizes.
  * workspace: agk_linear_xent_fwd_workspace_bytes bytes, 16-byte aligned,
@@ -63,6 +66,7 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
  * products, and the factor goes into their fp32 results: equal weights then
  * cost no rounding of their own.  dx is summed over the pieces in fp32 and
  * rounded once.  dx 16-byte aligned; rows * ldx at most 2^30 values (AGK_EINVAL).
+ * fp32: rows * cols, both rounded up to multiples of 64, at most 2^29.
  * Other sizes, alignments and the workspace as for the forward;
  * agk_linear_xent_bwd_workspace_bytes takes the same piece and depends on the
  * current device's compute units (few rows are spread over them).

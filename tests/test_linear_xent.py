@@ -2,8 +2,12 @@
 
 Bounds, per element (u = 2^-24: the most an fp32 rounding is off relative to the value; r: the
 storage type's, u or 2^-8 for bf16):
-- a logit, a sum of D exact (bf16) or rounded (fp32) products in fp32, is off by
-  dz <= (D + 2) u sum|x w|;
+- a logit, a sum of D products in fp32, is off by dz <= (D + 2) u sum|x w| + the products' own
+  error: none for bf16 (exact in fp32); for fp32, whose operands go in as two fp16 halves a + b,
+  scaled so that the largest value is below 2^15: |x - a| <= 2^-11 |x|, |x - a - b| <= 2^-22 |x|, so the
+  two remainders and b b', which are left out, are at most 3 * 2^-22 = 12 u of a product; and where a half
+  is below fp16's normal range its error is 2^-25 of a unit, 2^-39 of the scaled maximum's 2^14,
+  for either operand (two halves: 2^-38), against the other one's value;
 - a sum of exponentials of logits: each term relative to itself by dz + 8 u (its argument's
   rounding, the exponential's last places; |arg| exp(arg) <= 0.4 for the argument's scale) and
   the adding by the depth of the sums, at most 128 in a block, then the blocks in turn
@@ -29,6 +33,15 @@ R = {torch.float32: U, torch.bfloat16: 2.0 ** -8}
 BF, F = torch.bfloat16, torch.float32
 
 
+def products(a, b, dt):
+    """The error of a sum of products a @ b in fp32 (without the sum's own)."""
+    a, b = a.abs(), b.abs()
+    if dt == BF:
+        return 0.0
+    low = 2.0 ** -38 * (a.max() * b.sum(0, keepdim=True) + a.sum(1, keepdim=True) * b.max())
+    return 12 * U * (a @ b) + low
+
+
 def reference(x, w, labels, dloss, dw_dtype=None):
     """((loss, dx, dw), bounds) in fp64; dloss None: the loss alone."""
     dt = x.dtype
@@ -39,7 +52,7 @@ def reference(x, w, labels, dloss, dw_dtype=None):
         keep_g = keep & (dloss != 0)
     x0 = torch.where(keep[:, None], x, 0.0)
     z = x0 @ w.T
-    dz = (D + 2) * U * (x0.abs() @ w.abs().T)
+    dz = (D + 2) * U * (x0.abs() @ w.abs().T) + products(x0, w.T, dt)
     m = z.amax(1, keepdim=True)
     l = torch.log(torch.exp(z - m).sum(1, keepdim=True))
     at = labels.clamp(min=0)[:, None]
@@ -59,8 +72,9 @@ def reference(x, w, labels, dloss, dw_dtype=None):
     eG = wt.abs() * p * rel + 4 * U * G.abs() + (2.0 ** -8 * G.abs() if dt == BF else 0.0)
     dx, dw = G @ w, G.T @ x1
     pieces = 8
-    edx = eG @ w.abs() + (V + pieces + 8) * U * (G.abs() @ w.abs()) + (R[dt] + 2 * U) * dx.abs()
-    edw = eG.T @ x1.abs() + (N + 8) * U * (G.abs().T @ x1.abs()) + \
+    edx = eG @ w.abs() + (V + pieces + 8) * U * (G.abs() @ w.abs()) + products(G, w, dt) + \
+        (R[dt] + 2 * U) * dx.abs()
+    edw = eG.T @ x1.abs() + (N + 8) * U * (G.abs().T @ x1.abs()) + products(G.T, x1, dt) + \
         (R[dw_dtype or F] + 2 * U) * dw.abs()
     return (loss, dx, dw), (eloss, edx, edw)
 
