@@ -253,7 +253,9 @@ struct GradEpi {
 };
 
 // C (+)= alpha * product (alpha NULL: 1), the product rounded before it is added.  The
-// old values of a 32-row group are loaded together: one wait for 16 TNW loads.
+// old values of a 32-row group are loaded together: one wait for 16 TNW loads.  A bf16 C that
+// is not added to is stored 4 bytes at a time, as G is (ldc and N are even there): dw of 4099
+// tokens x 2048 x 50257 802 -> 739 us on MI355X, of 16 tokens x 4096 x 32000 (all stores) 74 -> 67.
 template <bool OUT_F32>
 struct AddEpi {
     void* C;
@@ -271,6 +273,30 @@ struct AddEpi {
         const float a = alpha ? *alpha : 1.0f;
         T* const c0 = static_cast<T*>(C) + static_cast<int64_t>(blockIdx.y) * slice;
         const bool inner = row0 + TMW * 32 <= M && col0 + TNW * 32 <= N;
+        if constexpr (!OUT_F32) {
+            if (!accumulate) {
+                const int odd = lane & 1, col = lane & 30;
+                const uint32_t pick = odd ? 0x07060302u : 0x01000504u;
+#pragma unroll
+                for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const int r = row0 + acc_row(i, e, half) + odd;
+                        uint16_t* const p = c0 + static_cast<int64_t>(r) * ldc + col0 + col;
+#pragma unroll
+                        for (int j = 0; j < TNW; ++j) {
+                            const uint32_t own =
+                                agk_gemm::pack_bf16(acc[i][j][e] * a, acc[i][j][e + 1] * a);
+                            const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(
+                                static_cast<int>(own), 0xb1, 0xf, 0xf, true));
+                            if (inner || (r < M && col0 + j * 32 + col < N))
+                                *reinterpret_cast<uint32_t*>(p + j * 32) =
+                                    __builtin_amdgcn_perm(own, other, pick);
+                        }
+                    }
+                return;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < TMW; ++i) {
             T* const p0 = c0 + static_cast<int64_t>(row0 + i * 32 + 4 * half) * ldc + col0 +
@@ -368,6 +394,90 @@ __global__ __launch_bounds__(256, SH::kPerCu) void xent_ring_kernel(
     const int k = slice_of<A_TR, B_TR>(A, lda, B, ldb, K, k_slice);
     agk_gemm::ring_body<A_TR, B_TR, SH>(A, lda, B, ldb, M, N, k, tiles_m, tiles_n,
                                         agk_gemm::kGroupM, epi, km);
+}
+
+// A product of few k (dw of few tokens: an outer product, whose time is its stores): all of K
+// staged at once, one barrier, no ring.  A tile's stages then take 24 KiB, or 48, instead of
+// 64-72, so that six or three workgroups share a CU, and a workgroup's loads and stores hide
+// behind the others'.  LinearK: NKT tiles of 64; PlanesK: one, in two planes.  dw in bf16, 4096 x
+// 32000 on MI355X, the shape pick_shape takes / this: 16 tokens 171 / 67 us (4.0 TB/s of stores),
+// 128 tokens 150 / 110.  A row-by-row order of the tiles changes little (62-76, 119).
+constexpr int kShortM = 64, kShortN = 128;
+
+template <bool A_TR, bool B_TR, int NKT, class Epi, class KM>
+__global__ __launch_bounds__(256, NKT == 1 ? 6 : 3) void xent_short_kernel(
+    const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
+    int N, int K, const Epi epi, const KM km, int tiles_m, int tiles_n) {
+    using namespace agk_gemm;
+    using SH = RingShape<kShortM, kShortN, 2, 3>;
+    __shared__ __attribute__((aligned(16))) uint16_t lds[NKT][SH::kElems];
+    const int lane = static_cast<int>(threadIdx.x & 63);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int wm = wave / SH::kWvn, wn = wave % SH::kWvn;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, kGroupM, tm, tn);
+    const int m0 = tm * kShortM, n0 = tn * kShortN;
+    const int rows_a = M - m0 < kShortM ? M - m0 : kShortM;
+    const int rows_b = N - n0 < kShortN ? N - n0 : kShortN;
+    const uint16_t* const a0 = A_TR ? A + m0 : A + static_cast<int64_t>(m0) * lda;
+    const uint16_t* const b0 = B_TR ? B + n0 : B + static_cast<int64_t>(n0) * ldb;
+    constexpr bool kPlanes = !std::is_same<KM, LinearK>::value;
+#pragma unroll
+    for (int t = 0; t < NKT; ++t) {
+        if (!kPlanes && t * BK >= K) break;
+        const int64_t pa = kPlanes && t ? km.more_a() / 2 : 0, pb = kPlanes && t ? km.more_b() / 2 : 0;
+        stage_k_tail<A_TR, kShortM>(lds[t], a0 + pa, lda, rows_a, kPlanes ? 0 : t * BK, K);
+        stage_k_tail<B_TR, kShortN>(lds[t] + kShortM * BK, b0 + pb, ldb, rows_b,
+                                    kPlanes ? 0 : t * BK, K);
+    }
+    f32x16 acc[SH::kTm][SH::kTn];
+#pragma unroll
+    for (int i = 0; i < SH::kTm; ++i)
+#pragma unroll
+        for (int j = 0; j < SH::kTn; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    __syncthreads();
+    // the walks' stages of A and B: {0, 0}, {0, 1}, {1, 0} for planes, {t, t} for k-tiles
+#pragma unroll
+    for (int t = 0; t < (kPlanes ? 3 : NKT); ++t) {
+        const uint16_t* const sa = lds[kPlanes ? t >> 1 : t];
+        const uint16_t* const sb = lds[kPlanes ? t & 1 : t] + kShortM * BK;
+        const int left = kPlanes ? K : K - t * BK;
+        for (int s = 0; s * 16 < left && s < BK / 16; ++s) {
+            RingFrags<SH::kTm, SH::kTn> f;
+#pragma unroll
+            for (int i = 0; i < SH::kTm; ++i)
+                f.a[i] = ring_frag<A_TR, kShortM>(sa, (wm * SH::kTm + i) * 32, s, lane);
+#pragma unroll
+            for (int j = 0; j < SH::kTn; ++j)
+                f.b[j] = ring_frag<B_TR, kShortN>(sb, (wn * SH::kTn + j) * 32, s, lane);
+            ring_mfma<KM::kF16>(f, acc);
+        }
+    }
+    epi(acc, m0 + wm * SH::kTm * 32, n0 + wn * SH::kTn * 32, lane);
+}
+
+// The most k it takes, and its launch.
+template <class KM>
+constexpr int short_k() {
+    return std::is_same<KM, agk_gemm::LinearK>::value ? 128 : 64;
+}
+template <bool A_TR, bool B_TR, class Epi, class KM = agk_gemm::LinearK>
+int launch_short(const Product& p, const Epi& e, const KM& km = {}) {
+    const int tiles_m = (p.M + kShortM - 1) / kShortM, tiles_n = (p.N + kShortN - 1) / kShortN;
+    const dim3 grid(tiles_m * tiles_n), block(256);
+    constexpr bool kPlanes = !std::is_same<KM, agk_gemm::LinearK>::value;
+    if constexpr (!kPlanes) {
+        if (p.K <= agk_gemm::BK) {
+            hipLaunchKernelGGL((xent_short_kernel<A_TR, B_TR, 1, Epi, KM>), grid, block, 0, p.st,
+                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, e, km, tiles_m, tiles_n);
+            return agk::check_launch();
+        }
+    }
+    hipLaunchKernelGGL((xent_short_kernel<A_TR, B_TR, 2, Epi, KM>), grid, block, 0, p.st, p.A,
+                       p.lda, p.B, p.ldb, p.M, p.N, p.K, e, km, tiles_m, tiles_n);
+    return agk::check_launch();
 }
 
 template <bool A_TR, bool B_TR, class Epi, class KM = agk_gemm::LinearK>
