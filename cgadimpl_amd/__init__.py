@@ -867,6 +867,12 @@ def _scratch(workspace, need, like):
     return workspace, workspace.numel() * workspace.element_size()
 
 
+def _row_column(x, rows):
+    """A float32 column of one value per row of x."""
+    shape = (rows, 1) if x.dim() == 2 else x.shape[:-1] + (1,)
+    return _empty(shape, _torch().float32, x)
+
+
 def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None,
                          stream=None):
     """y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis (gamma, beta: [cols] of
@@ -883,11 +889,11 @@ def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, r
     else:
         _want(y, "y", dev, x.numel(), x.dtype)
     if mean is None:
-        mean = _row_stat_like(x, torch.float32)
+        mean = _row_column(x, rows)
     else:
         _want(mean, "mean", dev, rows, torch.float32)
     if rstd is None:
-        rstd = _row_stat_like(x, torch.float32)
+        rstd = _row_column(x, rows)
     else:
         _want(rstd, "rstd", dev, rows, torch.float32)
     rc = lib().agk_layernorm_affine_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean),
@@ -1017,14 +1023,13 @@ def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dt
 
 def _distill_sizes(z, index, teacher):
     dev = _want_current(z)
-    if z.dim() < 1 or index.dim() != z.dim() or index.shape[:-1] != z.shape[:-1]:
-        raise ValueError("expected z [..., cols] and index [..., k]")
-    cols, k = z.shape[-1], index.shape[-1]
-    rows = z.numel() // cols if cols else index.shape[:-1].numel()
-    _want(index, "index", dev, rows * k, _torch().int64)
-    _want(teacher, "teacher", dev, rows * k, teacher.dtype)
-    if teacher.shape != index.shape:
-        raise ValueError("expected teacher [..., k]")
+    zs, shape = z.shape, index.shape
+    if len(zs) < 1 or len(shape) != len(zs) or shape[:-1] != zs[:-1] or teacher.shape != shape:
+        raise ValueError("expected z [..., cols], index [..., k] and teacher [..., k]")
+    cols, k, n = zs[-1], shape[-1], index.numel()
+    rows = z.numel() // cols if cols else zs[:-1].numel()
+    _want(index, "index", dev, n, _torch().int64)
+    _want(teacher, "teacher", dev, n, teacher.dtype)
     return dev, rows, cols, k
 
 
