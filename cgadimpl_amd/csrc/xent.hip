@@ -124,10 +124,11 @@ __device__ __forceinline__ float rows_max(const float* __restrict__ src, int64_t
     }
     return m;
 }
-// 2^(14 - e) for a largest value of 2^e ..: the matrix's scale.
+// e of a largest value of 2^e ..; the matrix's scale is 2^(14 - e), and the factor that takes a
+// product of two such matrices back, 2^(e - 28), has to be a normal number.
 __device__ __forceinline__ int top_exponent(float m) {
     const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
-    return m > 0.0f ? (e < -100 ? -100 : e) : 0;
+    return m > 0.0f ? (e < -98 ? -98 : e) : 0;
 }
 __device__ __forceinline__ float pow2(int e) {
     e = e < -126 ? -126 : e > 127 ? 127 : e;
@@ -142,10 +143,10 @@ struct Matrices {
     const float* w;
     int64_t ldx, ldw, rows, wrows;
     int cols, x_groups;
-    const int64_t* labels;  // NULL: every row of x; else those of tokens that are not left out
-    const float* dloss;
+    const int64_t* labels;  // tokens that are left out are read as zeros and have no part in
+    const float* dloss;     // the maximum; NULL in the forward
     __device__ __forceinline__ bool keep(int64_t t) const {
-        return !labels || (labels[t] >= 0 && dloss[t] != 0.0f);
+        return labels[t] >= 0 && (!dloss || dloss[t] != 0.0f);
     }
 };
 // parts[0 .. kMaxParts): x's maxima by workgroup, parts[kMaxParts ..): w's.
@@ -535,11 +536,12 @@ inline int check_args(const void* x, int64_t ldx, const void* w, int64_t ldw, in
         return AGK_EINVAL;
     // 256 x 256 tiles of all logits: one grid's worth
     if (rows > 0 && vocab > (kMaxTokens - 1) * 65536 / up(rows, 256) - 256) return AGK_EINVAL;
+    if (dtype == AGK_BF16 && cols % 8) return AGK_EINVAL;
     if (rows == 0) return AGK_OK;
     if (!x || !w || ldx < cols || ldw < cols) return AGK_EINVAL;
     if (rows > INT64_MAX / 16 / ldx || vocab > INT64_MAX / 16 / ldw) return AGK_EINVAL;
     if (dtype == AGK_BF16) {
-        if (cols % 8 || ldx % 8 || ldw % 8 || !aligned16(x) || !aligned16(w)) return AGK_EINVAL;
+        if (ldx % 8 || ldw % 8 || !aligned16(x) || !aligned16(w)) return AGK_EINVAL;
         if (256 * ldw > kMaxOperand || 256 * ldx > kMaxOperand) return AGK_EINVAL;
     } else if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 3u) ||
                cols > kMaxOperand / 1024) {  // 256 rows of two planes
@@ -598,7 +600,7 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     using namespace agk_xent;
     int rc = check_args(x, ldx, w, ldw, rows, vocab, cols, dtype);
     if (rc != AGK_OK || rows == 0) return rc;
-    if (!labels || !loss || !stats ||
+    if (!labels || !loss || !stats || (reinterpret_cast<uintptr_t>(loss) & 3u) ||
         ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(labels)) & 7u))
         return AGK_EINVAL;
     const FwdLayout o = fwd_layout(rows, vocab, cols, dtype);
@@ -630,7 +632,7 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         } else {
             const Matrices a{v0 ? nullptr : static_cast<const float*>(x),
                              static_cast<const float*>(w) + v0 * ldw, ldx, ldw, rows, n,
-                             static_cast<int>(cols), 0, nullptr, nullptr};
+                             static_cast<int>(cols), 0, labels, nullptr};
             rc = launch_planes(a, reinterpret_cast<float*>(ws + o.parts), kp, rows, n, x2, w2, sc,
                                &x_parts, st);
             if (rc != AGK_OK) return rc;
@@ -676,13 +678,14 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
                            st, static_cast<uint32_t*>(dw), n);
         return check_launch();
     }
-    if (!labels || !stats || !dloss ||
+    if (!labels || !stats || !dloss || (reinterpret_cast<uintptr_t>(dloss) & 3u) ||
         ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(labels)) & 7u))
         return AGK_EINVAL;
     if (!dx && !dw) return AGK_OK;
     const bool bf16 = dtype == AGK_BF16;
     if (dx && (reinterpret_cast<uintptr_t>(dx) & (bf16 ? 15u : 3u))) return AGK_EINVAL;
-    // 31-bit offsets of the products over tokens
+    // 31-bit offsets of the products: over tokens, and over G's smallest piece
+    if (up(rows, kLine) * (bf16 ? 1 : 2) > kMaxOperand / 256) return AGK_EINVAL;
     if (bf16 ? rows > kMaxOperand / ldx : up(rows, 64) > kMaxOperand / (2 * up(cols, 64)))
         return AGK_EINVAL;
     BwdLayout o = bwd_layout(rows, vocab, cols, cols, dtype, piece);

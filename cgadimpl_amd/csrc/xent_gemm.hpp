@@ -1,14 +1,14 @@
-// xent_gemm.hpp -- the bf16 products of the vocabulary head's loss (xent.hip): the
-// direct and ring kernels of gemm_direct.hpp / gemm_ring.hpp with epilogues that
-// take the logits while they are in registers.  One translation unit per product
-// instantiates its kernels (AGK_XENT_KERNELS and AGK_RING_KERNELS), to compile side by side.
+// xent_gemm.hpp -- the products of the vocabulary head's loss (xent.hip), of bf16 operands and
+// of fp32 ones as fp16 planes: the direct and ring kernels of gemm_direct.hpp /
+// gemm_ring.hpp with epilogues that take the logits while they are in registers, and a
+// kernel for few k.  One translation unit per product instantiates its kernels
+// (AGK_XENT_KERNELS and AGK_RING_KERNELS), to compile side by side.
 //
 // Every product has the vocabulary along M and the tokens along N where it makes or
 // takes logits (z^T = w x^T): an accumulator tile then holds, in each lane, 16
-// vocabulary rows of one token per 32 x 32 block (32 blocks' worth in the 256 x 256
-// kernel), so a token's maximum and sum of exponentials are sums within a lane and
-// one exchange between the wave's halves, where tokens along M would take a
-// 5-step exchange over 32 lanes for every row of the tile.
+// vocabulary rows of one token per 32 x 32 block, so a token's maximum and sum of
+// exponentials are sums within a lane and one exchange between the wave's halves, where
+// tokens along M would take a 5-step exchange over 32 lanes for every row of the tile.
 #pragma once
 
 #include <type_traits>
@@ -252,7 +252,7 @@ struct GradEpi {
     }
 };
 
-// C (+)= alpha * product (alpha NULL: 1), the product rounded before it is added.  The
+// C (+)= alpha * product (alpha NULL: 1), that in fp32 and rounded to C's type once.  The
 // old values of a 32-row group are loaded together: one wait for 16 TNW loads.  A bf16 C that
 // is not added to is stored 4 bytes at a time, as G is (ldc and N are even there): dw of 4099
 // tokens x 2048 x 50257 802 -> 739 us on MI355X, of 16 tokens x 4096 x 32000 (all stores) 74 -> 67.

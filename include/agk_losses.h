@@ -38,7 +38,10 @@ extern "C" {
  * fp32 and unrounded.  fp32 operands are multiplied as two fp16 halves each (in
  * the workspace, a piece of the vocabulary at a time), scaled by a power of two:
  * a product is off by at most 12 * 2^-24 of itself, less than the fp32 sum of
- * the row's products is.
+ * the row's products is.  Values below 2^-28 of their matrix's largest finite one
+ * (x's: over the rows with a label) are held to 2^-39 of that one.
+ * A logit of 2.3e38 and more makes its row's loss NaN.  The stats of a row whose
+ * label is negative hold nothing of use.
  * bf16: x and w 16-byte aligned, cols, ldx and ldw multiples of 8 (as
  * agk_linear_bf16); rows and vocab are free.  fp32: any sizes.
  * workspace: agk_linear_xent_fwd_workspace_bytes bytes, 16-byte aligned,
@@ -58,7 +61,7 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
  * with z computed again, `piece` vocabulary rows at a time (0: as many as make
  * G's piece about 512 MiB; others are rounded up to a multiple of 256).  Rows
  * whose label is negative or whose dloss is 0 are left out: dx (+)= 0 and
- * nothing in dw.
+ * nothing in dw.  dx and dw may not overlap the inputs or each other.
  * dx [rows][cols] of `dtype`; dw [vocab][cols] of dw_dtype (AGK_F32, or
  * AGK_BF16 where dtype is AGK_BF16); either may be NULL.  accumulate:
  * AGK_ACCUM_DX adds into dx, AGK_ACCUM_DGAMMA into dw.
@@ -66,7 +69,8 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
  * products, and the factor goes into their fp32 results: equal weights then
  * cost no rounding of their own.  dx is summed over the pieces in fp32 and
  * rounded once.  dx 16-byte aligned; rows * ldx at most 2^30 values (AGK_EINVAL).
- * fp32: rows * cols, both rounded up to multiples of 64, at most 2^29.
+ * fp32: rows * cols, both rounded up to multiples of 64, at most 2^29.  At most
+ * 2^22 rows, fp32 2^21.
  * Other sizes, alignments and the workspace as for the forward;
  * agk_linear_xent_bwd_workspace_bytes takes the same piece and depends on the
  * current device's compute units (few rows are spread over them).

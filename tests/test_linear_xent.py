@@ -365,3 +365,31 @@ def test_gradients_against_differences(cuda):
         want = (f(*hi) - f(*lo)) / (2 * h)
         terms = grads[i].double() * d
         assert abs(terms.sum() - want) <= 1e-5 * terms.abs().sum(), (i, terms.sum(), want)
+
+
+def test_left_out_rows_do_not_set_the_scale(cuda):
+    # the fp32 operands are scaled by their matrix's largest value: rows without a loss have no part
+    x, w, labels, dloss = inputs(70, 300, 33, F, seed=21)
+    labels[::7] = -1
+    dirty = torch.where((labels < 0)[:, None], 1e30, x)
+    out = agk.linear_cross_entropy_fwd(dirty, w, labels)
+    (loss,), (bound,) = reference(x, w, labels, None)
+    check(out[0], loss, bound, "loss")
+    clean = agk.linear_cross_entropy_fwd(x, w, labels)
+    keep = labels >= 0
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[1][keep], clean[1][keep])
+    for a, b in zip(agk.linear_cross_entropy_bwd(dirty, w, labels, out[1], dloss),
+                    agk.linear_cross_entropy_bwd(x, w, labels, clean[1], dloss)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("ex,ew", [(0, -101), (0, -99), (-101, 0), (-60, -60), (30, -101), (60, -60)])
+def test_scales_of_any_size(cuda, ex, ew):
+    x, w, labels, dloss = inputs(40, 200, 29, F, seed=22)
+    x, w = x * 2.0 ** ex, w * 2.0 ** ew
+    loss, stats = agk.linear_cross_entropy_fwd(x, w, labels)
+    dx, dw = agk.linear_cross_entropy_bwd(x, w, labels, stats, dloss)
+    ref, bound = reference(x, w, labels, dloss)
+    for got, want, tol, what in zip((loss, dx, dw), ref, bound, ("loss", "dx", "dw")):
+        check(got, want, tol, what)
+        assert got.abs().max() > 0

@@ -104,7 +104,14 @@ def test_linear_xent_more_validation():
     assert _xent_bwd(dx=FAKE + 8) == EINVAL and _xent_bwd(dw=FAKE + 2) == EINVAL
     # rows * ldx past 2^30
     assert _xent_bwd(rows=(1 << 24) - 8, vocab=99, cols=72, ldx=72, ldw=72) == EINVAL
+    # G's pieces of at least 256 vocabulary rows, whatever the width
+    assert _xent_bwd(rows=(1 << 22) + 1, cols=8, ldx=8, ldw=8) == EINVAL
+    assert _xent_bwd(rows=1 << 22, cols=8, ldx=8, ldw=8, ws=None) == EWORKSPACE
+    assert _xent_bwd(rows=(1 << 21) + 1, cols=8, ldx=8, ldw=8, dtype=F32) == EINVAL
+    assert _xent_bwd(rows=1 << 21, cols=8, ldx=8, ldw=8, dtype=F32, ws=None) == EWORKSPACE
+    assert _xent_fwd(loss=FAKE + 2) == EINVAL and _xent_bwd(dloss=FAKE + 2) == EINVAL
     assert _xent_bwd(rows=0, x=None, w=None, dw=None) == OK
+    assert _xent_bwd(rows=0, cols=57, x=None, w=None, dw_dtype=BF16) == EINVAL
     assert _xent_bwd(rows=0, x=None, w=None, acc=2) == OK
     f = agk.lib().agk_linear_xent_fwd_workspace_bytes
     b = agk.lib().agk_linear_xent_bwd_workspace_bytes
