@@ -9,6 +9,7 @@ is no Python or CPU fallback: if the library is missing, every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional, Tuple
 
@@ -873,8 +874,21 @@ def _row_column(x, rows):
     return _empty(shape, _torch().float32, x)
 
 
-def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None,
-                         stream=None):
+def _on_stream(call):
+    """`call` with the keyword `stream` (None: the current one).  The call runs with that stream
+    current, so that what it allocates (its workspace goes back to the allocator as it returns)
+    and clears is ordered on the stream that its kernels use."""
+    @functools.wraps(call)
+    def on(*args, stream=None, **kwargs):
+        if stream is None:
+            return call(*args, **kwargs)
+        with _torch().cuda.stream(stream):
+            return call(*args, **kwargs)
+    return on
+
+
+@_on_stream
+def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None):
     """y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis (gamma, beta: [cols] of
     x's dtype, or None); returns (y, mean, rstd), the statistics float32 [..., 1]."""
     torch = _torch()
@@ -898,14 +912,15 @@ def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, r
         _want(rstd, "rstd", dev, rows, torch.float32)
     rc = lib().agk_layernorm_affine_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean),
                                         _ptr(rstd), rows, cols, float(eps), _dtype_code(x),
-                                        _stream(stream))
+                                        _stream(None))
     _check(rc, "agk_layernorm_affine_fwd")
     return y, mean, rstd
 
 
+@_on_stream
 def layernorm_affine_bwd(x, gamma, mean, rstd, dy, dx=None, dgamma=None, dbeta=None,
                          accumulate=False, want_dx: bool = True, want_dgamma: bool = True,
-                         want_dbeta: bool = True, workspace=None, stream=None):
+                         want_dbeta: bool = True, workspace=None):
     """VJP of layernorm_affine_fwd: (dx, dgamma, dbeta), None where not wanted; dgamma and dbeta
     float32 [cols].  accumulate: a bool (every output) or AGK_ACCUM_DX / _DGAMMA / _DBETA bits."""
     torch = _torch()
@@ -939,7 +954,7 @@ def layernorm_affine_bwd(x, gamma, mean, rstd, dy, dx=None, dgamma=None, dbeta=N
     ws, ws_bytes = _scratch(workspace, need, x)
     rc = lib().agk_layernorm_affine_bwd(_ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dy),
                                         _ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(ws), ws_bytes,
-                                        rows, cols, _dtype_code(x), acc, _stream(stream))
+                                        rows, cols, _dtype_code(x), acc, _stream(None))
     _check(rc, "agk_layernorm_affine_bwd")
     return dx, dgamma, dbeta
 
@@ -971,7 +986,8 @@ def _loss_and_stats(shape, rows, dev, like, loss, stats):
     return loss, stats
 
 
-def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None, stream=None):
+@_on_stream
+def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None):
     """The softmax cross entropy of z = x @ w.T against labels, without z in memory
     (agk_linear_xent_fwd): x [..., cols], w [vocab, cols], labels int64 [...]; a negative label is
     a row without a loss.  Returns (loss, stats): float32 [...] and [..., 2] (each row's maximum
@@ -984,14 +1000,15 @@ def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None
         rows, vocab, cols, dt), x)
     rc = lib().agk_linear_xent_fwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(loss),
                                    _ptr(stats), _ptr(ws), ws_bytes, rows, vocab, cols, dt,
-                                   _stream(stream))
+                                   _stream(None))
     _check(rc, "agk_linear_xent_fwd")
     return loss, stats
 
 
+@_on_stream
 def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dtype=None,
                              accumulate=False, want_dx: bool = True, want_dw: bool = True,
-                             piece: int = 0, workspace=None, stream=None):
+                             piece: int = 0, workspace=None):
     """Gradients of linear_cross_entropy_fwd for dloss, the float32 gradient of each row's loss
     (agk_linear_xent_bwd): (dx, dw), None where not wanted.  dw is float32 unless dw_dtype (or
     dw) says otherwise.  accumulate: a bool (both) or AGK_ACCUM_DX / AGK_ACCUM_DGAMMA (dw) bits.
@@ -1016,7 +1033,7 @@ def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dt
     rc = lib().agk_linear_xent_bwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(stats),
                                    _ptr(dloss), _ptr(dx), _ptr(dw),
                                    _dtype_code(dw) if dw is not None else AGK_F32, _ptr(ws),
-                                   ws_bytes, rows, vocab, cols, piece, dt, acc, _stream(stream))
+                                   ws_bytes, rows, vocab, cols, piece, dt, acc, _stream(None))
     _check(rc, "agk_linear_xent_bwd")
     return dx, dw
 
@@ -1033,8 +1050,9 @@ def _distill_sizes(z, index, teacher):
     return dev, rows, cols, k
 
 
+@_on_stream
 def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, stats=None,
-                     workspace=None, stream=None):
+                     workspace=None):
     """T^2 KL(p || q) per row of q = softmax(z / T) over all columns from p = softmax(teacher / T)
     over the row's k named columns (agk_distill_topk_fwd): z [..., cols], index int64 [..., k] (a
     negative one is an empty entry), teacher [..., k] float32 or bfloat16.  Returns (loss, stats):
@@ -1045,13 +1063,14 @@ def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, sta
     ws, ws_bytes = _scratch(workspace, lib().agk_distill_topk_workspace_bytes(rows, cols, dt), z)
     rc = lib().agk_distill_topk_fwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(loss), _ptr(stats),
                                     _ptr(ws), ws_bytes, rows, cols, k, float(temperature), dt,
-                                    _dtype_code(teacher), _stream(stream))
+                                    _dtype_code(teacher), _stream(None))
     _check(rc, "agk_distill_topk_fwd")
     return loss, stats
 
 
+@_on_stream
 def distill_topk_bwd(z, index, teacher, stats, dloss, temperature: float = 1.0, dz=None,
-                     accumulate: bool = False, stream=None):
+                     accumulate: bool = False):
     """Gradient of z for dloss, the float32 gradient of each row's loss: dz (+)= dloss * T *
     (q - p at the named columns) (agk_distill_topk_bwd).  dz may be z (in place)."""
     torch = _torch()
@@ -1064,6 +1083,6 @@ def distill_topk_bwd(z, index, teacher, stats, dloss, temperature: float = 1.0, 
         _want(dz, "dz", dev, z.numel(), z.dtype)
     rc = lib().agk_distill_topk_bwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(stats), _ptr(dloss),
                                     _ptr(dz), rows, cols, k, float(temperature), _dtype_code(z),
-                                    _dtype_code(teacher), _acc_dx(accumulate), _stream(stream))
+                                    _dtype_code(teacher), _acc_dx(accumulate), _stream(None))
     _check(rc, "agk_distill_topk_bwd")
     return dz
