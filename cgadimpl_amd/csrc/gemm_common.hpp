@@ -132,7 +132,8 @@ __device__ __forceinline__ f32x16 mfma16(const bf16x8& a, const bf16x8& b, const
 // Where the direct and ring kernels find k-tile t of an operand: LinearK, K once through.
 // (A product whose operands are stored as several planes brings an order of its own.)
 struct LinearK {
-    static constexpr bool kF16 = false;  // bf16 operands
+    static constexpr bool kF16 = false;     // bf16 operands
+    static constexpr bool kStream = false;  // A's loads in the ring non-temporal
     __device__ __forceinline__ int start(int n) { return n; }  // n whole k-tiles: the tiles in all
     __device__ __forceinline__ int a(int t, int step) const { return t * step; }  // byte offsets
     __device__ __forceinline__ int b(int t, int step) const { return t * step; }

@@ -214,6 +214,10 @@ __device__ __forceinline__ void ring_load_a(const RingRsrc& q, uint16_t* lds, ui
                                             int at) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(q.a, (lds_ptr_t)lds, 16, off, at, 0, 0);
 }
+__device__ __forceinline__ void ring_load_a_stream(const RingRsrc& q, uint16_t* lds, uint32_t off,
+                                                   int at) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(q.a, (lds_ptr_t)lds, 16, off, at, 0, 2);
+}
 __device__ __forceinline__ void ring_load_b(const RingRsrc& q, uint16_t* lds, uint32_t off,
                                             int at) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(q.b, (lds_ptr_t)lds, 16, off, at, 0, 0);
@@ -228,8 +232,11 @@ __device__ __forceinline__ void ring_issue_a(const RingOperands& r, const KM& km
     const bool in = t < r.nk;
     const RingRsrc q = ring_rsrc(r, in);
 #pragma unroll
-    for (int j = 0; j < SH::kBM / 32; ++j)
-        ring_load_a(q, stage + (wave * (SH::kBM / 32) + j) * 512, o.a[j], in ? km.a(t, r.step_a) : 0);
+    for (int j = 0; j < SH::kBM / 32; ++j) {
+        uint16_t* const to = stage + (wave * (SH::kBM / 32) + j) * 512;
+        if constexpr (KM::kStream) ring_load_a_stream(q, to, o.a[j], in ? km.a(t, r.step_a) : 0);
+        else ring_load_a(q, to, o.a[j], in ? km.a(t, r.step_a) : 0);
+    }
 }
 template <class SH, class KM>
 __device__ __forceinline__ void ring_issue_b(const RingOperands& r, const KM& km,

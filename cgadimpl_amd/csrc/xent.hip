@@ -377,8 +377,7 @@ constexpr int64_t kMaxOperand = 1LL << 30;    // values a product's 31-bit offse
 constexpr int64_t kMaxTokens = 1LL << 24;     // a workgroup per token within a grid
 
 // G's rows are padded to whole 128-byte lines of bf16: the products fetch 128 bytes of
-// a row at a time, which at any other pitch straddle two lines.
-constexpr int64_t kLine = 64;
+// a row at a time, which at any other pitch straddle two lines (kLine).
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 inline size_t region(int64_t bytes) { return static_cast<size_t>(up(bytes, 256)); }
@@ -396,12 +395,22 @@ inline int64_t piece_rows(int64_t vocab, int64_t ldg, int64_t ldw, int planes, i
     return up((vocab + n - 1) / n, 256);
 }
 
-// The forward's tile: by the general rule, with the 32-row wave blocks of the 64-row
-// tiles (ids 7 and 8: four times the partials) for few tokens only.
-constexpr int64_t kFewTokens = 128;
-inline int lse_shape(int64_t rows, int64_t vocab, int64_t cols) {
+// The tile of the logits' products: by the general rule, but for one column of 64 tokens, whose
+// time is the read of w: 64 x 64 tiles (id 8) as long as one round holds them, 128 x 64 beyond.
+// Forward of 16 tokens, us, rule / this: 4096 x 12000 37 / 28, x 20000 43 / 39, x 28000 54 / 43,
+// 64 x 8192 x 12000 69 / 52; 64 x 64 tiles in two rounds: 2048 x 50257 46, 128 x 64 41.
+inline int logits_shape(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
     using namespace agk_gemm;
-    const int s = pick_shape(vocab, rows, cols, device_cus());
+    const int cus = device_cus();
+    if (dtype == AGK_BF16 && rows <= 64 && cols >= BK) return vocab <= 128 * cus ? 8 : 6;
+    return pick_shape(vocab, rows, cols, cus);
+}
+// The forward's: the 32-row wave blocks of the 64-row tiles (ids 7 and 8: four times the partials)
+// for few tokens only.
+constexpr int64_t kFewTokens = 128;
+inline int lse_shape(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
+    using namespace agk_gemm;
+    const int s = logits_shape(rows, vocab, cols, dtype);
     if ((s != 7 && s != 8) || rows <= kFewTokens) return s;
     return agk::grid_fits(((vocab + 127) / 128) * ((rows + 63) / 64), 256) ? 6 : kRingLargest;
 }
@@ -621,7 +630,7 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
         const int nv = static_cast<int>(n);
-        const int shape = lse_shape(rows, n, bf16 ? cols : o.kp);
+        const int shape = lse_shape(rows, n, bf16 ? cols : o.kp, dtype);
         float2* const to = part + blocks * rows;
         if (bf16) {
             rc = launch_lse(shape,
@@ -728,7 +737,7 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         char* const out = static_cast<char*>(dw) + v0 * cols * dw_size;
         if (bf16) {
             const uint16_t* const wp = static_cast<const uint16_t*>(w) + v0 * ldw;
-            rc = launch_grad(agk_gemm::pick_shape(n, rows, cols, cus),
+            rc = launch_grad(logits_shape(rows, n, cols, dtype),
                              Product{wp, ldw, static_cast<const uint16_t*>(x), ldx, nv, m, c1, 1, 0,
                                      st},
                              GradEpi<1>{g, in, weight, labels, v0, ldg, nv, nv, m, nullptr});

@@ -22,6 +22,7 @@ namespace agk_xent {
 using agk_gemm::f32x16;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int64_t kLine = 64;  // bf16 of a 128-byte line
 
 // fp32 operands.  A matrix is stored scaled by a power of two that brings its largest value to
 // 2^14 .. 2^15, each value as two fp16 whose sum it is to 2^-22 of it: x = a + b, a = fp16(x), b =
@@ -36,7 +37,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // MI355X: fp32 instruction 2.47 ms, bf16 planes 1.59, fp16 planes 0.96; relative error of dx
 // 6e-7 (fp32 products of the BLAS library: 3e-6).
 struct PlanesK {
-    static constexpr bool kF16 = true;
+    static constexpr bool kF16 = true, kStream = false;
     static constexpr int kWalks = 3;
     int plane_a, plane_b;  // bytes from one plane to the next
     int n;                 // k-tiles of a plane
@@ -67,6 +68,32 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&plane)[2]) {
     plane[0] = __builtin_bit_cast(uint32_t, a);
     plane[1] = __builtin_bit_cast(uint32_t, b);
 }
+
+// Few tokens, one column of tiles: the time is the read of w, each row by one workgroup, so its
+// loads are non-temporal.  Workgroups that walk K in step read the same offsets of rows that lie,
+// as a rule, a power of two apart, which are in a few of the memory's channels; so each starts at
+// a k-tile of its own.  Forward on MI355X, w not in the caches, in step / turned (us): 16 tokens x
+// 4096 x 32000 55 / 48 (of it the join and two launches' gaps 8; 262 MB at 6.6 TB/s), x 2048 x
+// 50257 50 / 41, 64 x 8192 x 32000 108 / 96.  It does not pay with few tiles, which are bound by
+// latency (16 x 4096 x 8000, 125 tiles: 24 / 27), nor where rows are not whole 128-byte lines,
+// two k-tiles sharing one (16 x 1000 x 100000: 55 / 63); deeper rings gain nothing (4 or 7 stages of 128 x
+// 32: the same).
+struct TurnedK {
+    static constexpr bool kF16 = false, kStream = true;
+    int n, first;
+
+    __device__ __forceinline__ int start(int tiles) {
+        n = tiles;
+        first = tiles ? static_cast<int>(blockIdx.x % static_cast<unsigned>(tiles)) : 0;
+        return tiles;
+    }
+    __device__ __forceinline__ int a(int t, int step) const {
+        return (t + first >= n ? t + first - n : t + first) * step;
+    }
+    __device__ __forceinline__ int b(int t, int step) const { return a(t, step); }
+    __device__ __forceinline__ int more_a() const { return 0; }
+    __device__ __forceinline__ int more_b() const { return 0; }
+};
 
 // exp(x) on v_exp_f32; see fast_exp in rowops.hip for its error.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -513,6 +540,28 @@ int launch_product(int shape, const Product& p, const Epi& e, const KM& km = {})
     switch (shape) { AGK_RING_SHAPES(AGK_XENT_CASE) }
 #undef AGK_XENT_CASE
     return agk::check_launch();
+}
+
+// A product of x and w, both k-contiguous: on TurnedK where one column of tiles holds the tokens
+// and the tiles are enough to be bound by the read of w.
+template <class Epi>
+int launch_logits(int shape, const Product& p, const Epi& e) {
+    using namespace agk_gemm;
+    const int least = p.lda % kLine == 0 ? device_cus() * 3 / 4 : 0x7fffffff;
+#define AGK_XENT_CASE(ID, BM_, BN_, WVM, NST)                                                    \
+    if constexpr (BM_ <= 128 && BN_ <= 128) {                                                    \
+        const int tiles_m = (p.M + BM_ - 1) / BM_;                                               \
+        if (shape == ID && p.N <= BN_ && tiles_m >= least) {                                     \
+            using SH = RingShape<BM_, BN_, WVM, NST>;                                            \
+            hipLaunchKernelGGL((xent_ring_kernel<false, false, SH, Epi, TurnedK>),               \
+                               dim3(tiles_m), dim3(256), 0, p.st, p.A, p.lda, p.B, p.ldb, p.M,   \
+                               p.N, p.K, p.k_slice, e, TurnedK{}, tiles_m, 1);                   \
+            return agk::check_launch();                                                          \
+        }                                                                                        \
+    }
+    AGK_RING_SHAPES(AGK_XENT_CASE)
+#undef AGK_XENT_CASE
+    return launch_product<false, false>(shape, p, e);
 }
 
 }  // namespace agk_xent

@@ -6,7 +6,7 @@
 namespace agk_xent {
 
 int launch_grad(int shape, const Product& p, const GradEpi<1>& e) {
-    return launch_product<false, false>(shape, p, e);
+    return launch_logits(shape, p, e);
 }
 int launch_grad(int shape, const Product& p, const GradEpi<2>& e, const PlanesK& k) {
     return launch_product<false, false>(shape, p, e, k);

@@ -6,7 +6,7 @@
 namespace agk_xent {
 
 int launch_lse(int shape, const Product& p, const LseEpi<false>& e) {
-    return launch_product<false, false>(shape, p, e);
+    return launch_logits(shape, p, e);
 }
 int launch_lse(int shape, const Product& p, const LseEpi<true>& e, const PlanesK& k) {
     return launch_product<false, false>(shape, p, e, k);

@@ -393,3 +393,30 @@ def test_scales_of_any_size(cuda, ex, ew):
     for got, want, tol, what in zip((loss, dx, dw), ref, bound, ("loss", "dx", "dw")):
         check(got, want, tol, what)
         assert got.abs().max() > 0
+
+
+@pytest.mark.parametrize("N,V,D,pitch", [
+    (1, 12289, 64, 64), (33, 13001, 192, 192), (64, 33001, 128, 128), (20, 32900, 64, 64),
+    (7, 20011, 200, 256), (64, 33003, 72, 128), (65, 25000, 192, 192), (100, 30011, 136, 192),
+    (3, 33001, 72, 72)])
+def test_few_tokens_of_many_words(cuda, N, V, D, pitch):
+    # one column of tiles whose workgroups start their walks of K at different tiles
+    x, w, labels, dloss = inputs(N, V, D, BF, seed=23)
+    wide = torch.full((V, pitch), float("nan"), device="cuda", dtype=BF)
+    wide[:, :D] = w
+    lib = agk.lib()
+    P = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    loss, stats = torch.empty(N, device="cuda"), torch.empty(N, 2, device="cuda")
+    dx, dw = torch.empty_like(x), torch.empty(V, D, device="cuda")
+    nf = lib.agk_linear_xent_fwd_workspace_bytes(N, V, D, agk.AGK_BF16)
+    nb = lib.agk_linear_xent_bwd_workspace_bytes(N, V, D, agk.AGK_BF16, 0)
+    ws = torch.empty(max(nf, nb), dtype=torch.uint8, device="cuda")
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.agk_linear_xent_fwd(P(x), D, P(wide), pitch, P(labels), P(loss), P(stats), P(ws), nf,
+                                   N, V, D, agk.AGK_BF16, st) == 0
+    assert lib.agk_linear_xent_bwd(P(x), D, P(wide), pitch, P(labels), P(stats), P(dloss), P(dx),
+                                   P(dw), agk.AGK_F32, P(ws), nb, N, V, D, 0, agk.AGK_BF16, 0,
+                                   st) == 0
+    ref, bound = reference(x, w, labels, dloss)
+    for got, want, tol, what in zip((loss, dx, dw), ref, bound, ("loss", "dx", "dw")):
+        check(got, want, tol, (what, N, V, D))
