@@ -6,9 +6,10 @@
 //
 // Both passes stream z: the forward reads it once, keeping a running maximum and sum
 // per lane, the backward reads it once and writes dz.  The teacher's part is a few
-// hundred values a row.  HBM bounds them.  A row is one workgroup's; rows too few to fill the chip are
-// cut into segments, whose {max, sum} meet in a second kernel (forward); the backward takes
-// a row in chunks always, each computing the row's p again.
+// hundred values a row.  HBM bounds them: 8192 x 50257 bf16, k = 64, 135 us forward (6.1 TB/s) and
+// 270 backward (6.1) on MI355X.  In the forward a row is one workgroup's; a few very wide rows
+// are cut into segments, whose {max, sum} meet in a second kernel; the backward takes a row in
+// chunks always, each computing the row's p again.
 
 #include <hip/hip_runtime.h>
 
@@ -324,11 +325,12 @@ __global__ __launch_bounds__(64) void distill_join(const Args a, const float2* _
 // One wave per chunk of kChunk 16-byte slots of a row, four chunks in a row per workgroup
 // and no barrier: a stream of reads and writes runs fastest where the chip works through
 // memory in one compact window (copies: 6.05 TB/s with 16 KiB per workgroup, 4.2-5.2 with
-// workgroups that loop over long rows).  The wave issues its loads of z behind those of the
-// row's teacher and computes p for itself while they are in flight (PER entries per lane, a
-// maximum and a sum over the wave).  The entries whose column lies in the chunk are then taken one by one, in order:
-// the column's slot and element are the same for the whole wave, so that one lane's
-// register takes - c p.  Columns named twice need nothing more.
+// workgroups that loop over long rows; this kernel so, 352 us where it takes 270 now).  The
+// wave issues its loads of z behind those of the row's teacher and computes p for itself while
+// they are in flight (PER entries per lane, a maximum and a sum over the wave).  The entries
+// whose column lies in the chunk are then taken one by one, in order: the column's slot and
+// element are the same for the whole wave, so that one lane's register takes - c p.  Columns
+// named twice need nothing more.
 constexpr int kSlots = 4;              // 16-byte slots per lane
 constexpr int kChunk = 64 * kSlots;    // and per wave
 

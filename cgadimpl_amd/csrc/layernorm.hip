@@ -10,8 +10,11 @@
 // columns' dgamma and dbeta terms in fp32 over its rows; the workgroup's sums are one
 // partial row of each, and a second kernel adds the partial rows in fp64 in a fixed
 // order (no atomics: bit-identical run to run).  HBM-bound: x and dy read once, dx
-// written once.  Rows of less than one slot, or too wide for registers, take a looped
-// kernel that reads x and dy twice.
+// written once; 16384 x 8192 bf16 137 us on MI355X (5.9 TB/s) and 4.6 for the second kernel.
+// One workgroup per CU that loops, not one per group of rows: the partial rows are then
+// 256 whatever the rows are, and their two writes and reads stay in the caches.  4099 x 1030
+// f32: 13.8 + 3.9 us, bound by latency (5.4 groups of rows per workgroup).  Rows of less than
+// one slot, or too wide for registers, take a looped kernel that reads x and dy twice.
 
 #include <hip/hip_runtime.h>
 

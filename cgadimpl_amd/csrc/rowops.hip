@@ -881,6 +881,8 @@ struct LnFwd {
 
 // LayerNorm with weight and bias (col0 = gamma, col1 = beta besides):
 //   y = (x - mean) * rstd * gamma + beta
+// x read once and y written once, the row in registers between: 16384 x 8192 bf16 95 us on
+// MI355X (5.6 TB/s, HBM), 16 x 4096 5 us (the latency of two sums one after the other).
 struct LnAffineFwd {
     static constexpr int kIn = 1;
     template <class C>

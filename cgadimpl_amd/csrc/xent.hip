@@ -9,7 +9,9 @@
 // again, a piece of the vocabulary at a time, leaving G's piece in bf16 (the matrix
 // cores' operand), and takes the two products from it.  dw's rows belong to one piece;
 // dx adds up in fp32 over the pieces.  8 tokens vocab cols flop a step, 2 of the forward and
-// 6 of the backward (2 of them the logits again: the price of not keeping them).
+// 6 of the backward (2 of them the logits again: the price of not keeping them).  The matrix
+// cores bound them: 8192 x 4096 x 131072 forward 6.2 ms and backward 19.9 on MI355X, 1350
+// TFLOP/s; a few tokens' forward is bound by the read of w (TurnedK).
 //
 // fp32.  The same kernels on operands split into two fp16 planes (PlanesK), x once a call
 // and w a piece at a time, after a pass over them for their largest values; G leaves its
