@@ -230,36 +230,47 @@ struct GradEpi {
         // even lanes: {own low, neighbour's low}; odd lanes: {neighbour's high, own high}
         const uint32_t pick = odd ? 0x07060302u : 0x01000504u;
         const float sc = PLANES == 1 ? 1.0f : *scale;
+        float w[TNW], m[TNW], shift[TNW];
+        int at[TNW];
+        bool hit = false, some_out = false;
 #pragma unroll
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
             const bool in = col < tokens;
             const float2 st = in ? stats[col] : make_float2(0.0f, 0.0f);
-            const float w = in ? (PLANES == 1 ? weight[col] : weight[col] * kTop) : 0.0f;
-            const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
-            const bool hit = __any(at >= 0);
-            const bool some_out = __any(w == 0.0f);
+            w[j] = in ? (PLANES == 1 ? weight[col] : weight[col] * kTop) : 0.0f;
+            at[j] = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
+            hit = hit || at[j] >= 0;
+            some_out = some_out || w[j] == 0.0f;
             // bf16: exp(z - (m + l)), m + l rounded once (2^-24 of its size: far below G's
             // rounding); fp32: the difference z - m first
-            const float m = PLANES == 1 ? 0.0f : st.x;
-            const float shift = (PLANES == 1 ? st.x + st.y : st.y) * kLog2e;
-            const bool store = col < ldg;  // ldg is even: a pair is in or out
-            uint16_t* const out =
-                G + (col & ~1) + static_cast<int64_t>(row0 + odd) * (PLANES * ldg);
+            m[j] = PLANES == 1 ? 0.0f : st.x;
+            shift[j] = (PLANES == 1 ? st.x + st.y : st.y) * kLog2e;
+        }
+        hit = __any(hit);
+        some_out = __any(some_out);
+        uint16_t* const out =
+            G + col0 + (lane & 30) + static_cast<int64_t>(row0 + odd) * (PLANES * ldg);
+        const int left = ldg - col0 - (lane & 30);  // ldg is even: a pair is in or out
+        // a row's tokens together: its lines are written whole
 #pragma unroll
-            for (int i = 0; i < TMW; ++i)
+        for (int i = 0; i < TMW; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const int r = acc_row(i, e, half);
+            for (int e = 0; e < 16; e += 2) {
+                const int r = acc_row(i, e, half);
+                uint16_t* const row = out + static_cast<int64_t>(r) * (PLANES * ldg);
+                const bool store = inner || row0 + r + odd < padded_rows;
+#pragma unroll
+                for (int j = 0; j < TNW; ++j) {
                     float g[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const float z = PLANES == 1 ? acc[i][j][e + u]
-                                                    : __builtin_fmaf(acc[i][j][e + u], sc, -m);
-                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -shift));
-                        if (hit) p -= at == r + u ? 1.0f : 0.0f;
-                        g[u] = w * p;
-                        if (some_out) g[u] = w != 0.0f ? g[u] : 0.0f;  // z may be NaN there
+                                                    : __builtin_fmaf(acc[i][j][e + u], sc, -m[j]);
+                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -shift[j]));
+                        if (hit) p -= at[j] == r + u ? 1.0f : 0.0f;
+                        g[u] = w[j] * p;
+                        if (some_out) g[u] = w[j] != 0.0f ? g[u] : 0.0f;  // z may be NaN there
                         if (!inner) g[u] = row0 + r + u < rows ? g[u] : 0.0f;
                     }
                     uint32_t own[2];
@@ -270,12 +281,11 @@ struct GradEpi {
                         const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(
                             static_cast<int>(own[q]), 0xb1, 0xf, 0xf, true));
                         const uint32_t v = __builtin_amdgcn_perm(own[q], other, pick);
-                        if (store && (inner || row0 + r + odd < padded_rows))
-                            *reinterpret_cast<uint32_t*>(
-                                out + static_cast<int64_t>(r) * (PLANES * ldg) + q * ldg) = v;
+                        if (store && j * 32 < left)
+                            *reinterpret_cast<uint32_t*>(row + j * 32 + q * ldg) = v;
                     }
                 }
-        }
+            }
     }
 };
 
