@@ -14,8 +14,8 @@
 // TFLOP/s; a few tokens' forward is bound by the read of w (TurnedK).
 //
 // fp32.  The same kernels on operands split into two fp16 planes (PlanesK), x once a call
-// and w a piece at a time, after a pass over them for their largest values; G leaves its
-// kernel split.
+// and w a piece at a time; in the backward, whose products sum along every index, after a pass
+// over them for their largest values.  G leaves its kernel split.
 //
 // A token that is left out (a negative label, or a zero dloss) has a zero row of G
 // whatever its logits are, and the product over tokens reads its row of x as zeros,
@@ -102,28 +102,20 @@ struct Scalars {
     float dw;
 };
 
-// Largest finite |value| of `rows` rows, one wave to a row; rows are left out where keep says so.
+// This lane's share of the largest finite |value| of a row (and of m), a wave to a row.
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
-template <class Keep>
-__device__ __forceinline__ float rows_max(const float* __restrict__ src, int64_t ld, int64_t rows,
-                                          int cols, int64_t first, int64_t stride, Keep keep) {
-    const int lane = static_cast<int>(threadIdx.x & 63);
-    float m = 0.0f;
+__device__ __forceinline__ float row_max(const float* __restrict__ p, int cols, int lane, float m) {
     auto take = [&](float v) {
         v = __builtin_fabsf(v);
         if (v < __builtin_inff()) m = v > m ? v : m;
     };
-    for (int64_t r = first; r < rows; r += stride) {
-        if (!keep(r)) continue;
-        const float* const p = src + r * ld;
-        int c = lane * 4;
-        for (; c + 4 <= cols; c += 256) {
-            const f32x4_a4 q = *reinterpret_cast<const f32x4_a4*>(p + c);
+    int c = lane * 4;
+    for (; c + 4 <= cols; c += 256) {
+        const f32x4_a4 q = *reinterpret_cast<const f32x4_a4*>(p + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) take(q[e]);
-        }
-        for (int e = c; e < cols && e < c + 4; ++e) take(p[e]);
+        for (int e = 0; e < 4; ++e) take(q[e]);
     }
+    for (int e = c; e < cols && e < c + 4; ++e) take(p[e]);
     return m;
 }
 // e of a largest value of 2^e ..; the matrix's scale is 2^(14 - e), and the factor that takes a
@@ -146,7 +138,7 @@ struct Matrices {
     int64_t ldx, ldw, rows, wrows;
     int cols, x_groups;
     const int64_t* labels;  // tokens that are left out are read as zeros and have no part in
-    const float* dloss;     // the maximum; NULL in the forward
+    const float* dloss;     // the maxima; NULL in the forward
     __device__ __forceinline__ bool keep(int64_t t) const {
         return labels[t] >= 0 && (!dloss || dloss[t] != 0.0f);
     }
@@ -159,10 +151,11 @@ __global__ __launch_bounds__(256) void xent_max(const Matrices a, float* __restr
     const int k = is_x ? g : g - a.x_groups;
     const int64_t groups = is_x ? a.x_groups : static_cast<int>(gridDim.x) - a.x_groups;
     const int64_t first = static_cast<int64_t>(k) * 4 + (threadIdx.x >> 6);
-    float m = is_x ? rows_max(a.x, a.ldx, a.rows, a.cols, first, groups * 4,
-                              [&](int64_t t) { return a.keep(t); })
-                   : rows_max(a.w, a.ldw, a.wrows, a.cols, first, groups * 4,
-                              [](int64_t) { return true; });
+    const int lane = static_cast<int>(threadIdx.x & 63);
+    float m = 0.0f;
+    for (int64_t r = first; r < (is_x ? a.rows : a.wrows); r += groups * 4)
+        if (!is_x || a.keep(r))
+            m = row_max(is_x ? a.x + r * a.ldx : a.w + r * a.ldw, a.cols, lane, m);
     for (int h = 32; h > 0; h /= 2) m = fmaxf(m, __shfl_xor(m, h));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -191,6 +184,30 @@ __device__ __forceinline__ void split_row(const float* __restrict__ src, int col
 #pragma unroll
         for (int q = 0; q < 2; ++q)
             *reinterpret_cast<uint2*>(dst + q * kp + c) = make_uint2(lo[q], hi[q]);
+    }
+}
+
+// The forward's planes, each row by a scale of its own: the product is summed along the rows, so
+// its factors are one per logit's row and column (scales: x's, then w's), and no pass over the
+// matrices for their largest value goes before.
+__global__ __launch_bounds__(256) void xent_split_rows(const Matrices a, int kp,
+                                                       uint16_t* __restrict__ x2,
+                                                       uint16_t* __restrict__ w2,
+                                                       float* __restrict__ x_scales,
+                                                       float* __restrict__ w_scales) {
+    const int wave = static_cast<int>(threadIdx.x >> 6), lane = static_cast<int>(threadIdx.x & 63);
+    const bool is_x = static_cast<int>(blockIdx.x) < a.x_groups;
+    const int64_t g = is_x ? blockIdx.x : blockIdx.x - a.x_groups;
+    const int64_t groups = is_x ? a.x_groups : static_cast<int>(gridDim.x) - a.x_groups;
+    for (int64_t r = g * 4 + wave; r < (is_x ? a.rows : a.wrows); r += groups * 4) {
+        const float* p = is_x ? a.x + r * a.ldx : a.w + r * a.ldw;
+        if (is_x && !a.keep(r)) p = nullptr;
+        float m = p ? row_max(p, a.cols, lane, 0.0f) : 0.0f;
+        for (int h = 32; h > 0; h /= 2) m = fmaxf(m, __shfl_xor(m, h));
+        const int e = top_exponent(m);
+        split_row(p, a.cols, kp, pow2(14 - e), (is_x ? x2 : w2) + r * 2 * static_cast<int64_t>(kp),
+                  lane);
+        if (lane == 0) (is_x ? x_scales : w_scales)[r] = pow2(e - 14);
     }
 }
 
@@ -491,16 +508,15 @@ inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
 // The workspaces.  `cols` of the operands as staged: kp for planes (whole k-tiles).
 struct FwdLayout {
     int64_t kp, piece;
-    size_t scalars, parts, picked, part, x2, w2, total;
+    size_t scales, picked, part, x2, w2, total;
 };
 inline FwdLayout fwd_layout(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
     FwdLayout o;
     const bool bf16 = dtype == AGK_BF16;
     o.kp = up(cols, 64);
     o.piece = bf16 ? vocab : piece_rows(vocab, 64, o.kp, 2, 0);
-    o.scalars = 0;
-    o.parts = o.scalars + region(sizeof(Scalars));
-    o.picked = o.parts + (bf16 ? 0 : region(2 * kMaxParts * 4));
+    o.scales = 0;  // x's and w's; a wave's block of up to 128 rows can pass the last one
+    o.picked = o.scales + (bf16 ? 0 : region((up(rows, 64) + o.piece + 128) * 4));
     o.part = o.picked + region(rows * 4);
     o.x2 = o.part + region(max_blocks(rows, vocab, o.piece) * rows * 8);
     o.w2 = o.x2 + (bf16 ? 0 : region(rows * o.kp * 4));
@@ -574,6 +590,16 @@ int launch_join(const float2* part, int64_t blocks, const float* picked, const i
     return check_launch();
 }
 
+// The forward's planes: x's (where a.x) and those of a piece of w.
+int launch_planes_rows(Matrices a, int64_t kp, uint16_t* x2, uint16_t* w2, float* x_scales,
+                       float* w_scales, hipStream_t st) {
+    a.x_groups = a.x ? static_cast<int>(std::min<int64_t>((a.rows + 3) / 4, 4096)) : 0;
+    const int w_groups = static_cast<int>(std::min<int64_t>((a.wrows + 3) / 4, 16384));
+    hipLaunchKernelGGL(xent_split_rows, dim3(a.x_groups + w_groups), dim3(256), 0, st, a,
+                       static_cast<int>(kp), x2, w2, x_scales, w_scales);
+    return check_launch();
+}
+
 // The maxima's pass and the split of x (where a.x) and of a piece of w: rows to x_padded and
 // w_padded.  x's maxima and planes stay for the pieces after the first.
 int launch_planes(Matrices a, float* parts, int64_t kp, int64_t x_padded, int64_t w_padded,
@@ -624,11 +650,11 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     float2* const part = reinterpret_cast<float2*>(ws + o.part);
     uint16_t* const x2 = reinterpret_cast<uint16_t*>(ws + o.x2);
     uint16_t* const w2 = reinterpret_cast<uint16_t*>(ws + o.w2);
-    Scalars* const sc = reinterpret_cast<Scalars*>(ws + o.scalars);
+    float* const x_scales = reinterpret_cast<float*>(ws + o.scales);
+    float* const w_scales = x_scales + up(rows, 64);
     const bool bf16 = dtype == AGK_BF16;
     const int m = static_cast<int>(rows), kp = static_cast<int>(o.kp);
     int64_t blocks = 0;
-    int x_parts = 0;
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
         const int nv = static_cast<int>(n);
@@ -639,16 +665,15 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
                             Product{static_cast<const uint16_t*>(w), ldw,
                                     static_cast<const uint16_t*>(x), ldx, nv, m,
                                     static_cast<int>(cols), 1, 0, st},
-                            LseEpi<false>{to, picked, labels, v0, nv, m, nullptr});
+                            LseEpi<false>{to, picked, labels, v0, nv, m, nullptr, nullptr});
         } else {
             const Matrices a{v0 ? nullptr : static_cast<const float*>(x),
                              static_cast<const float*>(w) + v0 * ldw, ldx, ldw, rows, n,
                              static_cast<int>(cols), 0, labels, nullptr};
-            rc = launch_planes(a, reinterpret_cast<float*>(ws + o.parts), kp, rows, n, x2, w2, sc,
-                               &x_parts, st);
+            rc = launch_planes_rows(a, kp, x2, w2, x_scales, w_scales, st);
             if (rc != AGK_OK) return rc;
             rc = launch_lse(shape, Product{w2, 2 * o.kp, x2, 2 * o.kp, nv, m, kp, 1, 0, st},
-                            LseEpi<true>{to, picked, labels, v0, nv, m, &sc->z},
+                            LseEpi<true>{to, picked, labels, v0, nv, m, w_scales, x_scales},
                             PlanesK{kp * 2, kp * 2, 0});
         }
         if (rc != AGK_OK) return rc;

@@ -134,7 +134,7 @@ __device__ __forceinline__ float max3_of(float a, float b, float c) {
 // maxima per instruction, one fma, one exponential and one addition per logit, in four
 // chains.  The fma takes z log2(e) - t, t = m log2(e) rounded; the rounding, exact as
 // another fma, goes into the sum as a factor.  SCALED: the accumulators are the logits over
-// *scale (a power of two).
+// row_scale[row] * token_scale[token] (powers of two; row_scale has whole tiles' rows).
 template <bool SCALED>
 struct LseEpi {
     float2* part;
@@ -142,18 +142,13 @@ struct LseEpi {
     const int64_t* labels;
     int64_t v0;  // the first vocabulary row of the operand, which has `vocab` of them
     int vocab, tokens;
-    const float* scale;
+    const float* row_scale;
+    const float* token_scale;
 
-    template <bool INNER, int TMW, int TNW>
-    __device__ __forceinline__ float2 reduce(const f32x16 (&acc)[TMW][TNW], int j, int left,
-                                             int half, float sc) const {
+    // at(i, e): the logit in element e of group i, or the smallest value past the vocabulary
+    template <int TMW, class At>
+    __device__ __forceinline__ float2 reduce(At at) const {
         constexpr float kNone = -__builtin_inff();
-        const float log2e = SCALED ? sc * kLog2e : kLog2e;
-        // rows past the vocabulary: the smallest value, so that the sums below leave them out
-        auto at = [&](int i, int e) -> float {
-            if constexpr (INNER) return acc[i][j][e];
-            else return acc_row(i, e, half) < left ? acc[i][j][e] : kNone;
-        };
         float m4[4] = {kNone, kNone, kNone, kNone};
 #pragma unroll
         for (int i = 0; i < TMW; ++i)
@@ -162,17 +157,17 @@ struct LseEpi {
                 m4[(e / 2) & 3] = max3_of(m4[(e / 2) & 3], at(i, e), at(i, e + 1));
         float m = max_of(max_of(m4[0], m4[1]), max_of(m4[2], m4[3]));
         m = max_of(m, other_half(m));
-        const float t = m == kNone ? 0.0f : m * log2e;  // no -inf - -inf
+        const float t = m == kNone ? 0.0f : m * kLog2e;  // no -inf - -inf
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < TMW; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                s4[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(at(i, e), log2e, -t));
+                s4[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(at(i, e), kLog2e, -t));
         float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         s += other_half(s);
-        if (m != kNone) s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(m, log2e, -t));
-        return make_float2(SCALED ? m * sc : m, s);
+        if (m != kNone) s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -t));
+        return make_float2(m, s);
     }
 
     template <int TMW, int TNW>
@@ -181,23 +176,42 @@ struct LseEpi {
         if (row0 >= vocab) return;
         const int half = lane >> 5;
         const bool inner = row0 + TMW * 32 <= vocab;
-        const float sc = SCALED ? *scale : 1.0f;
         float2* const out = part + static_cast<int64_t>(row0 / (TMW * 32)) * tokens;
 #pragma unroll
         for (int j = 0; j < TNW; ++j) {
             const int col = col0 + j * 32 + (lane & 31);
             const bool in = col < tokens;
-            const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
-            const float2 v = inner ? reduce<true>(acc, j, 0, half, sc)
-                                   : reduce<false>(acc, j, vocab - row0, half, sc);
+            const int label = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
+            f32x16 z[TMW];
+#pragma unroll
+            for (int i = 0; i < TMW; ++i) {
+                z[i] = acc[i][j];
+                if constexpr (SCALED) {
+                    const float ts = in ? token_scale[col] : 1.0f;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 rs = *reinterpret_cast<const float4*>(
+                            row_scale + row0 + acc_row(i, q * 4, half));
+                        z[i][q * 4] *= rs.x * ts;
+                        z[i][q * 4 + 1] *= rs.y * ts;
+                        z[i][q * 4 + 2] *= rs.z * ts;
+                        z[i][q * 4 + 3] *= rs.w * ts;
+                    }
+                }
+            }
+            const int left = vocab - row0;
+            const float2 v =
+                inner ? reduce<TMW>([&](int i, int e) -> float { return z[i][e]; })
+                      : reduce<TMW>([&](int i, int e) -> float {
+                            return acc_row(i, e, half) < left ? z[i][e] : -__builtin_inff();
+                        });
             if (in && half == 0) out[col] = v;
-            if (__any(at >= 0)) {
+            if (__any(label >= 0)) {
 #pragma unroll
                 for (int i = 0; i < TMW; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (at == acc_row(i, e, half) && row0 + at < vocab)
-                            picked[col] = SCALED ? acc[i][j][e] * sc : acc[i][j][e];
+                        if (label == acc_row(i, e, half) && label < left) picked[col] = z[i][e];
             }
         }
     }
