@@ -93,7 +93,7 @@ def host_library(name: str, sources: list[str], compiler: str = "g++") -> str:
 # beyond the HIP runtime).
 KERNEL_SOURCES = ["rmsnorm.hip", "gemm.hip", "gemm_ring_n.hip", "gemm_ring_t.hip", "gemm_f32.hip",
                   "rowops.hip", "bcast.hip", "layernorm.hip", "xent.hip", "xent_lse.hip",
-                  "xent_grad.hip", "xent_dx.hip", "xent_dw.hip", "distill.hip"]
+                  "xent_grad.hip", "xent_dx.hip", "xent_dw.hip", "xent_f32.hip", "distill.hip"]
 KERNEL_LIBS: list[str] = []
 # The benchmark's own measurement probes (csrc/agk_bench.h): loaded by bench.py
 # only, not part of the product ABI.

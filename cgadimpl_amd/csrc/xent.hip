@@ -15,7 +15,8 @@
 //
 // fp32.  The same kernels on operands split into two fp16 planes (PlanesK), x once a call
 // and w a piece at a time; in the backward, whose products sum along every index, after a pass
-// over them for their largest values.  G leaves its kernel split.
+// over them for their largest values.  G leaves its kernel split.  Few tokens, whose time is the
+// traffic of w, take the fp32 instruction instead (xent_f32.hip).
 //
 // A token that is left out (a negative label, or a zero dloss) has a zero row of G
 // whatever its logits are, and the product over tokens reads its row of x as zeros,
@@ -260,22 +261,28 @@ __global__ __launch_bounds__(256) void xent_split(const Matrices a, const float*
 // The first workgroup: weight[t] = dloss[t] / alpha for a token with a label, 0 for one
 // without, NaN for one whose label is past the vocabulary; zeros to padded.  alpha: the
 // largest finite |dloss| of the tokens with a label (1 where that is 0).
-// The others (bf16): a token's row each, dst[t] = x[t], or zeros for one that is left out.
+// The others: a token's row each, dst[t] = x[t], or zeros for one that is left out.
+template <class T>
 __global__ __launch_bounds__(1024) void xent_tokens(const float* __restrict__ dloss,
                                                     const int64_t* __restrict__ labels,
                                                     float* __restrict__ weight,
                                                     Scalars* __restrict__ sc, int64_t tokens,
                                                     int64_t padded, int64_t vocab,
-                                                    const uint16_t* __restrict__ x, int64_t ldx,
-                                                    uint16_t* __restrict__ dst, int cols) {
+                                                    const T* __restrict__ x, int64_t ldx,
+                                                    T* __restrict__ dst, int cols) {
     if (blockIdx.x > 0) {
         for (int64_t t = (static_cast<int64_t>(blockIdx.x) - 1) * 4 + (threadIdx.x >> 8);
              t < tokens; t += (static_cast<int64_t>(gridDim.x) - 1) * 4) {
             const bool keep = labels[t] >= 0 && dloss[t] != 0.0f;
-            const agk::u32x4* const from = reinterpret_cast<const agk::u32x4*>(x + t * ldx);
-            agk::u32x4* const to = reinterpret_cast<agk::u32x4*>(dst + t * cols);
-            for (int c = static_cast<int>(threadIdx.x & 255); c < cols / 8; c += 256)
-                to[c] = keep ? from[c] : agk::u32x4{0u, 0u, 0u, 0u};
+            if constexpr (sizeof(T) == 2) {
+                const agk::u32x4* const from = reinterpret_cast<const agk::u32x4*>(x + t * ldx);
+                agk::u32x4* const to = reinterpret_cast<agk::u32x4*>(dst + t * cols);
+                for (int c = static_cast<int>(threadIdx.x & 255); c < cols / 8; c += 256)
+                    to[c] = keep ? from[c] : agk::u32x4{0u, 0u, 0u, 0u};
+            } else {
+                for (int c = static_cast<int>(threadIdx.x & 255); c < cols; c += 256)
+                    dst[t * cols + c] = keep ? x[t * ldx + c] : 0.0f;
+            }
         }
         return;
     }
@@ -505,6 +512,22 @@ inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
     return d;
 }
 
+// fp32 of few tokens on the fp32 instruction, which reads w as it lies (its 32-row blocks are what
+// max_blocks counts for kFewTokens and less; its k-strided loads take four columns).  Forward /
+// backward on MI355X, us, planes / this: 16 tokens x 2048 x 32000 203, 389 / 63, 237; 64 x 1024 x
+// 32000 92, 210 / 46, 155; 128 x 1024 x 20000 73, 179 / 59, 172; 129 x 1024 x 32000 106, 302 / 110, 330.
+inline bool on_instruction(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
+    return dtype == AGK_F32 && rows <= kFewTokens && cols >= 4 && vocab <= 1LL << 28;
+}
+// dx's slices there: two workgroups per CU, each slice with 256 k at least.
+inline DxPlan dx_plan32(int64_t rows8, int64_t cols, int64_t k) {
+    const int64_t tiles = rows8 <= 32 ? (cols + 127) / 128 : (rows8 + 63) / 64 * ((cols + 63) / 64);
+    const int64_t n = std::max<int64_t>(
+        std::min<int64_t>({2 * agk_gemm::device_cus() / tiles, k / 256, 64}), 1);
+    const int64_t ks = up((k + n - 1) / n, 32);
+    return DxPlan{0, static_cast<int>((k + ks - 1) / ks), static_cast<int>(ks)};
+}
+
 // The workspaces.  `cols` of the operands as staged: kp for planes (whole k-tiles).
 struct FwdLayout {
     int64_t kp, piece;
@@ -512,19 +535,20 @@ struct FwdLayout {
 };
 inline FwdLayout fwd_layout(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
     FwdLayout o;
-    const bool bf16 = dtype == AGK_BF16;
+    const bool whole = dtype == AGK_BF16 || on_instruction(rows, vocab, cols, dtype);
     o.kp = up(cols, 64);
-    o.piece = bf16 ? vocab : piece_rows(vocab, 64, o.kp, 2, 0);
+    o.piece = whole ? vocab : piece_rows(vocab, 64, o.kp, 2, 0);
     o.scales = 0;  // x's and w's; a wave's block of up to 128 rows can pass the last one
-    o.picked = o.scales + (bf16 ? 0 : region((up(rows, 64) + o.piece + 128) * 4));
+    o.picked = o.scales + (whole ? 0 : region((up(rows, 64) + o.piece + 128) * 4));
     o.part = o.picked + region(rows * 4);
     o.x2 = o.part + region(max_blocks(rows, vocab, o.piece) * rows * 8);
-    o.w2 = o.x2 + (bf16 ? 0 : region(rows * o.kp * 4));
-    o.total = o.w2 + (bf16 ? 0 : region(o.piece * o.kp * 4));
+    o.w2 = o.x2 + (whole ? 0 : region(rows * o.kp * 4));
+    o.total = o.w2 + (whole ? 0 : region(o.piece * o.kp * 4));
     return o;
 }
 
 struct BwdLayout {
+    bool instr;  // on_instruction
     int planes;
     int64_t piece, padded;             // vocabulary rows of a piece, and of its operands
     int64_t rows8, rows64, ldg, kp, cols8;
@@ -535,21 +559,23 @@ inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t l
                             int64_t piece) {
     BwdLayout o;
     const bool bf16 = dtype == AGK_BF16;
+    o.instr = on_instruction(rows, vocab, cols, dtype);
     o.planes = bf16 ? 1 : 2;
     o.rows8 = up(rows, 8);
     o.rows64 = up(rows, 64);
-    o.ldg = up(rows, kLine);
+    o.ldg = o.instr ? up(rows, 32) : up(rows, kLine);
     o.kp = up(cols, 64);
     o.cols8 = up(cols, 8);
     o.piece = piece_rows(vocab, o.ldg, bf16 ? ldw : o.kp, o.planes, piece);
-    o.padded = bf16 ? o.piece : up(o.piece, 64);
-    o.dx = dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : PlanesK::kWalks);
+    o.padded = bf16 || o.instr ? o.piece : up(o.piece, 64);
+    o.dx = o.instr ? dx_plan32(o.rows8, cols, o.piece)
+                   : dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : PlanesK::kWalks);
     o.weight = 0;
     o.scalars = o.weight + region(o.rows8 * 4);
     o.parts = o.scalars + region(sizeof(Scalars));
     o.x = o.parts + (bf16 ? 0 : region(2 * kMaxParts * 4));
     o.w2 = o.x + region(bf16 ? rows * cols * 2 : o.rows64 * o.kp * 4);
-    o.g = o.w2 + (bf16 ? 0 : region(o.padded * o.kp * 4));
+    o.g = o.w2 + (bf16 || o.instr ? 0 : region(o.padded * o.kp * 4));
     o.acc = o.g + region(o.padded * o.ldg * 2 * o.planes);
     o.total = o.acc + region(static_cast<int64_t>(o.dx.slices) * o.rows8 * o.cols8 * 4);
     return o;
@@ -654,6 +680,15 @@ int agk_linear_xent_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     float* const w_scales = x_scales + up(rows, 64);
     const bool bf16 = dtype == AGK_BF16;
     const int m = static_cast<int>(rows), kp = static_cast<int>(o.kp);
+    if (on_instruction(rows, vocab, cols, dtype)) {
+        const int nv = static_cast<int>(vocab);
+        rc = launch_lse(ProductF32{static_cast<const float*>(w), ldw, static_cast<const float*>(x),
+                                   ldx, nv, m, static_cast<int>(cols), 1, 0, st},
+                        LseEpi<false>{part, picked, labels, 0, nv, m, nullptr, nullptr});
+        if (rc != AGK_OK) return rc;
+        return launch_join(part, (vocab + 31) / 32, picked, labels, loss,
+                           reinterpret_cast<float2*>(stats), rows, vocab, st);
+    }
     int64_t blocks = 0;
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
@@ -750,15 +785,41 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const int c1 = static_cast<int>(cols), c8 = static_cast<int>(o.cols8);
     const int cus = agk_gemm::device_cus();
     const int64_t slice = o.rows8 * o.cols8;
-    const int64_t copied = bf16 && dw ? rows : 0;
+    const int64_t copied = (bf16 || o.instr) && dw ? rows : 0;
     const dim3 grid(1 + agk::capped_blocks((copied + 3) / 4, 1 << 20)), block(1024);
-    hipLaunchKernelGGL(xent_tokens, grid, block, 0, st, dloss, labels, weight, sc, rows, o.rows8,
-                       vocab, static_cast<const uint16_t*>(x), ldx, xk, c1);
+    if (bf16)
+        hipLaunchKernelGGL(xent_tokens<uint16_t>, grid, block, 0, st, dloss, labels, weight, sc,
+                           rows, o.rows8, vocab, static_cast<const uint16_t*>(x), ldx, xk, c1);
+    else
+        hipLaunchKernelGGL(xent_tokens<float>, grid, block, 0, st, dloss, labels, weight, sc, rows,
+                           o.rows8, vocab, static_cast<const float*>(x), ldx,
+                           reinterpret_cast<float*>(xk), c1);
     if ((rc = check_launch()) != AGK_OK) return rc;
     int x_parts = 0;
     for (int64_t v0 = 0; v0 < vocab; v0 += o.piece) {
         const int64_t n = std::min(o.piece, vocab - v0);
         const int nv = static_cast<int>(n), np = static_cast<int>(bf16 ? n : up(n, 64));
+        if (o.instr) {
+            const float* const wp = static_cast<const float*>(w) + v0 * ldw;
+            float* const g32 = reinterpret_cast<float*>(g);
+            const float* const x0 = reinterpret_cast<const float*>(xk);
+            rc = launch_grad(ProductF32{wp, ldw, static_cast<const float*>(x), ldx, nv, m, c1, 1, 0,
+                                        st},
+                             GradEpiF32{g32, in, weight, labels, v0, ldg, nv, m});
+            if (rc != AGK_OK) return rc;
+            // the last piece is shorter: fewer slices, which the others' sums are left in
+            const int slices = static_cast<int>((n + o.dx.k_slice - 1) / o.dx.k_slice);
+            if (dx)
+                rc = launch_dx(ProductF32{g32, ldg, wp, ldw, m8, c1, nv, slices, o.dx.k_slice, st},
+                               AddEpi<true>{acc, c8, slice, nullptr, m8, c1, v0 > 0});
+            if (rc != AGK_OK) return rc;
+            if (dw)
+                rc = launch_dw(ProductF32{g32, ldg, x0, cols, nv, c1, m, 1, 0, st},
+                               AddEpi<true>{static_cast<float*>(dw) + v0 * cols, cols, 0,
+                                            &sc->alpha, nv, c1, acc_dw});
+            if (rc != AGK_OK) return rc;
+            continue;
+        }
         const DxPlan d = n == o.piece ? o.dx : last_piece(o.dx, np);
         const AddEpi<true> de{acc, c8, slice, bf16 ? nullptr : &sc->dx, m8, c8, v0 > 0};
         char* const out = static_cast<char*>(dw) + v0 * cols * dw_size;

@@ -303,6 +303,43 @@ struct GradEpi {
     }
 };
 
+// The same in fp32, from logits in fp32: rows of ldg tokens, zeros from `tokens` on.
+struct GradEpiF32 {
+    float* G;
+    const float2* stats;
+    const float* weight;
+    const int64_t* labels;
+    int64_t v0;
+    int ldg, rows, tokens;
+
+    template <int TMW, int TNW>
+    __device__ __forceinline__ void operator()(const f32x16 (&acc)[TMW][TNW], int row0, int col0,
+                                               int lane) const {
+        const int half = lane >> 5;
+#pragma unroll
+        for (int j = 0; j < TNW; ++j) {
+            const int col = col0 + j * 32 + (lane & 31);
+            if (col >= ldg) continue;
+            const bool in = col < tokens;
+            const float2 st = in ? stats[col] : make_float2(0.0f, 0.0f);
+            const float w = in ? weight[col] : 0.0f;
+            const int at = in ? label_row(labels[col], v0 + row0, TMW * 32) : -1;
+            const float shift = st.y * kLog2e;
+#pragma unroll
+            for (int i = 0; i < TMW; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int r = acc_row(i, e, half);
+                    float p = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(acc[i][j][e] - st.x, kLog2e, -shift));
+                    p -= at == r ? 1.0f : 0.0f;
+                    if (row0 + r < rows)
+                        G[static_cast<int64_t>(row0 + r) * ldg + col] = w != 0.0f ? w * p : 0.0f;
+                }
+        }
+    }
+};
+
 // C (+)= alpha * product (alpha NULL: 1), that in fp32 and rounded to C's type once.  The
 // old values of a 32-row group are loaded together: one wait for 16 TNW loads.  A bf16 C that
 // is not added to is stored 4 bytes at a time, as G is (ldc and N are even there): dw of 4099
@@ -396,6 +433,21 @@ struct Product {
     int M, N, K, slices, k_slice;
     hipStream_t st;
 };
+
+// The same of fp32 operands as they lie (xent_f32.hip); a k-strided one has at least four rows.
+struct ProductF32 {
+    const float* A;
+    int64_t lda;
+    const float* B;
+    int64_t ldb;
+    int M, N, K, slices, k_slice;
+    hipStream_t st;
+};
+
+int launch_lse(const ProductF32& p, const LseEpi<false>& e);
+int launch_grad(const ProductF32& p, const GradEpiF32& e);
+int launch_dx(const ProductF32& p, const AddEpi<true>& e);
+int launch_dw(const ProductF32& p, const AddEpi<true>& e);
 
 // bf16 operands, and fp32 ones as planes (their leading dimension: two planes' worth).
 int launch_lse(int shape, const Product& p, const LseEpi<false>& e);

@@ -35,11 +35,12 @@ extern "C" {
  * [rows][2] fp32, 8-byte aligned, receives m and l, which the backward reads.
  * z exists in pieces only: bf16 products leave the matrix cores as the maximum
  * and sum of exponentials of each token's logits over a few vocabulary rows, in
- * fp32 and unrounded.  fp32 operands are multiplied as two fp16 halves each (in
- * the workspace, a piece of the vocabulary at a time), scaled by a power of two:
- * a product is off by at most 12 * 2^-24 of itself, less than the fp32 sum of
- * the row's products is.  Values below 2^-28 of their matrix's largest finite one
- * (x's: over the rows with a label) are held to 2^-39 of that one.
+ * fp32 and unrounded.  fp32 operands of more than 128 rows are multiplied as two
+ * fp16 halves each (in the workspace, a piece of the vocabulary at a time), scaled
+ * by a power of two: a product is off by at most 12 * 2^-24 of itself, less than
+ * the fp32 sum of the row's products is.  Values below 2^-28 of the largest finite
+ * one of their row (backward: of their matrix, x's over the rows that are not left
+ * out) are held to 2^-39 of that one.
  * A logit of 2.3e38 and more makes its row's loss NaN.  The stats of a row whose
  * label is negative hold nothing of use.
  * bf16: x and w 16-byte aligned, cols, ldx and ldw multiples of 8 (as

@@ -367,9 +367,10 @@ def test_gradients_against_differences(cuda):
         assert abs(terms.sum() - want) <= 1e-5 * terms.abs().sum(), (i, terms.sum(), want)
 
 
-def test_left_out_rows_do_not_set_the_scale(cuda):
+@pytest.mark.parametrize("N", [70, 170])
+def test_left_out_rows_do_not_set_the_scale(cuda, N):
     # the fp32 operands are scaled by their matrix's largest value: rows without a loss have no part
-    x, w, labels, dloss = inputs(70, 300, 33, F, seed=21)
+    x, w, labels, dloss = inputs(N, 300, 33, F, seed=21)
     labels[::7] = -1
     dirty = torch.where((labels < 0)[:, None], 1e30, x)
     out = agk.linear_cross_entropy_fwd(dirty, w, labels)
@@ -383,9 +384,10 @@ def test_left_out_rows_do_not_set_the_scale(cuda):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N", [40, 150])
 @pytest.mark.parametrize("ex,ew", [(0, -101), (0, -99), (-101, 0), (-60, -60), (30, -101), (60, -60)])
-def test_scales_of_any_size(cuda, ex, ew):
-    x, w, labels, dloss = inputs(40, 200, 29, F, seed=22)
+def test_scales_of_any_size(cuda, N, ex, ew):
+    x, w, labels, dloss = inputs(N, 200, 29, F, seed=22)
     x, w = x * 2.0 ** ex, w * 2.0 ** ew
     loss, stats = agk.linear_cross_entropy_fwd(x, w, labels)
     dx, dw = agk.linear_cross_entropy_bwd(x, w, labels, stats, dloss)
@@ -420,3 +422,46 @@ def test_few_tokens_of_many_words(cuda, N, V, D, pitch):
     ref, bound = reference(x, w, labels, dloss)
     for got, want, tol, what in zip((loss, dx, dw), ref, bound, ("loss", "dx", "dw")):
         check(got, want, tol, (what, N, V, D))
+
+
+def test_rows_of_unlike_sizes(cuda):
+    # fp32 forward: each row and each word has a scale of its own, so large ones cost others nothing
+    x, w, labels, _ = inputs(150, 900, 61, F, seed=24, ignored=0.0)
+    x, w = x.clone(), w.clone()
+    x[::5] *= 2.0 ** -30
+    w[::7] *= 2.0 ** 20
+    x[:, 0] = 0.0                      # words of 2^20 meet tokens of 2^-30 in most columns
+    x[1::2] *= 2.0 ** -22
+    (want,), (bound,) = reference(x, w, labels, None)
+    # the products' own error, by rows instead of by matrices
+    a, b = x.double().abs(), w.double().abs()
+    low = 2.0 ** -38 * (a.amax(1, keepdim=True) * b.sum(1) + a.sum(1, keepdim=True) * b.amax(1))
+    z = a @ b.T
+    dz = ((x.shape[1] + 2 + 12) * U * z + low).amax(1)
+    zz = x.double() @ w.double().T
+    m = zz.amax(1)
+    l = torch.logsumexp(zz, 1) - m
+    tight = 2 * dz + (168 + 900 / 2048) * U + 4 * U * (m.abs() + l.abs() + want.abs())
+    got = agk.linear_cross_entropy_fwd(x, w, labels)[0]
+    check(got, want, tight, "loss")
+
+
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("N", [1, 31, 33, 128, 129])
+@pytest.mark.parametrize("piece", [1, 512, 0])
+def test_few_tokens_in_pieces(cuda, dtype, N, piece):
+    V, D = 1700, 72 if dtype == BF else 71
+    x, w, labels, dloss = inputs(N, V, D, dtype, seed=25)
+    loss, stats = agk.linear_cross_entropy_fwd(x, w, labels)
+    dx0 = torch.randn(N, D, device="cuda").to(dtype)
+    dw0 = torch.randn(V, D, device="cuda")
+    dx, dw = dx0.clone(), dw0.clone()
+    agk.linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=dx, dw=dw, accumulate=True,
+                                 piece=piece)
+    new = agk.linear_cross_entropy_bwd(x, w, labels, stats, dloss, piece=piece)
+    ref, bound = reference(x, w, labels, dloss)
+    for got, added, base, want, tol, what in zip(new, (dx, dw), (dx0, dw0), ref[1:], bound[1:],
+                                                 ("dx", "dw")):
+        check(got, want, tol, what)
+        r = R[got.dtype]
+        check(added, base.double() + want, tol + r * (base.double() + want).abs() + 2 * r * tol, what)
