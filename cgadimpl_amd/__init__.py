@@ -9,7 +9,6 @@ is no Python or CPU fallback: if the library is missing, every call raises.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 from typing import Optional, Tuple
 
@@ -829,43 +828,61 @@ def logsumexp_jvp(z, tz, ty=None, stream=None):
 
 
 # ---- LayerNorm with weight and bias (include/agk_rowops.h) ------------------------
+# A small call is mostly this binding's host time, 8-11 us on MI355X's host with the launch's
+# 3.2 and 1.2 per allocation, so each tensor is looked at once.
 
-def _want(t, name, dev, n, dtype):
-    """Checks one operand: n values of `dtype` on device `dev` (_ptr checks that it is contiguous)."""
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.numel() != n:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {n} values")
-    if t.get_device() != dev:
-        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{dev}")
+_current_device = None    # set by _device_of
+_device_stream = None
 
 
-_current_device = None
-
-
-def _want_current(t) -> int:
+def _device_of(t):
     """The device of t, which has to be the current one: the kernels run on its current stream."""
-    global _current_device
+    global _current_device, _device_stream
     dev = t.get_device()
     if dev < 0:
         raise ValueError("tensor must live on the GPU")
     if _current_device is None:
         torch = _torch()
         torch.cuda.init()
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _device_stream = raw or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
     if dev != _current_device():
         raise ValueError(f"tensors on {t.device} while cuda:{_current_device()} is current")
     return dev
 
 
+def _given(t, name, dev, n, dtype) -> int:
+    """The address of one operand: n contiguous values of `dtype` on device `dev`."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.numel() != n:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {n} values")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{dev}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous (row-major)")
+    return t.data_ptr()
+
+
 def _scratch(workspace, need, like):
-    """(workspace, bytes): the caller's tensor, or what the call needs."""
+    """(tensor to hold until the call returns, address, bytes): the caller's workspace, or what
+    the call needs."""
     if workspace is None:
-        workspace = _empty((need,), _torch().uint8, like) if need else None
-        return workspace, need
+        if not need:
+            return None, None, 0
+        workspace = _empty((need,), _torch().uint8, like)
+        return workspace, workspace.data_ptr(), need
     if workspace.device != like.device:
         raise ValueError("the workspace is on another device")
-    return workspace, workspace.numel() * workspace.element_size()
+    return workspace, _ptr(workspace), workspace.numel() * workspace.element_size()
+
+
+def _on(stream, call, *args):
+    """`call` with `stream` current, so that what it allocates (its workspace goes back to the
+    allocator as it returns) and clears is ordered on the stream that its kernels use."""
+    with _torch().cuda.stream(stream):
+        return call(*args)
 
 
 def _row_column(x, rows):
@@ -874,215 +891,225 @@ def _row_column(x, rows):
     return _empty(shape, _torch().float32, x)
 
 
-def _on_stream(call):
-    """`call` with the keyword `stream` (None: the current one).  The call runs with that stream
-    current, so that what it allocates (its workspace goes back to the allocator as it returns)
-    and clears is ordered on the stream that its kernels use."""
-    @functools.wraps(call)
-    def on(*args, stream=None, **kwargs):
-        if stream is None:
-            return call(*args, **kwargs)
-        with _torch().cuda.stream(stream):
-            return call(*args, **kwargs)
-    return on
-
-
-@_on_stream
-def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None):
+def layernorm_affine_fwd(x, gamma, beta, eps: float = 1e-5, y=None, mean=None, rstd=None,
+                         stream=None):
     """y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis (gamma, beta: [cols] of
     x's dtype, or None); returns (y, mean, rstd), the statistics float32 [..., 1]."""
+    if stream is not None:
+        return _on(stream, layernorm_affine_fwd, x, gamma, beta, eps, y, mean, rstd)
     torch = _torch()
-    dev = _want_current(x)
+    dev = _device_of(x)
     rows, cols = _rows_cols(x)
-    if gamma is not None:
-        _want(gamma, "gamma", dev, cols, x.dtype)
-    if beta is not None:
-        _want(beta, "beta", dev, cols, x.dtype)
+    dtype, f32 = x.dtype, torch.float32
+    px = _given(x, "x", dev, rows * cols, dtype)
+    pg = None if gamma is None else _given(gamma, "gamma", dev, cols, dtype)
+    pb = None if beta is None else _given(beta, "beta", dev, cols, dtype)
     if y is None:
         y = torch.empty_like(x)
+        py = y.data_ptr()
     else:
-        _want(y, "y", dev, x.numel(), x.dtype)
+        py = _given(y, "y", dev, rows * cols, dtype)
     if mean is None:
         mean = _row_column(x, rows)
+        pm = mean.data_ptr()
     else:
-        _want(mean, "mean", dev, rows, torch.float32)
+        pm = _given(mean, "mean", dev, rows, f32)
     if rstd is None:
         rstd = _row_column(x, rows)
+        pr = rstd.data_ptr()
     else:
-        _want(rstd, "rstd", dev, rows, torch.float32)
-    rc = lib().agk_layernorm_affine_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean),
-                                        _ptr(rstd), rows, cols, float(eps), _dtype_code(x),
-                                        _stream(None))
+        pr = _given(rstd, "rstd", dev, rows, f32)
+    rc = lib().agk_layernorm_affine_fwd(px, pg, pb, py, pm, pr, rows, cols, eps, _dtype_code(x),
+                                        _device_stream(dev))
     _check(rc, "agk_layernorm_affine_fwd")
     return y, mean, rstd
 
 
-@_on_stream
 def layernorm_affine_bwd(x, gamma, mean, rstd, dy, dx=None, dgamma=None, dbeta=None,
                          accumulate=False, want_dx: bool = True, want_dgamma: bool = True,
-                         want_dbeta: bool = True, workspace=None):
+                         want_dbeta: bool = True, workspace=None, stream=None):
     """VJP of layernorm_affine_fwd: (dx, dgamma, dbeta), None where not wanted; dgamma and dbeta
     float32 [cols].  accumulate: a bool (every output) or AGK_ACCUM_DX / _DGAMMA / _DBETA bits."""
+    if stream is not None:
+        return _on(stream, layernorm_affine_bwd, x, gamma, mean, rstd, dy, dx, dgamma, dbeta,
+                   accumulate, want_dx, want_dgamma, want_dbeta, workspace)
     torch = _torch()
-    dev = _want_current(x)
+    dev = _device_of(x)
     rows, cols = _rows_cols(x)
+    dtype, f32 = x.dtype, torch.float32
     acc = (7 if accumulate else 0) if isinstance(accumulate, bool) else int(accumulate)
-    _want(dy, "dy", dev, x.numel(), x.dtype)
-    _want(mean, "mean", dev, rows, torch.float32)
-    _want(rstd, "rstd", dev, rows, torch.float32)
-    if gamma is not None:
-        _want(gamma, "gamma", dev, cols, x.dtype)
+    px = _given(x, "x", dev, rows * cols, dtype)
+    pdy = _given(dy, "dy", dev, rows * cols, dtype)
+    pm = _given(mean, "mean", dev, rows, f32)
+    pr = _given(rstd, "rstd", dev, rows, f32)
+    pg = None if gamma is None else _given(gamma, "gamma", dev, cols, dtype)
+    pdx = pdg = pdb = None
     if dx is not None:
-        _want(dx, "dx", dev, x.numel(), x.dtype)
+        pdx = _given(dx, "dx", dev, rows * cols, dtype)
     elif want_dx:
         dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
+        pdx = dx.data_ptr()
     if dgamma is not None:
-        _want(dgamma, "dgamma", dev, cols, torch.float32)
+        pdg = _given(dgamma, "dgamma", dev, cols, f32)
     elif want_dgamma:
-        dgamma = _empty((cols,), torch.float32, x)
+        dgamma = _empty((cols,), f32, x)
+        pdg = dgamma.data_ptr()
         if acc & AGK_ACCUM_DGAMMA:
             dgamma.zero_()
     if dbeta is not None:
-        _want(dbeta, "dbeta", dev, cols, torch.float32)
+        pdb = _given(dbeta, "dbeta", dev, cols, f32)
     elif want_dbeta:
-        dbeta = _empty((cols,), torch.float32, x)
+        dbeta = _empty((cols,), f32, x)
+        pdb = dbeta.data_ptr()
         if acc & AGK_ACCUM_DBETA:
             dbeta.zero_()
     need = 0
     if dgamma is not None or dbeta is not None:
         need = lib().agk_layernorm_affine_bwd_workspace_bytes(rows, cols)
-    ws, ws_bytes = _scratch(workspace, need, x)
-    rc = lib().agk_layernorm_affine_bwd(_ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dy),
-                                        _ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(ws), ws_bytes,
-                                        rows, cols, _dtype_code(x), acc, _stream(None))
+    held, ws, ws_bytes = _scratch(workspace, need, x)
+    rc = lib().agk_layernorm_affine_bwd(px, pg, pm, pr, pdy, pdx, pdg, pdb, ws, ws_bytes, rows, cols,
+                                        _dtype_code(x), acc, _device_stream(dev))
     _check(rc, "agk_layernorm_affine_bwd")
     return dx, dgamma, dbeta
 
 
 # ---- losses (include/agk_losses.h) --------------------------------------------------
 
-def _xent_sizes(x, w, labels):
-    dev = _want_current(x)
-    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1]:
+def _xent_operands(x, w, labels):
+    """(device, rows, vocab, cols, addresses of x, w and labels)."""
+    dev = _device_of(x)
+    xs, ws = x.shape, w.shape
+    if len(xs) < 1 or len(ws) != 2 or ws[1] != xs[-1]:
         raise ValueError("expected x [..., cols] and w [vocab, cols]")
-    if labels.shape != x.shape[:-1]:
+    if labels.shape != xs[:-1]:
         raise ValueError("expected one label for each row of x")
-    rows, cols = labels.numel(), x.shape[-1]
-    _want(w, "w", dev, w.numel(), x.dtype)
-    _want(labels, "labels", dev, rows, _torch().int64)
-    return dev, rows, w.shape[0], cols
+    rows, (vocab, cols) = labels.numel(), ws
+    px = _given(x, "x", dev, rows * cols, x.dtype)
+    pw = _given(w, "w", dev, vocab * cols, x.dtype)
+    return dev, rows, vocab, cols, px, pw, _given(labels, "labels", dev, rows, _torch().int64)
 
 
 def _loss_and_stats(shape, rows, dev, like, loss, stats):
+    """(loss, stats, their addresses)."""
     f32 = _torch().float32
     if loss is None:
         loss = _empty(shape, f32, like)
+        pl = loss.data_ptr()
     else:
-        _want(loss, "loss", dev, rows, f32)
+        pl = _given(loss, "loss", dev, rows, f32)
     if stats is None:
         stats = _empty(shape + (2,), f32, like)
+        ps = stats.data_ptr()
     else:
-        _want(stats, "stats", dev, 2 * rows, f32)
-    return loss, stats
+        ps = _given(stats, "stats", dev, 2 * rows, f32)
+    return loss, stats, pl, ps
 
 
-@_on_stream
-def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None):
+def linear_cross_entropy_fwd(x, w, labels, loss=None, stats=None, workspace=None, stream=None):
     """The softmax cross entropy of z = x @ w.T against labels, without z in memory
     (agk_linear_xent_fwd): x [..., cols], w [vocab, cols], labels int64 [...]; a negative label is
     a row without a loss.  Returns (loss, stats): float32 [...] and [..., 2] (each row's maximum
     logit and log of its sum of exponentials above it, for the backward)."""
-    torch = _torch()
-    dev, rows, vocab, cols = _xent_sizes(x, w, labels)
-    loss, stats = _loss_and_stats(labels.shape, rows, dev, x, loss, stats)
+    if stream is not None:
+        return _on(stream, linear_cross_entropy_fwd, x, w, labels, loss, stats, workspace)
+    dev, rows, vocab, cols, px, pw, pl = _xent_operands(x, w, labels)
+    loss, stats, ploss, pstats = _loss_and_stats(labels.shape, rows, dev, x, loss, stats)
     dt = _dtype_code(x)
-    ws, ws_bytes = _scratch(workspace, lib().agk_linear_xent_fwd_workspace_bytes(
-        rows, vocab, cols, dt), x)
-    rc = lib().agk_linear_xent_fwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(loss),
-                                   _ptr(stats), _ptr(ws), ws_bytes, rows, vocab, cols, dt,
-                                   _stream(None))
+    held, ws, ws_bytes = _scratch(
+        workspace, lib().agk_linear_xent_fwd_workspace_bytes(rows, vocab, cols, dt), x)
+    rc = lib().agk_linear_xent_fwd(px, cols, pw, cols, pl, ploss, pstats, ws, ws_bytes, rows, vocab,
+                                   cols, dt, _device_stream(dev))
     _check(rc, "agk_linear_xent_fwd")
     return loss, stats
 
 
-@_on_stream
 def linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=None, dw=None, dw_dtype=None,
                              accumulate=False, want_dx: bool = True, want_dw: bool = True,
-                             piece: int = 0, workspace=None):
+                             piece: int = 0, workspace=None, stream=None):
     """Gradients of linear_cross_entropy_fwd for dloss, the float32 gradient of each row's loss
     (agk_linear_xent_bwd): (dx, dw), None where not wanted.  dw is float32 unless dw_dtype (or
     dw) says otherwise.  accumulate: a bool (both) or AGK_ACCUM_DX / AGK_ACCUM_DGAMMA (dw) bits.
     piece: vocabulary rows whose logits exist at a time (0: the library's choice)."""
+    if stream is not None:
+        return _on(stream, linear_cross_entropy_bwd, x, w, labels, stats, dloss, dx, dw, dw_dtype,
+                   accumulate, want_dx, want_dw, piece, workspace)
     torch = _torch()
-    dev, rows, vocab, cols = _xent_sizes(x, w, labels)
+    dev, rows, vocab, cols, px, pw, pl = _xent_operands(x, w, labels)
     acc = _accum_flags(accumulate)
-    _want(stats, "stats", dev, 2 * rows, torch.float32)
-    _want(dloss, "dloss", dev, rows, torch.float32)
+    pstats = _given(stats, "stats", dev, 2 * rows, torch.float32)
+    pdloss = _given(dloss, "dloss", dev, rows, torch.float32)
+    pdx = pdw = None
     if dx is not None:
-        _want(dx, "dx", dev, x.numel(), x.dtype)
+        pdx = _given(dx, "dx", dev, rows * cols, x.dtype)
     elif want_dx:
         dx = torch.zeros_like(x) if acc & AGK_ACCUM_DX else torch.empty_like(x)
+        pdx = dx.data_ptr()
     if dw is not None:
-        _want(dw, "dw", dev, w.numel(), dw_dtype or dw.dtype)
+        pdw = _given(dw, "dw", dev, vocab * cols, dw_dtype or dw.dtype)
     elif want_dw:
         new = torch.zeros if acc & AGK_ACCUM_DGAMMA else torch.empty
         dw = new(vocab, cols, dtype=dw_dtype or torch.float32, device=x.device)
+        pdw = dw.data_ptr()
     dt = _dtype_code(x)
-    ws, ws_bytes = _scratch(workspace, lib().agk_linear_xent_bwd_workspace_bytes(
-        rows, vocab, cols, dt, piece), x)
-    rc = lib().agk_linear_xent_bwd(_ptr(x), cols, _ptr(w), cols, _ptr(labels), _ptr(stats),
-                                   _ptr(dloss), _ptr(dx), _ptr(dw),
-                                   _dtype_code(dw) if dw is not None else AGK_F32, _ptr(ws),
-                                   ws_bytes, rows, vocab, cols, piece, dt, acc, _stream(None))
+    held, ws, ws_bytes = _scratch(
+        workspace, lib().agk_linear_xent_bwd_workspace_bytes(rows, vocab, cols, dt, piece), x)
+    rc = lib().agk_linear_xent_bwd(px, cols, pw, cols, pl, pstats, pdloss, pdx, pdw,
+                                   _dtype_code(dw) if dw is not None else AGK_F32, ws, ws_bytes,
+                                   rows, vocab, cols, piece, dt, acc, _device_stream(dev))
     _check(rc, "agk_linear_xent_bwd")
     return dx, dw
 
 
-def _distill_sizes(z, index, teacher):
-    dev = _want_current(z)
+def _distill_operands(z, index, teacher):
+    """(device, rows, cols, k, addresses of z, index and teacher)."""
+    dev = _device_of(z)
     zs, shape = z.shape, index.shape
     if len(zs) < 1 or len(shape) != len(zs) or shape[:-1] != zs[:-1] or teacher.shape != shape:
         raise ValueError("expected z [..., cols], index [..., k] and teacher [..., k]")
-    cols, k, n = zs[-1], shape[-1], index.numel()
-    rows = z.numel() // cols if cols else zs[:-1].numel()
-    _want(index, "index", dev, n, _torch().int64)
-    _want(teacher, "teacher", dev, n, teacher.dtype)
-    return dev, rows, cols, k
+    cols, k, n, total = zs[-1], shape[-1], index.numel(), z.numel()
+    rows = total // cols if cols else zs[:-1].numel()
+    pz = _given(z, "z", dev, total, z.dtype)
+    pi = _given(index, "index", dev, n, _torch().int64)
+    return dev, rows, cols, k, pz, pi, _given(teacher, "teacher", dev, n, teacher.dtype)
 
 
-@_on_stream
 def distill_topk_fwd(z, index, teacher, temperature: float = 1.0, loss=None, stats=None,
-                     workspace=None):
+                     workspace=None, stream=None):
     """T^2 KL(p || q) per row of q = softmax(z / T) over all columns from p = softmax(teacher / T)
     over the row's k named columns (agk_distill_topk_fwd): z [..., cols], index int64 [..., k] (a
     negative one is an empty entry), teacher [..., k] float32 or bfloat16.  Returns (loss, stats):
     float32 [...] and [..., 2]."""
-    dev, rows, cols, k = _distill_sizes(z, index, teacher)
-    loss, stats = _loss_and_stats(z.shape[:-1], rows, dev, z, loss, stats)
+    if stream is not None:
+        return _on(stream, distill_topk_fwd, z, index, teacher, temperature, loss, stats, workspace)
+    dev, rows, cols, k, pz, pi, pt = _distill_operands(z, index, teacher)
+    loss, stats, pl, ps = _loss_and_stats(z.shape[:-1], rows, dev, z, loss, stats)
     dt = _dtype_code(z)
-    ws, ws_bytes = _scratch(workspace, lib().agk_distill_topk_workspace_bytes(rows, cols, dt), z)
-    rc = lib().agk_distill_topk_fwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(loss), _ptr(stats),
-                                    _ptr(ws), ws_bytes, rows, cols, k, float(temperature), dt,
-                                    _dtype_code(teacher), _stream(None))
+    held, ws, ws_bytes = _scratch(
+        workspace, lib().agk_distill_topk_workspace_bytes(rows, cols, dt), z)
+    rc = lib().agk_distill_topk_fwd(pz, pi, pt, pl, ps, ws, ws_bytes, rows, cols, k, temperature, dt,
+                                    _dtype_code(teacher), _device_stream(dev))
     _check(rc, "agk_distill_topk_fwd")
     return loss, stats
 
 
-@_on_stream
 def distill_topk_bwd(z, index, teacher, stats, dloss, temperature: float = 1.0, dz=None,
-                     accumulate: bool = False):
+                     accumulate: bool = False, stream=None):
     """Gradient of z for dloss, the float32 gradient of each row's loss: dz (+)= dloss * T *
     (q - p at the named columns) (agk_distill_topk_bwd).  dz may be z (in place)."""
+    if stream is not None:
+        return _on(stream, distill_topk_bwd, z, index, teacher, stats, dloss, temperature, dz,
+                   accumulate)
     torch = _torch()
-    dev, rows, cols, k = _distill_sizes(z, index, teacher)
-    _want(stats, "stats", dev, 2 * rows, torch.float32)
-    _want(dloss, "dloss", dev, rows, torch.float32)
+    dev, rows, cols, k, pz, pi, pt = _distill_operands(z, index, teacher)
+    ps = _given(stats, "stats", dev, 2 * rows, torch.float32)
+    pl = _given(dloss, "dloss", dev, rows, torch.float32)
     if dz is None:
         dz = torch.zeros_like(z) if accumulate else torch.empty_like(z)
+        pdz = dz.data_ptr()
     else:
-        _want(dz, "dz", dev, z.numel(), z.dtype)
-    rc = lib().agk_distill_topk_bwd(_ptr(z), _ptr(index), _ptr(teacher), _ptr(stats), _ptr(dloss),
-                                    _ptr(dz), rows, cols, k, float(temperature), _dtype_code(z),
-                                    _dtype_code(teacher), _acc_dx(accumulate), _stream(None))
+        pdz = _given(dz, "dz", dev, rows * cols, z.dtype)
+    rc = lib().agk_distill_topk_bwd(pz, pi, pt, ps, pl, pdz, rows, cols, k, temperature,
+                                    _dtype_code(z), _dtype_code(teacher),
+                                    AGK_ACCUM_DX if accumulate else 0, _device_stream(dev))
     _check(rc, "agk_distill_topk_bwd")
     return dz
