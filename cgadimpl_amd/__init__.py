@@ -249,14 +249,14 @@ def _stream(stream) -> int:
 
 
 def _empty(shape, dtype, like):
-    """A contiguous uninitialised tensor on like's device.  One-dimensional ones (and
-    per-row columns) through empty_strided, whose argument parsing is 0.4 us shorter."""
+    """A contiguous uninitialised tensor on like's device.  Those of one or two dimensions
+    through empty_strided, whose argument parsing is 0.4 us shorter."""
     torch = _torch()
     n = len(shape)
     if n == 1:
         return torch.empty_strided(shape, (1,), dtype=dtype, device=like.device)
-    if n == 2 and shape[1] == 1:
-        return torch.empty_strided(shape, (1, 1), dtype=dtype, device=like.device)
+    if n == 2:
+        return torch.empty_strided(shape, (shape[1] or 1, 1), dtype=dtype, device=like.device)
     return torch.empty(shape, dtype=dtype, device=like.device)
 
 
