@@ -468,9 +468,27 @@ inline int64_t max_blocks(int64_t rows, int64_t vocab, int64_t piece) {
 struct DxPlan {
     int shape, slices, k_slice;
 };
+// The plan for the last piece, of n rows: as many of the slices as leave each a whole k-tile.
+inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
+    DxPlan d = plan;
+    for (;; --d.slices) {
+        d.k_slice = static_cast<int>(up((n + d.slices - 1) / d.slices, 64));
+        d.slices = static_cast<int>((n + d.k_slice - 1) / d.k_slice);
+        if (d.slices == 1 || n - (d.slices - 1) * static_cast<int64_t>(d.k_slice) >= 64) break;
+    }
+    if (n < 64) d.shape = agk_gemm::kRingSmallK;
+    return d;
+}
+
 inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks) {
     using namespace agk_gemm;
     const int64_t cus = device_cus();
+    // Few tokens are bound by the read of w: 64 x 128 tiles, as many slices as give each CU one.
+    // dx alone (with the logits again) on MI355X, us, the cost below / this: 16 x 4096 x 32000 112 /
+    // 103, 64 x 2048 x 50257 104 / 95, 64 x 4096 x 131072 402 / 391; with 256 columns no slices are enough.
+    const int64_t across = (cols + 127) / 128, cuts = cus / across;
+    if (rows8 <= 64 && walks == 1 && cuts >= 1 && cuts <= kMaxSlices && k >= cuts * kMinSlice)
+        return last_piece(DxPlan{7, static_cast<int>(cuts), 0}, k);
     DxPlan best{pick_shape(rows8, cols, k, device_cus()), 1, static_cast<int>(up(k, 64))};
     double best_cost = 1e30;
     for (const RingCost& s : kRingCosts) {
@@ -498,18 +516,6 @@ inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks) {
         }
     }
     return best;
-}
-
-// The plan for the last piece, of n rows: as many of the slices as leave each a whole k-tile.
-inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
-    DxPlan d = plan;
-    for (;; --d.slices) {
-        d.k_slice = static_cast<int>(up((n + d.slices - 1) / d.slices, 64));
-        d.slices = static_cast<int>((n + d.k_slice - 1) / d.k_slice);
-        if (d.slices == 1 || n - (d.slices - 1) * static_cast<int64_t>(d.k_slice) >= 64) break;
-    }
-    if (n < 64) d.shape = agk_gemm::kRingSmallK;
-    return d;
 }
 
 // fp32 of few tokens on the fp32 instruction, which reads w as it lies (its 32-row blocks are what
