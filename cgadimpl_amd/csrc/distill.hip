@@ -8,8 +8,8 @@
 // per lane, the backward reads it once and writes dz.  The teacher's part is a few
 // hundred values a row.  HBM bounds them: 8192 x 50257 bf16, k = 64, 135 us forward (6.1 TB/s) and
 // 270 backward (6.1) on MI355X.  In the forward a row is one workgroup's; a few very wide rows
-// are cut into segments, whose {max, sum} meet in a second kernel; the backward takes a row in
-// chunks always, each computing the row's p again.
+// are cut into segments, whose {max, sum} meet in a second kernel, and where rows are many each
+// is a wave's; the backward takes a row in chunks always, each computing the row's p again.
 
 #include <hip/hip_runtime.h>
 
@@ -140,8 +140,7 @@ __device__ __forceinline__ Parts parts_of(const void* p, int n) {
     return q;
 }
 // The element of head or tail that lane t has (-1: none).
-__device__ __forceinline__ int edge(const Parts& q, int n) {
-    const int t = static_cast<int>(threadIdx.x);
+__device__ __forceinline__ int edge(const Parts& q, int n, int t) {
     const int c = t < 8 ? (t < q.head ? t : -1) : t < 16 ? q.tail0 + t - 8 : -1;
     return c < n ? c : -1;
 }
@@ -179,7 +178,7 @@ struct Lse {
     }
 };
 
-// {max, sum} of a segment, in every lane of a workgroup of LANES.
+// {max, sum} of a segment, in every lane of a workgroup of LANES, or of a wave (LANES = 64).
 constexpr int kBatch = 4;  // 16-byte loads in flight per lane
 template <class S, int LANES>
 __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, float& m, float& s,
@@ -193,7 +192,8 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
     const Parts q = parts_of<S>(z, n);
     const u32x4* const body = reinterpret_cast<const u32x4*>(z + q.head);
     Lse r{-__builtin_inff(), 0.0f};
-    int v = static_cast<int>(threadIdx.x);
+    const int lane = static_cast<int>(LANES == 64 ? threadIdx.x & 63 : threadIdx.x);
+    int v = lane;
     for (; v + (kBatch - 1) * LANES < q.slots; v += LANES * kBatch) {
         u32x4 raw[kBatch];
 #pragma unroll
@@ -213,7 +213,7 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
         S::unpack(__builtin_nontemporal_load(body + v), f);
         r.add(f, a.scale);
     }
-    if (const int c = edge(q, n); c >= 0) {
+    if (const int c = edge(q, n, lane); c >= 0) {
         const float f[1] = {S::get(z + c)};
         r.add(f, a.scale);
     }
@@ -224,6 +224,7 @@ __device__ __forceinline__ void seg_lse(const Args& a, int64_t row, int seg, flo
         const float m2 = __shfl_xor(m, h), s2 = __shfl_xor(s, h);
         join(m, s, m2, s2, a.scale);
     }
+    if constexpr (LANES == 64) return;
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(m, s);
     __syncthreads();
     m = red[0].x;
@@ -264,8 +265,8 @@ __device__ __forceinline__ void row_loss(const Args& a, int64_t row, float m, fl
     }
 }
 
-// One workgroup per row (segs == 1), looping over what the grid leaves.  Its first wave
-// has the teacher's part.
+// One workgroup per row, looping over what the grid leaves.  Its first wave has the
+// teacher's part.
 template <class S, int LANES, int PER>
 __global__ __launch_bounds__(LANES) void distill_fwd(const Args a, float* __restrict__ loss,
                                                      float2* __restrict__ stats) {
@@ -283,6 +284,23 @@ __global__ __launch_bounds__(LANES) void distill_fwd(const Args a, float* __rest
         seg_lse<S, LANES>(a, row, 0, m, s, red);
         if (first) row_loss<PER>(a, row, m, s, t, zt, loss, stats);
         __syncthreads();
+    }
+}
+
+// One wave per row, four rows per workgroup.
+template <class S, int PER>
+__global__ __launch_bounds__(kLanes) void distill_fwd_wave(const Args a, float* __restrict__ loss,
+                                                           float2* __restrict__ stats) {
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves +
+                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+         row < a.rows; row += static_cast<int64_t>(gridDim.x) * kWaves) {
+        Teacher<PER> t;
+        float zt[PER], m, s;
+        t.load(a, row);
+        t.place(a);
+        named_z<S, PER>(a, row, t, zt);
+        seg_lse<S, 64>(a, row, 0, m, s, nullptr);
+        row_loss<PER>(a, row, m, s, t, zt, loss, stats);
     }
 }
 
@@ -488,6 +506,16 @@ inline Args args(const void* z, const int64_t* index, const void* t, int64_t row
     return a;
 }
 
+// Lanes of a row in the forward, by how many rows share the chip: a wave each from seven waves
+// per CU on (no barrier, and four loads in flight each are enough), looping on three workgroups per CU
+// where rows are long, which keeps the chip's accesses together; then workgroups of 256 lanes, of 512
+// and, up to one per CU, of 1024.  MI355X, us, 256 lanes / this: 20000 x 2000 bf16 43 / 28, 16384 x 8000
+// bf16 (k = 256) 103 / 77, 2048 x 50257 f32 72 / 63 (6.6 TB/s), 8192 x 50257 bf16 132 / 130 (uncapped
+// 141), 500 x 32000 bf16 11.4 / 10.4 (1024 lanes 15.2), 300 x 50257 f32 22 / 16 (1024 lanes 20).  Waves
+// for fewer rows: 1500 x 100000 bf16 64, 256 lanes 54; 512 lanes: 1000 x 150000 bf16 59, 256 lanes 54.
+constexpr int64_t kWaveRows = 7 * 256, kGroupRows = 3 * 256;
+constexpr int64_t kShortSlots = 2048, kLongGroups = 3 * 256;
+
 template <class S, int PER>
 int forward_per(const Args& a, float* loss, float2* stats, float2* part, hipStream_t st) {
     if (a.segs > 1) {
@@ -499,14 +527,21 @@ int forward_per(const Args& a, float* loss, float2* stats, float2* part, hipStre
                            st, a, part, loss, stats);
         return check_launch();
     }
-    // a workgroup of 1024 lanes for rows too few to give every CU several of 256 (bf16 1000 x
-    // 50257 30.6 us against 23.1 with 256 lanes and 1100 rows; 300 rows 15.4)
-    if (a.rows < 512 && a.cols / S::kVec > 1024)
-        hipLaunchKernelGGL((distill_fwd<S, 1024, PER>), dim3(static_cast<unsigned>(a.rows)),
-                           dim3(1024), 0, st, a, loss, stats);
-    else
-        hipLaunchKernelGGL((distill_fwd<S, kLanes, PER>), dim3(capped_blocks(a.rows, kLanes)),
+    const int64_t slots = a.cols / S::kVec;
+    if (a.rows >= kWaveRows) {
+        int64_t groups = (a.rows + kWaves - 1) / kWaves;
+        if (slots > kShortSlots) groups = std::min(groups, kLongGroups);
+        hipLaunchKernelGGL((distill_fwd_wave<S, PER>), dim3(capped_blocks(groups, kLanes)),
                            dim3(kLanes), 0, st, a, loss, stats);
+        return check_launch();
+    }
+#define AGK_FWD(LANES)                                                                     \
+    hipLaunchKernelGGL((distill_fwd<S, LANES, PER>), dim3(capped_blocks(a.rows, LANES)),   \
+                       dim3(LANES), 0, st, a, loss, stats)
+    if (a.rows >= kGroupRows || slots <= 1024) AGK_FWD(kLanes);
+    else if (a.rows > 256) AGK_FWD(512);
+    else AGK_FWD(1024);
+#undef AGK_FWD
     return check_launch();
 }
 template <class S>

@@ -259,3 +259,48 @@ def test_gradient_against_differences(cuda):
     want = (f(z.double() + h * d) - f(z.double() - h * d)) / (2 * h)
     terms = dz.double() * d
     assert abs(terms.sum() - want) <= 1e-5 * terms.abs().sum()
+
+
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("rows,cols,k", [(1800, 20011, 20), (3100, 1003, 70), (2500, 3, 2),
+                                         (1792, 8200, 300), (1791, 8200, 9), (500, 9001, 30),
+                                         (768, 9001, 30), (257, 8300, 64)])
+def test_many_rows(cuda, dtype, rows, cols, k):
+    z, index, t, dloss = inputs(rows, cols, k, dtype, seed=5)
+    loss, dz = run(z, index, t, dloss, 1.5)
+    ref, bound = reference(z, index, t, dloss, 1.5)
+    check(loss, ref[0], bound[0], "loss")
+    check(dz, ref[1], bound[1], "dz")
+
+
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("cols", [333, 20001])
+def test_special_rows_among_many(cuda, dtype, cols):
+    rows, k, T = 1830, 12, 2.0
+    z, index, t, dloss = inputs(rows, cols, k, dtype, seed=6, empty=0.0)
+    r = torch.arange(rows, device="cuda") % 10
+    odd = 2 * torch.arange(k, device="cuda") + 1
+    index[r == 1] = -1
+    t[r == 2] = NEG
+    z[r == 1] = float("nan")
+    z[r == 2] = float("inf")
+    low = r == 3
+    z[low] = torch.finfo(dtype).min
+    masked = (r == 4).nonzero()[:, 0]
+    z[masked, ::2] = NEG
+    index[masked] = odd
+    low_masked = (r == 5).nonzero()[:, 0]
+    z[low_masked, ::2] = torch.finfo(dtype).min
+    index[low_masked] = odd
+    loss, dz = run(z, index, t, dloss, T)
+    empty = (r == 1) | (r == 2)
+    assert (loss[empty] == 0).all() and (dz[empty] == 0).all()
+    ref, bound = reference(torch.where(empty[:, None], 0.0, z), index, t, dloss, T)
+    check(loss, ref[0], bound[0], "loss")
+    check(dz, ref[1], bound[1], "dz")
+    z[r == 6, 7 % cols] = float("nan")
+    index[r == 7, 3] = cols
+    l2, d2 = run(z, index, t, dloss, T)
+    bad = (r == 6) | (r == 7)
+    assert l2[bad].isnan().all() and d2[bad].isnan().any(1).all()
+    assert torch.equal(l2[~bad], loss[~bad]) and torch.equal(d2[~bad], dz[~bad])
