@@ -34,15 +34,25 @@ constexpr int kBlocks = 256;  // workgroups, one per CU, and partial rows
 
 // (TPR, NV): lanes of a row and 16-byte slots per lane; 1024 / TPR rows at a time.  Rows of
 // more than a wave take the fewest whole waves that hold them, of the steps below: with
-// powers of two 4099 f32 rows of 1030 columns (258 slots) left half of the lanes idle.
+// powers of two 4099 f32 rows of 1030 columns (258 slots) left half of the lanes idle, and with 1024
+// lanes alone 8192 x 8193 bf16 took 172 us (640 lanes of two slots: 121), f32 200 (158).
 #define AGK_LN_SHAPES(X)                                                                 \
     X(1, 1) X(2, 1) X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(192, 1)       \
-    X(256, 1) X(320, 1) X(512, 1) X(640, 1) X(768, 1) X(1024, 1) X(1024, 2) X(1024, 4)
+    X(256, 1) X(320, 1) X(512, 1) X(640, 1) X(768, 1) X(1024, 1)                \
+    X(640, 2) X(768, 2) X(1024, 2) X(640, 4) X(768, 4) X(1024, 4)
 
 // The widest shape's 32 columns of bf16 a lane do not fit its registers.
 template <class S>
 constexpr bool enabled(int nv) {
     return !(std::is_same<S, BF16>::value && nv == 4);
+}
+
+// The widest shapes' sums of dgamma and dbeta (16 columns a lane, 128 KiB a workgroup) lie in LDS,
+// each lane's own: in registers beside two rows they spilled (MI355X, us, so / now: 8192 x 16384
+// f32 661 / 300, 5.4 TB/s; bf16 395 / 151).
+template <class S>
+constexpr bool lds_sums(int nv) {
+    return nv * S::kVec >= 16;
 }
 
 template <class T>
@@ -96,7 +106,10 @@ __global__ __launch_bounds__(kLanes / TPR * TPR) void ln_bwd(const Args<typename
     using T = typename S::T;
     constexpr int W = S::kVec;
     constexpr int G = kLanes / TPR;
+    constexpr bool kLdsSums = lds_sums<S>(NV);
+    constexpr int kQuads = NV * W / 4;  // of a lane's columns
     __shared__ float2 red[2][TPR > 64 ? G * (TPR / 64) : 1];
+    __shared__ float4 sums[kLdsSums ? 2 * kQuads * TPR : 1];  // [dgamma, dbeta][quad][lane]
     extern __shared__ float part[];  // G > 1: [G][cols]
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const int cols = p.cols;
@@ -118,11 +131,21 @@ __global__ __launch_bounds__(kLanes / TPR * TPR) void ln_bwd(const Args<typename
 #pragma unroll
             for (int e = 0; e < W; ++e) gm[k][e] = 1.0f;
     }
-    float dg[NV][W], db[NV][W];
+    float dg[NV][W], db[NV][W];  // kLdsSums: of one row
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < W; ++e) dg[k][e] = db[k][e] = 0.0f;
+    if constexpr (kLdsSums) {
+#pragma unroll
+        for (int q = 0; q < 2 * kQuads; ++q) sums[q * TPR + t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    auto add = [](float4& s, const float* v) {
+        s.x += v[0];
+        s.y += v[1];
+        s.z += v[2];
+        s.w += v[3];
+    };
 
     const int64_t stride = static_cast<int64_t>(gridDim.x) * G;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * G;
@@ -159,8 +182,20 @@ __global__ __launch_bounds__(kLanes / TPR * TPR) void ln_bwd(const Args<typename
                 const float xh = take ? xhat : 0.0f;
                 sh += h;
                 shx += h * xh;
-                dg[k][e] += d * xh;
-                db[k][e] += d;
+                if constexpr (kLdsSums) {
+                    dg[k][e] = d * xh;
+                    db[k][e] = d;
+                } else {
+                    dg[k][e] += d * xh;
+                    db[k][e] += d;
+                }
+            }
+            if constexpr (kLdsSums) {
+#pragma unroll
+                for (int q = 0; q < W / 4; ++q) {
+                    add(sums[(k * (W / 4) + q) * TPR + t], dg[k] + q * 4);
+                    add(sums[(kQuads + k * (W / 4) + q) * TPR + t], db[k] + q * 4);
+                }
             }
         }
         row_sum2<TPR, G>(sh, shx, red, parity);
@@ -203,6 +238,19 @@ __global__ __launch_bounds__(kLanes / TPR * TPR) void ln_bwd(const Args<typename
     }
 
     if (!p.partial) return;
+    if constexpr (kLdsSums) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int q = 0; q < W / 4; ++q) {
+                const float4 g = sums[(k * (W / 4) + q) * TPR + t];
+                const float4 b4 = sums[(kQuads + k * (W / 4) + q) * TPR + t];
+                dg[k][q * 4] = g.x, dg[k][q * 4 + 1] = g.y;
+                dg[k][q * 4 + 2] = g.z, dg[k][q * 4 + 3] = g.w;
+                db[k][q * 4] = b4.x, db[k][q * 4 + 1] = b4.y;
+                db[k][q * 4 + 2] = b4.z, db[k][q * 4 + 3] = b4.w;
+            }
+    }
     const int64_t nblk = gridDim.x;
     float* const out[2] = {p.partial + blockIdx.x * static_cast<int64_t>(cols),
                            p.partial + (nblk + blockIdx.x) * static_cast<int64_t>(cols)};
@@ -334,11 +382,10 @@ inline Shape pick(int64_t cols) {
     s.nv = nv;
     s.tpr = 1024;
     for (int tpr : kTpr)
-        if (static_cast<int64_t>(tpr) * nv >= slots) {
+        if ((nv == 1 || tpr >= 640) && static_cast<int64_t>(tpr) * nv >= slots) {
             s.tpr = tpr;
             break;
         }
-    if (nv > 1) s.tpr = 1024;
     return s;
 }
 

@@ -1168,6 +1168,7 @@ inline bool fits_buffer(int cols) {
 template <class Op, class S>
 inline bool prefers_looped_vec(const RowArgs& p, int64_t rows, int cols) {
     if (cols < kVecMinCols || !fits_buffer<S>(cols) || !same_offset<typename S::T>(p)) return false;
+    if (std::is_same<Op, LnAffineFwd>::value) return false;
     const int64_t nslot = row_slots(cols, S::kVec);
     return Op::kIn == 1 ||
            (std::is_same<S, BF16>::value ? nslot > 2048 : rows > 1500 && nslot <= 2560);

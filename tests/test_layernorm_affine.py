@@ -270,3 +270,26 @@ def test_gradients_against_differences(cuda):
         got = (grad.double() * d).sum()
         # 1e-6 of the terms' magnitude: 32 u and the differences' own error
         assert abs(got - want) <= 1e-6 * (grad.double() * d).abs().sum(), (i, got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(700, 16384), (600, 9000), (530, 8193), (520, 12001),
+                                       (1030, 5001), (300, 16383), (900, 6144), (257, 10240)])
+def test_wide_rows_several_to_a_workgroup(cuda, dtype, rows, cols):
+    x, g, b, dy = inputs(rows, cols, dtype, seed=7)
+    y, mean, rstd = agk.layernorm_affine_fwd(x, g, b, EPS)
+    dx, dg, db = agk.layernorm_affine_bwd(x, g, mean, rstd, dy)
+    ref, bound = reference(x, g, b, dy)
+    for got, want, tol, what in zip((y, dx, dg, db), ref, bound, ("y", "dx", "dgamma", "dbeta")):
+        check(got, want, tol, what)
+    # into what is there: each output's own addition, one rounding more
+    old = [torch.randn_like(v) for v in (dx, dg, db)]
+    into = [v.clone() for v in old]
+    agk.layernorm_affine_bwd(x, g, mean, rstd, dy, dx=into[0], dgamma=into[1], dbeta=into[2],
+                             accumulate=True)
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    for got, base, want, tol, r in zip(into, old, ref[1:], bound[1:], (half, 2.0 ** -24, 2.0 ** -24)):
+        total = base.double() + want
+        check(got, total, tol + 2 * r * (total.abs() + tol), "accumulated")
+    only = agk.layernorm_affine_bwd(x, g, mean, rstd, dy, want_dx=False)
+    assert only[0] is None and torch.equal(only[1], dg) and torch.equal(only[2], db)
