@@ -480,7 +480,7 @@ inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
     return d;
 }
 
-inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks) {
+inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks, double* us = nullptr) {
     using namespace agk_gemm;
     const int64_t cus = device_cus();
     // Few tokens are bound by the read of w: 64 x 128 tiles, as many slices as give each CU one.
@@ -488,7 +488,10 @@ inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks) {
     // 103, 64 x 2048 x 50257 104 / 95, 64 x 4096 x 131072 402 / 391; with 256 columns no slices are enough.
     const int64_t across = (cols + 127) / 128, cuts = cus / across;
     if (rows8 <= 64 && walks == 1 && cuts >= 1 && cuts <= kMaxSlices && k >= cuts * kMinSlice)
+    {
+        if (us) *us = static_cast<double>(k * cols) * 2 / 5e6 + 2 * kRoundUs;
         return last_piece(DxPlan{7, static_cast<int>(cuts), 0}, k);
+    }
     DxPlan best{pick_shape(rows8, cols, k, device_cus()), 1, static_cast<int>(up(k, 64))};
     double best_cost = 1e30;
     for (const RingCost& s : kRingCosts) {
@@ -515,6 +518,7 @@ inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks) {
             }
         }
     }
+    if (us) *us = best_cost;
     return best;
 }
 
@@ -558,7 +562,13 @@ struct BwdLayout {
     int planes;
     int64_t piece, padded;             // vocabulary rows of a piece, and of its operands
     int64_t rows8, rows64, ldg, kp, cols8;
-    DxPlan dx;
+    int64_t main;  // dx: rows of the first product, the others (bf16) by a second
+    DxPlan dx, rest;
+    // The fp32 sums of dx: every slice's rows of cols8.
+    int64_t rest_acc() const { return static_cast<int64_t>(dx.slices) * main * cols8; }
+    int64_t acc_values() const {
+        return rest_acc() + (main < rows8 ? rest.slices * (rows8 - main) * cols8 : 0);
+    }
     size_t weight, scalars, parts, x, w2, g, acc, total;
 };
 inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t ldw, int dtype,
@@ -574,8 +584,24 @@ inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t l
     o.cols8 = up(cols, 8);
     o.piece = piece_rows(vocab, o.ldg, bf16 ? ldw : o.kp, o.planes, piece);
     o.padded = bf16 || o.instr ? o.piece : up(o.piece, 64);
+    double us = 0.0;
+    o.main = o.rows8;
     o.dx = o.instr ? dx_plan32(o.rows8, cols, o.piece)
-                   : dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : PlanesK::kWalks);
+                   : dx_plan(o.rows8, o.cols8, o.padded, bf16 ? 1 : PlanesK::kWalks, &us);
+    o.rest = o.dx;
+    // A few tokens past whole 256-row tiles cost a row of tiles: by themselves they are one more
+    // read of w (4099 tokens x 2048 x 50257 on MI355X 811 us, so 605 + 47).
+    const int64_t whole = rows / 256 * 256;
+    if (bf16 && whole >= 1024 && rows > whole && rows - whole <= 64) {
+        double us_main = 0.0, us_rest = 0.0;
+        const DxPlan a = dx_plan(whole, o.cols8, o.padded, 1, &us_main);
+        const DxPlan b = dx_plan(o.rows8 - whole, o.cols8, o.padded, 1, &us_rest);
+        if (us_main + us_rest < us) {
+            o.main = whole;
+            o.dx = a;
+            o.rest = b;
+        }
+    }
     o.weight = 0;
     o.scalars = o.weight + region(o.rows8 * 4);
     o.parts = o.scalars + region(sizeof(Scalars));
@@ -583,7 +609,7 @@ inline BwdLayout bwd_layout(int64_t rows, int64_t vocab, int64_t cols, int64_t l
     o.w2 = o.x + region(bf16 ? rows * cols * 2 : o.rows64 * o.kp * 4);
     o.g = o.w2 + (bf16 || o.instr ? 0 : region(o.padded * o.kp * 4));
     o.acc = o.g + region(o.padded * o.ldg * 2 * o.planes);
-    o.total = o.acc + region(static_cast<int64_t>(o.dx.slices) * o.rows8 * o.cols8 * 4);
+    o.total = o.acc + region(o.acc_values() * 4);
     return o;
 }
 
@@ -772,9 +798,12 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         const int64_t p = piece_rows(vocab, o.ldg, ldw, 1, piece);
         if (p < o.piece) {
             o.piece = p;
-            const int64_t had = o.dx.slices;
-            o.dx = dx_plan(o.rows8, o.cols8, p, 1);
-            if (o.dx.slices > had) o.dx = last_piece(DxPlan{o.dx.shape, static_cast<int>(had), 0}, p);
+            auto again = [&](int64_t rows, const DxPlan& had) {
+                const DxPlan d = dx_plan(rows, o.cols8, p, 1);
+                return d.slices > had.slices ? last_piece(DxPlan{d.shape, had.slices, 0}, p) : d;
+            };
+            o.dx = again(o.main, o.dx);
+            o.rest = o.main < o.rows8 ? again(o.rows8 - o.main, o.rest) : o.dx;
         }
     }
     agk::clear_pending_error();
@@ -790,7 +819,9 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const int ldg = static_cast<int>(o.ldg), kp = static_cast<int>(o.kp);
     const int c1 = static_cast<int>(cols), c8 = static_cast<int>(o.cols8);
     const int cus = agk_gemm::device_cus();
-    const int64_t slice = o.rows8 * o.cols8;
+    const int64_t slice = o.main * o.cols8, left8 = o.rows8 - o.main;
+    const int mm = static_cast<int>(o.main);
+    float* const acc_rest = acc + o.rest_acc();
     const int64_t copied = (bf16 || o.instr) && dw ? rows : 0;
     const dim3 grid(1 + agk::capped_blocks((copied + 3) / 4, 1 << 20)), block(1024);
     if (bf16)
@@ -827,7 +858,7 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
             continue;
         }
         const DxPlan d = n == o.piece ? o.dx : last_piece(o.dx, np);
-        const AddEpi<true> de{acc, c8, slice, bf16 ? nullptr : &sc->dx, m8, c8, v0 > 0};
+        const AddEpi<true> de{acc, c8, slice, bf16 ? nullptr : &sc->dx, mm, c8, v0 > 0};
         char* const out = static_cast<char*>(dw) + v0 * cols * dw_size;
         if (bf16) {
             const uint16_t* const wp = static_cast<const uint16_t*>(w) + v0 * ldw;
@@ -838,7 +869,15 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
             if (rc != AGK_OK) return rc;
             if (dx)
                 rc = launch_dx(d.shape,
-                               Product{g, ldg, wp, ldw, m8, c1, nv, d.slices, d.k_slice, st}, de);
+                               Product{g, ldg, wp, ldw, mm, c1, nv, d.slices, d.k_slice, st}, de);
+            if (rc != AGK_OK) return rc;
+            if (dx && left8) {
+                const DxPlan r = n == o.piece ? o.rest : last_piece(o.rest, n);
+                const int ml = static_cast<int>(left8);
+                rc = launch_dx(r.shape,
+                               Product{g + mm, ldg, wp, ldw, ml, c1, nv, r.slices, r.k_slice, st},
+                               AddEpi<true>{acc_rest, c8, left8 * o.cols8, nullptr, ml, c8, v0 > 0});
+            }
             if (rc != AGK_OK) return rc;
             const Product wt{g, ldg, xk, cols, nv, c1, m, 1, 0, st};
             const int shape = agk_gemm::pick_shape(n, cols, rows, cus);
@@ -873,12 +912,21 @@ int agk_linear_xent_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
         if (rc != AGK_OK) return rc;
     }
     if (!dx) return AGK_OK;
-    const int64_t lanes = rows * o.cols8 / (bf16 ? 8 : 4);
+    const int64_t first = std::min(rows, o.main);
+    const int64_t lanes = first * o.cols8 / (bf16 ? 8 : 4);
     const dim3 out_grid(static_cast<unsigned>((lanes + 255) / 256));
-    if (bf16)
+    if (bf16) {
+        uint16_t* const out = static_cast<uint16_t*>(dx);
         hipLaunchKernelGGL(xent_dx_out, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice, sc,
-                           weight, static_cast<uint16_t*>(dx), lanes, c8 / 8, acc_dx);
-    else
+                           weight, out, lanes, c8 / 8, acc_dx);
+        if (left8) {
+            if ((rc = check_launch()) != AGK_OK) return rc;
+            const int64_t more = (rows - first) * o.cols8 / 8;
+            hipLaunchKernelGGL(xent_dx_out, dim3(static_cast<unsigned>((more + 255) / 256)),
+                               dim3(256), 0, st, acc_rest, o.rest.slices, left8 * o.cols8, sc,
+                               weight + first, out + first * cols, more, c8 / 8, acc_dx);
+        }
+    } else
         hipLaunchKernelGGL(xent_dx_out32, out_grid, dim3(256), 0, st, acc, o.dx.slices, slice, sc,
                            weight, static_cast<float*>(dx), rows, c1, c8, acc_dx);
     return check_launch();

@@ -465,3 +465,22 @@ def test_few_tokens_in_pieces(cuda, dtype, N, piece):
         check(got, want, tol, what)
         r = R[got.dtype]
         check(added, base.double() + want, tol + r * (base.double() + want).abs() + 2 * r * tol, what)
+
+
+@pytest.mark.parametrize("piece", [0, 1024])
+@pytest.mark.parametrize("N", [4097, 4103, 4160])
+def test_a_few_tokens_past_whole_tiles(cuda, N, piece):
+    # their dx is a product of its own
+    V, D = 3000, 2048
+    x, w, labels, dloss = inputs(N, V, D, BF, seed=26)
+    loss, stats = agk.linear_cross_entropy_fwd(x, w, labels)
+    dx0 = torch.randn(N, D, device="cuda").to(BF)
+    into = dx0.clone()
+    dx, dw = agk.linear_cross_entropy_bwd(x, w, labels, stats, dloss, piece=piece)
+    agk.linear_cross_entropy_bwd(x, w, labels, stats, dloss, dx=into, want_dw=False, piece=piece,
+                                 accumulate=True)
+    ref, bound = reference(x, w, labels, dloss)
+    for got, want, tol, what in zip((loss, dx, dw), ref, bound, ("loss", "dx", "dw")):
+        check(got, want, tol, what)
+    total = dx0.double() + ref[1]
+    check(into, total, bound[1] + 2.0 ** -8 * total.abs() + 2.0 ** -7 * bound[1], "dx added")
