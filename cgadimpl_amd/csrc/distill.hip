@@ -506,13 +506,14 @@ inline Args args(const void* z, const int64_t* index, const void* t, int64_t row
     return a;
 }
 
-// Lanes of a row in the forward, by how many rows share the chip: a wave each from seven waves
-// per CU on (no barrier, and four loads in flight each are enough), looping on three workgroups per CU
-// where rows are long, which keeps the chip's accesses together; then workgroups of 256 lanes, of 512
-// and, up to one per CU, of 1024.  MI355X, us, 256 lanes / this: 20000 x 2000 bf16 43 / 28, 16384 x 8000
-// bf16 (k = 256) 103 / 77, 2048 x 50257 f32 72 / 63 (6.6 TB/s), 8192 x 50257 bf16 132 / 130 (uncapped
-// 141), 500 x 32000 bf16 11.4 / 10.4 (1024 lanes 15.2), 300 x 50257 f32 22 / 16 (1024 lanes 20).  Waves
-// for fewer rows: 1500 x 100000 bf16 64, 256 lanes 54; 512 lanes: 1000 x 150000 bf16 59, 256 lanes 54.
+// Lanes of a row in the forward, by how many rows share the chip: a wave each from seven
+// waves per CU on (no barrier, and four loads in flight each are enough), looping on three
+// workgroups per CU where rows are long, which keeps the chip's accesses together; then
+// workgroups of 256 lanes, of 512 and, up to one per CU, of 1024.  MI355X, us, 256 lanes /
+// this: 20000 x 2000 bf16 43 / 28, 16384 x 8000 bf16 (k = 256) 103 / 77, 2048 x 50257 f32 72
+// / 63 (6.6 TB/s), 8192 x 50257 bf16 132 / 130 (uncapped 141), 500 x 32000 bf16 11.4 / 10.4
+// (1024 lanes 15.2), 300 x 50257 f32 22 / 16 (1024 lanes 20).  Waves for fewer rows: 1500 x
+// 100000 bf16 64, 256 lanes 54; 512 lanes: 1000 x 150000 bf16 59, 256 lanes 54.
 constexpr int64_t kWaveRows = 7 * 256, kGroupRows = 3 * 256;
 constexpr int64_t kShortSlots = 2048, kLongGroups = 3 * 256;
 

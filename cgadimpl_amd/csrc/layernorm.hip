@@ -34,8 +34,9 @@ constexpr int kBlocks = 256;  // workgroups, one per CU, and partial rows
 
 // (TPR, NV): lanes of a row and 16-byte slots per lane; 1024 / TPR rows at a time.  Rows of
 // more than a wave take the fewest whole waves that hold them, of the steps below: with
-// powers of two 4099 f32 rows of 1030 columns (258 slots) left half of the lanes idle, and with 1024
-// lanes alone 8192 x 8193 bf16 took 172 us (640 lanes of two slots: 121), f32 200 (158).
+// powers of two 4099 f32 rows of 1030 columns (258 slots) left half of the lanes idle, and
+// with 1024 lanes alone 8192 x 8193 bf16 took 172 us (640 lanes of two slots: 121), f32 200
+// (158).
 #define AGK_LN_SHAPES(X)                                                                 \
     X(1, 1) X(2, 1) X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(192, 1)       \
     X(256, 1) X(320, 1) X(512, 1) X(640, 1) X(768, 1) X(1024, 1)                \

@@ -395,9 +395,9 @@ __global__ __launch_bounds__(256) void xent_zero(uint32_t* __restrict__ out, int
 
 // G's piece.  Larger pieces cost dx fewer additions and leave fewer part-filled rounds of
 // tiles; that G then no longer fits the Infinity Cache does not show, the products being
-// bound by the matrix cores.  Backward on MI355X, us for pieces of 64 / 128 / 256 / 512 MiB / 1 GiB: 8192
-// tokens x 4096 x 131072 22842 / 21095 / 20474 / 20068 / 20073; 4099 x 2048 x 50257 (pieces of
-// 8192 / 16384 / 32768 rows, one piece) 2843 / 2805 / 2698 / 2444.
+// bound by the matrix cores.  Backward on MI355X, us for pieces of 64 / 128 / 256 / 512 MiB /
+// 1 GiB: 8192 tokens x 4096 x 131072 22842 / 21095 / 20474 / 20068 / 20073; 4099 x 2048 x
+// 50257 (pieces of 8192 / 16384 / 32768 rows, one piece) 2843 / 2805 / 2698 / 2444.
 constexpr int64_t kPieceBytes = 512LL << 20;
 constexpr int64_t kMaxOperand = 1LL << 30;    // values a product's 31-bit offsets reach
 constexpr int64_t kMaxTokens = 1LL << 24;     // a workgroup per token within a grid
@@ -483,9 +483,10 @@ inline DxPlan last_piece(const DxPlan& plan, int64_t n) {
 inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks, double* us = nullptr) {
     using namespace agk_gemm;
     const int64_t cus = device_cus();
-    // Few tokens are bound by the read of w: 64 x 128 tiles, as many slices as give each CU one.
-    // dx alone (with the logits again) on MI355X, us, the cost below / this: 16 x 4096 x 32000 112 /
-    // 103, 64 x 2048 x 50257 104 / 95, 64 x 4096 x 131072 402 / 391; with 256 columns no slices are enough.
+    // Few tokens are bound by the read of w: 64 x 128 tiles, as many slices as give each CU
+    // one. dx alone (with the logits again) on MI355X, us, the cost below / this: 16 x 4096 x
+    // 32000 112 / 103, 64 x 2048 x 50257 104 / 95, 64 x 4096 x 131072 402 / 391; with 256
+    // columns no slices are enough.
     const int64_t across = (cols + 127) / 128, cuts = cus / across;
     if (rows8 <= 64 && walks == 1 && cuts >= 1 && cuts <= kMaxSlices && k >= cuts * kMinSlice)
     {
@@ -522,10 +523,11 @@ inline DxPlan dx_plan(int64_t rows8, int64_t cols, int64_t k, int walks, double*
     return best;
 }
 
-// fp32 of few tokens on the fp32 instruction, which reads w as it lies (its 32-row blocks are what
-// max_blocks counts for kFewTokens and less; its k-strided loads take four columns).  Forward /
-// backward on MI355X, us, planes / this: 16 tokens x 2048 x 32000 203, 389 / 63, 237; 64 x 1024 x
-// 32000 92, 210 / 46, 155; 128 x 1024 x 20000 73, 179 / 59, 172; 129 x 1024 x 32000 106, 302 / 110, 330.
+// fp32 of few tokens on the fp32 instruction, which reads w as it lies (its 32-row blocks are
+// what max_blocks counts for kFewTokens and less; its k-strided loads take four columns).
+// Forward / backward on MI355X, us, planes / this: 16 tokens x 2048 x 32000 203, 389 / 63,
+// 237; 64 x 1024 x 32000 92, 210 / 46, 155; 128 x 1024 x 20000 73, 179 / 59, 172; 129 x 1024
+// x 32000 106, 302 / 110, 330.
 inline bool on_instruction(int64_t rows, int64_t vocab, int64_t cols, int dtype) {
     return dtype == AGK_F32 && rows <= kFewTokens && cols >= 4 && vocab <= 1LL << 28;
 }

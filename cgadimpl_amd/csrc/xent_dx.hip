@@ -1,4 +1,5 @@
-// xent_dx.hip -- kernels of xent_gemm.hpp: dx = G w: G^T [vocab][tokens] and w [vocab][cols] are both k-strided.
+// xent_dx.hip -- kernels of xent_gemm.hpp: dx = G w: G^T [vocab][tokens] and w [vocab][cols] are
+// both k-strided.
 #define AGK_RING_KERNELS
 #define AGK_XENT_KERNELS
 #include "xent_gemm.hpp"

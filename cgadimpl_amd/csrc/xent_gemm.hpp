@@ -24,18 +24,19 @@ using agk_gemm::f32x16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kLine = 64;  // bf16 of a 128-byte line
 
-// fp32 operands.  A matrix is stored scaled by a power of two that brings its largest value to
-// 2^14 .. 2^15, each value as two fp16 whose sum it is to 2^-22 of it: x = a + b, a = fp16(x), b =
-// fp16(x - a), in two planes side by side in each row.  A product of two is aa' + ab' + ba', three fp16
-// products summed in fp32 by walking K three times over different planes.  What is left out
-// (bb' and the two remainders) is at most 3 * 2^-22 of each product, 12 times an fp32 rounding
-// and of random sign: below the error of an fp32 sum of some dozens of products, and nothing
-// next to one of thousands.  Values 2^-28 of the largest and below lose relative bits
-// (fp16's smallest is 2^-24), at 2^-39 of the largest.  Three fp16 matrix instructions at 1250
-// TFLOP/s are 416 TFLOP/s of fp32; the fp32 matrix instruction gives 113-135 (of 157).  In three
-// bf16 planes (2^-25) it is six walks.  1000 tokens x 1000 x 32000, forward + backward on
-// MI355X: fp32 instruction 2.47 ms, bf16 planes 1.59, fp16 planes 0.96; relative error of dx
-// 6e-7 (fp32 products of the BLAS library: 3e-6).
+// fp32 operands.  A matrix (the forward: a row) is stored scaled by a power of two that
+// brings its largest value to 2^14 .. 2^15, each value as two fp16 whose sum it is to 2^-22
+// of it: x = a + b, a = fp16(x), b = fp16(x - a), in two planes side by side in each row.  A
+// product of two is aa' + ab' + ba', three fp16 products summed in fp32 by walking K three
+// times over different planes.  What is left out (bb' and the two remainders) is at most 3 *
+// 2^-22 of each product, 12 times an fp32 rounding and of random sign: below the error of an
+// fp32 sum of some dozens of products, and nothing next to one of thousands.  Values 2^-28 of
+// the largest and below lose relative bits (fp16's smallest is 2^-24), at 2^-39 of the
+// largest.  Three fp16 matrix instructions at 1250 TFLOP/s are 416 TFLOP/s of fp32; the fp32
+// matrix instruction gives 113-135 (of 157).  In three bf16 planes (2^-25) it is six walks.
+// 1000 tokens x 1000 x 32000, forward + backward on MI355X: fp32 instruction 2.47 ms, bf16
+// planes 1.59, fp16 planes 0.96; relative error of dx 6e-7 (fp32 products of the BLAS
+// library: 3e-6).
 struct PlanesK {
     static constexpr bool kF16 = true, kStream = false;
     static constexpr int kWalks = 3;
@@ -69,15 +70,15 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&plane)[2]) {
     plane[1] = __builtin_bit_cast(uint32_t, b);
 }
 
-// Few tokens, one column of tiles: the time is the read of w, each row by one workgroup, so its
-// loads are non-temporal.  Workgroups that walk K in step read the same offsets of rows that lie,
-// as a rule, a power of two apart, which are in a few of the memory's channels; so each starts at
-// a k-tile of its own.  Forward on MI355X, w not in the caches, in step / turned (us): 16 tokens x
-// 4096 x 32000 55 / 48 (of it the join and two launches' gaps 8; 262 MB at 6.6 TB/s), x 2048 x
-// 50257 50 / 41, 64 x 8192 x 32000 108 / 96.  It does not pay with few tiles, which are bound by
-// latency (16 x 4096 x 8000, 125 tiles: 24 / 27), nor where rows are not whole 128-byte lines,
-// two k-tiles sharing one (16 x 1000 x 100000: 55 / 63); deeper rings gain nothing (4 or 7 stages of 128 x
-// 32: the same).
+// Few tokens, one column of tiles: the time is the read of w, each row by one workgroup, so
+// its loads are non-temporal.  Workgroups that walk K in step read the same offsets of rows
+// that lie, as a rule, a power of two apart, which are in a few of the memory's channels; so
+// each starts at a k-tile of its own.  Forward on MI355X, w not in the caches, in step /
+// turned (us): 16 tokens x 4096 x 32000 55 / 48 (of it the join and two launches' gaps 8; 262
+// MB at 6.6 TB/s), x 2048 x 50257 50 / 41, 64 x 8192 x 32000 108 / 96.  It does not pay with
+// few tiles, which are bound by latency (16 x 4096 x 8000, 125 tiles: 24 / 27), nor where
+// rows are not whole 128-byte lines, two k-tiles sharing one (16 x 1000 x 100000: 55 / 63);
+// deeper rings gain nothing (4 or 7 stages of 128 x 32: the same).
 struct TurnedK {
     static constexpr bool kF16 = false, kStream = true;
     int n, first;

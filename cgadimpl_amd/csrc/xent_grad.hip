@@ -1,4 +1,5 @@
-// xent_grad.hip -- kernels of xent_gemm.hpp: the backward's z^T = w x^T, which leaves as the gradient of the logits.
+// xent_grad.hip -- kernels of xent_gemm.hpp: the backward's z^T = w x^T, which leaves as the
+// gradient of the logits.
 #define AGK_RING_KERNELS
 #define AGK_XENT_KERNELS
 #include "xent_gemm.hpp"

@@ -1,4 +1,5 @@
-// xent_lse.hip -- kernels of xent_gemm.hpp: the forward's product z^T = w x^T (both k-contiguous), reduced in its epilogue.
+// xent_lse.hip -- kernels of xent_gemm.hpp: the forward's product z^T = w x^T (both
+// k-contiguous), reduced in its epilogue.
 #define AGK_RING_KERNELS
 #define AGK_XENT_KERNELS
 #include "xent_gemm.hpp"

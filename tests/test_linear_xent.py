@@ -400,7 +400,7 @@ def test_scales_of_any_size(cuda, N, ex, ew):
 @pytest.mark.parametrize("N,V,D,pitch", [
     (1, 12289, 64, 64), (33, 13001, 192, 192), (64, 33001, 128, 128), (20, 32900, 64, 64),
     (7, 20011, 200, 256), (64, 33003, 72, 128), (65, 25000, 192, 192), (100, 30011, 136, 192),
-    (3, 33001, 72, 72)])
+    (3, 33001, 72, 72), (20, 20011, 40, 64), (64, 40003, 8, 64)])
 def test_few_tokens_of_many_words(cuda, N, V, D, pitch):
     # one column of tiles whose workgroups start their walks of K at different tiles
     x, w, labels, dloss = inputs(N, V, D, BF, seed=23)
