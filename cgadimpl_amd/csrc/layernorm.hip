@@ -409,6 +409,10 @@ int launch(const Args<typename S::T>& a, int64_t* nblk, hipStream_t st) {
     }
     const int g = kLanes / s.tpr;
     *nblk = blocks(a.rows, g);
+    // few groups of rows each: as many workgroups as have the same number of them, which is as
+    // quick and leaves fewer partial rows (MI355X, us: 300 x 16384 f32 43 -> 35, 300 x 8192 22 -> 18)
+    const int64_t groups = (a.rows + g - 1) / g, each = (groups + *nblk - 1) / *nblk;
+    if (each <= 4) *nblk = (groups + each - 1) / each;
     const size_t lds = g > 1 && a.partial ? static_cast<size_t>(g) * a.cols * 4 : 0;
     const dim3 grid(static_cast<unsigned>(*nblk)), block(g * s.tpr);
 #define AGK_X(TPR, NV)                                                                      \
