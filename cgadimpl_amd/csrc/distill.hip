@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "agk_losses.h"
 #include "rowcommon.hpp"
@@ -352,12 +353,62 @@ __global__ __launch_bounds__(64) void distill_join(const Args a, const float2* _
 constexpr int kSlots = 4;              // 16-byte slots per lane
 constexpr int kChunk = 64 * kSlots;    // and per wave
 
-template <class S, int PER, bool ACC>
-__global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) void distill_bwd(
+// Orders a wave's LDS accesses among its lanes (the hardware takes them in order).
+__device__ __forceinline__ void lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// DENSE: chunks of many entries (from kDense on).  One by one they would take longer than the
+// chunk's bytes; so their probabilities are added into an LDS array of the chunk's columns, 64
+// at a time: the lanes claim their columns' places in a small table (the lowest lane gets it,
+// so that a column's entries are added in their order), the winners add, the others try again.
+template <class S>
+struct Dense {
+    static constexpr int kEdge = kChunk * S::kVec;  // head, then tail, behind the chunk's columns
+    float delta[kEdge + 16];
+    unsigned claim[256];
+
+    __device__ __forceinline__ void clear(int lane) {
+#pragma unroll
+        for (int u = 0; u < kSlots; ++u)
+#pragma unroll
+            for (int e = 0; e < S::kVec; e += 4)
+                *reinterpret_cast<float4*>(delta + (u * 64 + lane) * S::kVec + e) =
+                    make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (lane < 16) delta[kEdge + lane] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) claim[u * 64 + lane] = ~0u;
+        lds_order();
+    }
+    // delta[pos] += p for lanes whose pos is not negative
+    __device__ __forceinline__ void add(int pos, float p, int lane) {
+        bool left = pos >= 0;
+        const int place = pos & 255;
+        while (__any(left)) {
+            if (left) atomicMin(&claim[place], static_cast<unsigned>(lane));
+            lds_order();
+            const bool won = left && *const_cast<volatile unsigned*>(&claim[place]) ==
+                                         static_cast<unsigned>(lane);
+            lds_order();
+            if (won) {
+                delta[pos] += p;
+                claim[place] = ~0u;
+            }
+            lds_order();
+            left = left && !won;
+        }
+    }
+};
+
+template <class S, int PER, bool ACC, bool DENSE>
+__global__ __launch_bounds__(kLanes, DENSE ? 3 : PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) void
+distill_bwd(
     const Args a, const float2* __restrict__ stats, const float* __restrict__ dloss, void* dz_,
     int chunks) {
     using T = typename S::T;
     constexpr int W = S::kVec;
+    __shared__ typename std::conditional<DENSE, Dense<S>, char>::type dense[kWaves];
     const int lane = static_cast<int>(threadIdx.x & 63);
     const int64_t items = a.rows * chunks;
     for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves +
@@ -415,31 +466,58 @@ __global__ __launch_bounds__(kLanes, PER == 1 && !ACC ? 8 : PER <= 4 ? 5 : 3) vo
             for (int e = 0; e < W; ++e) f[u][e] = grad(f[u][e]);
         }
         const int first = q.head + chunk * kChunk * W;  // the chunk's columns but the edges
+        if constexpr (DENSE) {
+            Dense<S>& d = dense[threadIdx.x >> 6];
+            d.clear(lane);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int r = t.at[i] - first;
-            const bool mine = t.at[i] >= 0 && ((r >= 0 && r < kChunk * W) ||
-                                             (chunk == 0 && r < 0) ||
-                                             (chunk == chunks - 1 && t.at[i] >= q.tail0));
-            unsigned long long todo = __ballot(mine);
-            while (todo) {
-                const int l = __builtin_ctzll(todo);
-                todo &= todo - 1;
-                const int col = __builtin_amdgcn_readlane(t.at[i], l);
-                const float d =
-                    c * (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.p[i]), l)) / sum);
-                if (col == ec) eg -= d;
-                const int rel = col - first;
-                if (rel < 0 || col >= q.tail0) continue;
-                const int slot = rel / W, elem = rel % W;
-                const float mine_d = lane == (slot & 63) ? d : 0.0f;
+            for (int i = 0; i < PER; ++i) {
+                const int at = t.at[i], r = at - first;
+                int pos = -1;
+                if (at >= 0 && at < q.head)
+                    pos = chunk == 0 ? Dense<S>::kEdge + at : -1;
+                else if (at >= q.tail0)
+                    pos = chunk == chunks - 1 ? Dense<S>::kEdge + 8 + at - q.tail0 : -1;
+                else if (at >= 0 && r >= 0 && r < kChunk * W)
+                    pos = r;
+                d.add(pos, t.p[i], lane);
+            }
+            const float inv = 1.0f / sum;
+            // (an untouched column keeps its value where c is not finite too)
+            auto less = [&](float g, float p) { return p == 0.0f ? g : g - c * (p * inv); };
 #pragma unroll
-                for (int u = 0; u < kSlots; ++u)
-                    if (u == slot / 64) {
+            for (int u = 0; u < kSlots; ++u)
 #pragma unroll
-                        for (int e = 0; e < W; ++e)
-                            if (e == elem) f[u][e] -= mine_d;
-                    }
+                for (int e = 0; e < W; ++e)
+                    f[u][e] = less(f[u][e], d.delta[(u * 64 + lane) * W + e]);
+            if (lane < 16) eg = less(eg, d.delta[Dense<S>::kEdge + lane]);
+            lds_order();
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int r = t.at[i] - first;
+                const bool mine = t.at[i] >= 0 && ((r >= 0 && r < kChunk * W) ||
+                                                 (chunk == 0 && r < 0) ||
+                                                 (chunk == chunks - 1 && t.at[i] >= q.tail0));
+                unsigned long long todo = __ballot(mine);
+                while (todo) {
+                    const int l = __builtin_ctzll(todo);
+                    todo &= todo - 1;
+                    const int col = __builtin_amdgcn_readlane(t.at[i], l);
+                    const float d =
+                        c * (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.p[i]), l)) / sum);
+                    if (col == ec) eg -= d;
+                    const int rel = col - first;
+                    if (rel < 0 || col >= q.tail0) continue;
+                    const int slot = rel / W, elem = rel % W;
+                    const float mine_d = lane == (slot & 63) ? d : 0.0f;
+#pragma unroll
+                    for (int u = 0; u < kSlots; ++u)
+                        if (u == slot / 64) {
+#pragma unroll
+                            for (int e = 0; e < W; ++e)
+                                if (e == elem) f[u][e] -= mine_d;
+                        }
+                }
             }
         }
         // a row without a teacher or weight: zeros, whatever z holds
@@ -552,6 +630,12 @@ int forward(const Args& a, float* loss, float2* stats, float2* part, hipStream_t
     return forward_per<S, kMaxK / 64>(a, loss, stats, part, st);
 }
 
+// Entries per chunk, were the columns even, from which the chunk takes them through LDS.  MI355X,
+// us, one by one / so: 10.4 entries (8192 x 50257 bf16, k = 256) 322 / 336, 16 (20000 x 2000 bf16)
+// 36 / 31, 26 (8192 x 20000 bf16) 183 / 138, 66 (16384 x 8000 bf16) 291 / 115, 102 (20000 x 2000
+// f32) 218 / 59.
+constexpr int kDense = 12;
+
 template <class S, int PER>
 int backward_per(const Args& a, const float2* stats, const float* dloss, void* dz, bool acc,
                  hipStream_t st) {
@@ -559,12 +643,16 @@ int backward_per(const Args& a, const float2* stats, const float* dloss, void* d
     const int chunks = static_cast<int>(std::max<int64_t>((n + kChunk - 1) / kChunk, 1));
     const int64_t groups = (a.rows * chunks + kWaves - 1) / kWaves;
     const dim3 grid(capped_blocks(groups, kLanes)), block(kLanes);
-    if (acc)
-        hipLaunchKernelGGL((distill_bwd<S, PER, true>), grid, block, 0, st, a, stats, dloss, dz,
-                           chunks);
-    else
-        hipLaunchKernelGGL((distill_bwd<S, PER, false>), grid, block, 0, st, a, stats, dloss, dz,
-                           chunks);
+    constexpr int64_t kCols = kChunk * S::kVec;
+    const bool dense = a.k * kCols >= kDense * std::max(a.cols, kCols);
+#define AGK_BWD(ACC, DENSE)                                                                     \
+    hipLaunchKernelGGL((distill_bwd<S, PER, ACC, DENSE>), grid, block, 0, st, a, stats, dloss,  \
+                       dz, chunks)
+    if (dense && acc) AGK_BWD(true, true);
+    else if (dense) AGK_BWD(false, true);
+    else if (acc) AGK_BWD(true, false);
+    else AGK_BWD(false, false);
+#undef AGK_BWD
     return check_launch();
 }
 template <class S>

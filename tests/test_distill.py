@@ -101,7 +101,8 @@ def test_against_fp64(cuda, dtype, t_dtype, rows, cols, k):
 
 
 @pytest.mark.parametrize("dtype", [F, BF])
-@pytest.mark.parametrize("rows,cols,k", [(5, 1001, 12), (2100, 260, 4), (3, 20000, 64)])
+@pytest.mark.parametrize("rows,cols,k", [(5, 1001, 12), (2100, 260, 4), (3, 20000, 64),
+                                         (33, 1003, 200), (7, 5001, 1000), (500, 2051, 70)])
 def test_in_place_and_accumulation(cuda, dtype, rows, cols, k):
     z, index, t, dloss = inputs(rows, cols, k, dtype)
     dloss[0] = 0.0
