@@ -1218,6 +1218,14 @@ int launch(const RowArgs& args, int64_t rows, int cols, hipStream_t st) {
         const Plan q{pl.tpr / 2, 4, pl.tpr >= 512 ? 1 : 512 / pl.tpr, false};
         if (has_shape(kFwdShapes, q)) pl = q;
     }
+    // fp32 layer norm with weight and bias: two slots per lane from 4096 rows on, as others have
+    // from kLargeRows (MI355X, us, four / two: 6000 x 4096 36.7 / 35.2, 10000 x 3000 46.3 / 43.5,
+    // 16384 x 4096 95.6 / 90.1, x 8192 195 / 185; 3000 x 8192 36.5 / 37.6, 10000 x 2048 29.0 / 29.6)
+    if (std::is_same<Op, LnAffineFwd>::value && std::is_same<S, F32>::value && pl.nv == 4 &&
+        rows > kLargeRows / 4 && cols > 2048) {
+        const Plan q{pl.tpr * 2, 2, 1, false};
+        if (has_shape(kFwdShapes, q)) pl = q;
+    }
     if (!vec && cols >= S::kVec && !few_short_rows<Op, S>(rows, cols) &&
         !prefers_looped_vec<Op, S>(p, rows, cols)) {
         pl = fwd_plan(row_slots(cols, S::kVec), rows);

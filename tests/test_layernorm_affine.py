@@ -95,7 +95,7 @@ def test_against_fp64(cuda, dtype, cols):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,cols", [(70000, 24), (20000, 72), (3000, 1030), (1031, 4096)])
+@pytest.mark.parametrize("rows,cols", [(70000, 24), (20000, 72), (3000, 1030), (1031, 4096), (4100, 2052)])
 def test_many_rows(cuda, dtype, rows, cols):
     x, g, b, dy = inputs(rows, cols, dtype)
     y, mean, rstd = agk.layernorm_affine_fwd(x, g, b, EPS)
