@@ -7,23 +7,21 @@
 namespace agk_xent {
 
 // Few tokens: the short kernel, where its tiles (the smallest) fit a grid.
-template <class KM>
 bool is_short(const Product& p) {
     const int64_t tiles = static_cast<int64_t>((p.M + kShortM - 1) / kShortM) *
                           ((p.N + kShortN - 1) / kShortN);
-    return p.K <= short_k<KM>() && agk::grid_fits(tiles, 256);
+    return p.K <= kShortK && agk::grid_fits(tiles, 256);
 }
 
 int launch_dw(int shape, const Product& p, const AddEpi<true>& e) {
-    if (is_short<agk_gemm::LinearK>(p)) return launch_short<false, true>(p, e);
+    if (is_short(p)) return launch_short<false, true>(p, e);
     return launch_product<false, true>(shape, p, e);
 }
 int launch_dw(int shape, const Product& p, const AddEpi<false>& e) {
-    if (is_short<agk_gemm::LinearK>(p)) return launch_short<false, true>(p, e);
+    if (is_short(p)) return launch_short<false, true>(p, e);
     return launch_product<false, true>(shape, p, e);
 }
 int launch_dw(int shape, const Product& p, const AddEpi<true>& e, const PlanesK& k) {
-    if (is_short<PlanesK>(p)) return launch_short<false, true>(p, e, k);
     return launch_product<false, true>(shape, p, e, k);
 }
 

@@ -501,17 +501,17 @@ __global__ __launch_bounds__(256, SH::kPerCu) void xent_ring_kernel(
 }
 
 // A product of few k (dw of few tokens: an outer product, whose time is its stores): all of K
-// staged at once, one barrier, no ring.  A tile's stages then take 24 KiB, or 48, instead of
-// 64-72, so that six or three workgroups share a CU, and a workgroup's loads and stores hide
-// behind the others'.  LinearK: NKT tiles of 64; PlanesK: one, in two planes.  dw in bf16, 4096 x
-// 32000 on MI355X, the shape pick_shape takes / this: 16 tokens 171 / 67 us (4.0 TB/s of stores),
-// 128 tokens 150 / 110.  A row-by-row order of the tiles changes little (62-76, 119).
-constexpr int kShortM = 64, kShortN = 128;
+// staged at once, one barrier, no ring.  A tile's stages (NKT tiles of 64 k) then take 24 KiB, or
+// 48, instead of 64-72, so that six or three workgroups share a CU, and a workgroup's loads and
+// stores hide behind the others'.  dw in bf16, 4096 x 32000 on MI355X, the shape pick_shape takes
+// / this: 16 tokens 171 / 67 us (4.0 TB/s of stores), 128 tokens 150 / 110.  A row-by-row order of
+// the tiles changes little (62-76, 119).
+constexpr int kShortM = 64, kShortN = 128, kShortK = 128;
 
-template <bool A_TR, bool B_TR, int NKT, class Epi, class KM>
+template <bool A_TR, bool B_TR, int NKT, class Epi>
 __global__ __launch_bounds__(256, NKT == 1 ? 6 : 3) void xent_short_kernel(
     const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int M,
-    int N, int K, const Epi epi, const KM km, int tiles_m, int tiles_n) {
+    int N, int K, const Epi epi, int tiles_m, int tiles_n) {
     using namespace agk_gemm;
     using SH = RingShape<kShortM, kShortN, 2, 3>;
     __shared__ __attribute__((aligned(16))) uint16_t lds[NKT][SH::kElems];
@@ -525,14 +525,11 @@ __global__ __launch_bounds__(256, NKT == 1 ? 6 : 3) void xent_short_kernel(
     const int rows_b = N - n0 < kShortN ? N - n0 : kShortN;
     const uint16_t* const a0 = A_TR ? A + m0 : A + static_cast<int64_t>(m0) * lda;
     const uint16_t* const b0 = B_TR ? B + n0 : B + static_cast<int64_t>(n0) * ldb;
-    constexpr bool kPlanes = !std::is_same<KM, LinearK>::value;
 #pragma unroll
     for (int t = 0; t < NKT; ++t) {
-        if (!kPlanes && t * BK >= K) break;
-        const int64_t pa = kPlanes && t ? km.more_a() / 2 : 0, pb = kPlanes && t ? km.more_b() / 2 : 0;
-        stage_k_tail<A_TR, kShortM>(lds[t], a0 + pa, lda, rows_a, kPlanes ? 0 : t * BK, K);
-        stage_k_tail<B_TR, kShortN>(lds[t] + kShortM * BK, b0 + pb, ldb, rows_b,
-                                    kPlanes ? 0 : t * BK, K);
+        if (t * BK >= K) break;
+        stage_k_tail<A_TR, kShortM>(lds[t], a0, lda, rows_a, t * BK, K);
+        stage_k_tail<B_TR, kShortN>(lds[t] + kShortM * BK, b0, ldb, rows_b, t * BK, K);
     }
     f32x16 acc[SH::kTm][SH::kTn];
 #pragma unroll
@@ -542,12 +539,11 @@ __global__ __launch_bounds__(256, NKT == 1 ? 6 : 3) void xent_short_kernel(
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     __syncthreads();
-    // the walks' stages of A and B: {0, 0}, {0, 1}, {1, 0} for planes, {t, t} for k-tiles
 #pragma unroll
-    for (int t = 0; t < (kPlanes ? 3 : NKT); ++t) {
-        const uint16_t* const sa = lds[kPlanes ? t >> 1 : t];
-        const uint16_t* const sb = lds[kPlanes ? t & 1 : t] + kShortM * BK;
-        const int left = kPlanes ? K : K - t * BK;
+    for (int t = 0; t < NKT; ++t) {
+        const uint16_t* const sa = lds[t];
+        const uint16_t* const sb = sa + kShortM * BK;
+        const int left = K - t * BK;
         for (int s = 0; s * 16 < left && s < BK / 16; ++s) {
             RingFrags<SH::kTm, SH::kTn> f;
 #pragma unroll
@@ -556,31 +552,23 @@ __global__ __launch_bounds__(256, NKT == 1 ? 6 : 3) void xent_short_kernel(
 #pragma unroll
             for (int j = 0; j < SH::kTn; ++j)
                 f.b[j] = ring_frag<B_TR, kShortN>(sb, (wn * SH::kTn + j) * 32, s, lane);
-            ring_mfma<KM::kF16>(f, acc);
+            ring_mfma<false>(f, acc);
         }
     }
     epi(acc, m0 + wm * SH::kTm * 32, n0 + wn * SH::kTn * 32, lane);
 }
 
-// The most k it takes, and its launch.
-template <class KM>
-constexpr int short_k() {
-    return std::is_same<KM, agk_gemm::LinearK>::value ? 128 : 64;
-}
-template <bool A_TR, bool B_TR, class Epi, class KM = agk_gemm::LinearK>
-int launch_short(const Product& p, const Epi& e, const KM& km = {}) {
+// K at most kShortK.
+template <bool A_TR, bool B_TR, class Epi>
+int launch_short(const Product& p, const Epi& e) {
     const int tiles_m = (p.M + kShortM - 1) / kShortM, tiles_n = (p.N + kShortN - 1) / kShortN;
     const dim3 grid(tiles_m * tiles_n), block(256);
-    constexpr bool kPlanes = !std::is_same<KM, agk_gemm::LinearK>::value;
-    if constexpr (!kPlanes) {
-        if (p.K <= agk_gemm::BK) {
-            hipLaunchKernelGGL((xent_short_kernel<A_TR, B_TR, 1, Epi, KM>), grid, block, 0, p.st,
-                               p.A, p.lda, p.B, p.ldb, p.M, p.N, p.K, e, km, tiles_m, tiles_n);
-            return agk::check_launch();
-        }
-    }
-    hipLaunchKernelGGL((xent_short_kernel<A_TR, B_TR, 2, Epi, KM>), grid, block, 0, p.st, p.A,
-                       p.lda, p.B, p.ldb, p.M, p.N, p.K, e, km, tiles_m, tiles_n);
+    if (p.K <= agk_gemm::BK)
+        hipLaunchKernelGGL((xent_short_kernel<A_TR, B_TR, 1, Epi>), grid, block, 0, p.st, p.A,
+                           p.lda, p.B, p.ldb, p.M, p.N, p.K, e, tiles_m, tiles_n);
+    else
+        hipLaunchKernelGGL((xent_short_kernel<A_TR, B_TR, 2, Epi>), grid, block, 0, p.st, p.A,
+                           p.lda, p.B, p.ldb, p.M, p.N, p.K, e, tiles_m, tiles_n);
     return agk::check_launch();
 }
 
