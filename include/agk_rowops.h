@@ -72,11 +72,10 @@ int agk_layernorm_bwd(const void* x, const float* mean, const float* rstd,
                       int dtype, int accumulate, agk_stream_t stream);
 
 /* LayerNorm with weight and bias, y = (x - mean) * rstd * gamma + beta; gamma
- * and beta [cols] of the storage type, NULL for none (ones, zeros; both NULL is
- * agk_layernorm_fwd).  Saves mean[rows] and rstd[rows] = 1/sqrt(var + eps) in
- * fp32, the variance as in agk_layernorm_fwd.  y may be x itself.  The
- * reference's layer has no weight and bias (laynor_nodeops,
- * cgadimpl/src/ops/normalization.cpp:10-22).                                 */
+ * and beta [cols] of the storage type, NULL for none (ones, zeros).  Saves
+ * mean[rows] and rstd[rows] = 1/sqrt(var + eps) in fp32, the variance as in
+ * agk_layernorm_fwd.  y may be x itself.  The reference's layer has no weight
+ * and bias (laynor_nodeops, cgadimpl/src/ops/normalization.cpp:10-22).       */
 int agk_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta, void* y,
                              float* mean, float* rstd, int64_t rows, int64_t cols, float eps,
                              int dtype, agk_stream_t stream);

@@ -293,3 +293,16 @@ def test_wide_rows_several_to_a_workgroup(cuda, dtype, rows, cols):
         check(got, total, tol + 2 * r * (total.abs() + tol), "accumulated")
     only = agk.layernorm_affine_bwd(x, g, mean, rstd, dy, want_dx=False)
     assert only[0] is None and torch.equal(only[1], dg) and torch.equal(only[2], db)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(300, 16383), (4100, 2052), (600, 8193), (20, 9001)])
+def test_wide_rows_in_place(cuda, dtype, rows, cols):
+    x, g, b, dy = inputs(rows, cols, dtype, seed=8)
+    y, mean, rstd = agk.layernorm_affine_fwd(x, g, b, EPS)
+    dx, dg, db = agk.layernorm_affine_bwd(x, g, mean, rstd, dy)
+    xc, dyc = x.clone(), dy.clone()
+    _, m2, r2 = agk.layernorm_affine_fwd(xc, g, b, EPS, y=xc)
+    assert torch.equal(xc, y) and torch.equal(m2, mean) and torch.equal(r2, rstd)
+    _, dg2, db2 = agk.layernorm_affine_bwd(x, g, mean, rstd, dyc, dx=dyc)
+    assert torch.equal(dyc, dx) and torch.equal(dg2, dg) and torch.equal(db2, db)
